@@ -41,7 +41,10 @@ extern "C" {
 #define PHANTOM_ATTN_ERR_CUDA 3        /* a CUDA runtime or driver call failed                */
 #define PHANTOM_ATTN_ERR_DEVICE 4      /* a device-side bounded wait expired (status word)    */
 
-/* Library version, e.g. 10000 for 1.0.0. */
+/* cache dtype of the paged entry points only: 8-bit integers with a scale for each token and head */
+#define PHANTOM_ATTN_I8 3
+
+/* Library version, e.g. 10100 for 1.1.0. */
 int phantom_attn_version(void);
 
 /* Message for the last failing call on this thread ("" if none). Valid until the next call. */
@@ -193,6 +196,68 @@ int phantom_attn_get_launch_shape(long long* l2_group_kib, int* max_ctas);
  */
 int phantom_attn_set_kv_parts(int allow);
 int phantom_attn_get_kv_parts(void);
+
+/* ---------------------------------------------------------------------------- paged key/value cache
+ *
+ * The serving side: ragged batches of sequences whose keys and values live in pages of a pool. No counterpart in the
+ * reference. Token t of sequence b lies in page page_table[b * table_stride + t / page_size], at place t % page_size;
+ * kv_lens[b] tokens of it are cached, and the last cu_new[b + 1] - cu_new[b] of those are its new tokens, which the packed
+ * (total_new, heads, head_dim) arrays of a call hold one sequence after another (cu_new[0] = 0, cu_new[batch] = total_new).
+ * Lengths, offsets and page ids are device data (32-bit): calls do not synchronise, and can be captured in a graph.
+ * Sequences may share pages that are only read. What the table or the lengths give out of range is never followed: such
+ * tokens are not written and read as zeros, and PHANTOM_ATTN_STATUS_PAGE is set in the device status word.
+ *
+ * Two kinds of cache: 16-bit (dtype PHANTOM_ATTN_F16 / BF16, values as they are), and 8-bit (PHANTOM_ATTN_I8) with fp32
+ * scales: a vector x (one token, one head) is held as q = round(127 x / top), ties to even, and scale = top / 127 with
+ * top = max(max|x|, 127 * 2^-100), and stands for q * scale. A vector with an infinity or a NaN gets the scale NaN.
+ *
+ * Strides count elements. The innermost (head_dim) extent is contiguous; every pointer and every stride of the 16- and
+ * 8-bit arrays is a multiple of 16 bytes. Scales are contiguous over a page's tokens, their other strides multiples of 4.
+ * head_dim is 64 or 128, page_size a power of two from 16 to 1024.
+ */
+typedef struct phantom_paged_cache {
+  void* k;                      /* (num_pages, heads, page_size, head_dim) by the strides below */
+  void* v;
+  float* k_scale;               /* (num_pages, heads, page_size); NULL unless dtype is PHANTOM_ATTN_I8 */
+  float* v_scale;
+  long long k_stride[3];        /* page, head, token */
+  long long v_stride[3];
+  long long k_scale_stride[2];  /* page, head */
+  long long v_scale_stride[2];
+  const int* page_table;        /* (batch, table_width), rows table_stride entries apart */
+  const int* kv_lens;           /* (batch) */
+  const int* cu_new;            /* (batch + 1) */
+  int batch;
+  int table_width;
+  int table_stride;
+  int num_pages;
+  int page_size;
+  int heads;
+  int head_dim;
+  int dtype;
+} phantom_paged_cache;
+
+/* Writes the new tokens' keys and values k, v (total_new, heads, head_dim; strides of token and head) into the cache, in
+ * the type dtype (PHANTOM_ATTN_F16 / BF16) or quantised from it. Two new tokens must not share a place. */
+int phantom_attn_paged_append(const phantom_paged_cache* cache, const void* k, const void* v, long long k_token,
+                              long long k_head, long long v_token, long long v_head, int total_new, int dtype, void* stream);
+
+/* The inverse: the keys and values that the cache holds of the new tokens (all of a sequence where cu_new counts
+ * kv_lens[b] of them), to contiguous k, v (total_new, heads, head_dim) of type dtype. */
+int phantom_attn_paged_read(const phantom_paged_cache* cache, void* k, void* v, int total_new, int dtype, void* stream);
+
+/* Attention of the new tokens over all cached tokens of their sequences: q (total_new, q_heads, head_dim; strides of token
+ * and head), o (total_new, q_heads, head_dim) contiguous, of type dtype, which is the cache's unless that is
+ * PHANTOM_ATTN_I8. Query head h reads key head h / (q_heads / heads). New token i of n sees the first kv_len - n + i + 1
+ * tokens of its sequence if causal, all of them otherwise; a token that sees none gets zeros. Scores are multiplied by
+ * scale (0: 1 / sqrt(head_dim)). max_new is the largest number of new tokens of a sequence, as the caller expects it: a
+ * hint that picks the kernel, not a limit (0: the average). Values cached within the length must be finite even where the
+ * causal mask hides them; what lies past the length may be anything. */
+int phantom_attn_paged(const phantom_paged_cache* cache, const void* q, long long q_token, long long q_head, void* o,
+                       int total_new, int q_heads, int dtype, int causal, float scale, int max_new, void* stream);
+
+/* device_status bit: a length, an offset or a page id of a paged call was out of range */
+#define PHANTOM_ATTN_STATUS_PAGE 512
 
 #ifdef __cplusplus
 }

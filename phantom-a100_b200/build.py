@@ -33,8 +33,8 @@ NVCC = os.path.join(CUDA_HOME, "bin", "nvcc")
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 NVCC_FLAGS = ["-O3", "-lineinfo", "-std=c++17", "-Xcompiler", "-fPIC", "-Xcompiler", "-Wall"] + ARCH
 
-KERNEL_SOURCES = ["attn_tc_sm100.cu", "attn_simt.cu", "capi.cu"]
-HEADERS = ["sm100_ptx.cuh", "launchers.h"]
+KERNEL_SOURCES = ["attn_tc_sm100.cu", "attn_simt.cu", "attn_paged.cu", "paged_cache.cu", "capi.cu"]
+HEADERS = ["sm100_ptx.cuh", "launchers.h", "paged.h", "paged_dev.cuh"]
 LIB_NAME = "libphantom_attn.so"
 
 

@@ -49,6 +49,7 @@
 #include <mutex>
 
 #include "launchers.h"
+#include "paged.h"
 #include "sm100_ptx.cuh"
 #include "../../include/phantom_attn.h"
 
@@ -1371,6 +1372,70 @@ cudaError_t scratch_usage(int dev, long long* high_water, long long* reserved, b
   *high_water = (long long)hw;
   *reserved = (long long)rs;
   return e;
+}
+
+cudaError_t sm_count(int dev, int* n) {
+  if (dev < 0 || dev >= kMaxDevices) return cudaErrorInvalidDevice;
+  *n = g_sm_count[dev].load(std::memory_order_relaxed);
+  if (*n != 0) return cudaSuccess;
+  const cudaError_t e = cudaDeviceGetAttribute(n, cudaDevAttrMultiProcessorCount, dev);
+  if (e == cudaSuccess) g_sm_count[dev].store(*n, std::memory_order_relaxed);
+  return e;
+}
+
+cudaError_t scratch_alloc(int dev, size_t bytes, cudaStream_t stream, void** out) {
+  cudaMemPool_t pool;
+  const cudaError_t e = device_pool(dev, &pool);
+  return e != cudaSuccess ? e : cudaMallocFromPoolAsync(out, bytes, pool, stream);
+}
+
+namespace {
+
+// Per-thread cache of the paged maps, as for the contiguous ones above (a map is a pure function of its key).
+struct PagedMapEntry {
+  CUtensorMap map;
+  const void* base = nullptr;
+  int pages = 0, heads = 0, page = 0, d = 0, elem = 0, rows = 0, cols = 0;
+  Strides3 st{};
+  bool bf16 = false, valid = false;
+};
+thread_local PagedMapEntry g_paged_maps[kMapCache];
+thread_local int g_paged_next = 0;
+
+}  // namespace
+
+bool make_paged_map(void* out, const void* base, int num_pages, int heads, int page, int d, const Strides3& st, int elem,
+                    bool bf16, int rows, int cols) {
+  CUtensorMap* m = static_cast<CUtensorMap*>(out);
+  for (const PagedMapEntry& e : g_paged_maps)
+    if (e.valid && e.base == base && e.pages == num_pages && e.heads == heads && e.page == page && e.d == d &&
+        e.elem == elem && e.rows == rows && e.cols == cols && e.bf16 == bf16 && e.st.page == st.page &&
+        e.st.head == st.head && e.st.token == st.token) {
+      *m = e.map;
+      return true;
+    }
+  EncodeTiledFn fn = encode_fn();
+  if (!fn) return false;
+  const cuuint64_t dims[4] = {(cuuint64_t)d, (cuuint64_t)page, (cuuint64_t)heads, (cuuint64_t)num_pages};
+  const cuuint64_t strides[3] = {(cuuint64_t)st.token * elem, (cuuint64_t)st.head * elem, (cuuint64_t)st.page * elem};
+  const cuuint32_t box[4] = {(cuuint32_t)cols, (cuuint32_t)rows, 1, 1};
+  const cuuint32_t estr[4] = {1, 1, 1, 1};
+  const CUtensorMapDataType type = elem == 1 ? CU_TENSOR_MAP_DATA_TYPE_UINT8
+                                   : bf16    ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
+                                             : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+  if (fn(m, type, 4, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+         cols * elem == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+         CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
+    return false;
+  PagedMapEntry& e = g_paged_maps[g_paged_next];
+  g_paged_next = (g_paged_next + 1) % kMapCache;
+  e.map = *m;
+  e.base = base;
+  e.pages = num_pages, e.heads = heads, e.page = page, e.d = d, e.elem = elem, e.rows = rows, e.cols = cols;
+  e.st = st;
+  e.bf16 = bf16;
+  e.valid = true;
+  return true;
 }
 
 cudaError_t launch_wait_expiry_probe(int* status, int* status2, cudaStream_t stream) {

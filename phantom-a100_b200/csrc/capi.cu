@@ -3,6 +3,7 @@
 // attn_fused_tuned.cu:5-21), keeps its error substrings, and dispatches to the sm_100a kernels.
 #include <cuda_runtime.h>
 
+#include <cmath>
 #include <cstdarg>
 #include <cstdio>
 #include <mutex>
@@ -11,6 +12,7 @@
 #include <vector>
 
 #include "launchers.h"
+#include "paged.h"
 #include "../../include/phantom_attn.h"
 
 namespace phantom {
@@ -201,6 +203,102 @@ int noalloc_setup(const char* name, int dev, unsigned char** scratch, int* cc, i
   return PHANTOM_ATTN_OK;
 }
 
+// ------------------------------------------------------------------ paged cache
+// One device pointer of a paged call, 16-byte aligned unless it is an int array (4 bytes).
+int check_paged_ptr(const char* name, const char* what, const void* p, int dev, int align) {
+  if (p == nullptr) return fail(PHANTOM_ATTN_ERR_INVALID, "%s: inputs must be CUDA tensors (%s is a null pointer)", name, what);
+  cudaPointerAttributes attr;
+  if (cudaPointerGetAttributes(&attr, p) != cudaSuccess) {
+    cudaGetLastError();
+    return fail(PHANTOM_ATTN_ERR_INVALID, "%s: inputs must be CUDA tensors (%s)", name, what);
+  }
+  if (attr.type != cudaMemoryTypeDevice && attr.type != cudaMemoryTypeManaged)
+    return fail(PHANTOM_ATTN_ERR_INVALID, "%s: inputs must be CUDA tensors (%s)", name, what);
+  if (attr.type == cudaMemoryTypeDevice && attr.device != dev)
+    return fail(PHANTOM_ATTN_ERR_INVALID, "%s: all tensors must be on the same device (%s; current device %d)", name, what, dev);
+  if (reinterpret_cast<uintptr_t>(p) % align != 0)
+    return fail(PHANTOM_ATTN_ERR_INVALID, "%s: %s must be %d-byte aligned", name, what, align);
+  return PHANTOM_ATTN_OK;
+}
+
+// A stride of an array of `elem`-byte elements: positive or zero, a multiple of 16 bytes, below TMA's 2^40 bytes.
+bool stride_ok(long long st, int elem) { return st >= 0 && st * elem % 16 == 0 && st < (1LL << 40) / elem; }
+
+// What every paged call checks, host-only first. dtype: of the packed 16-bit arrays.
+int check_paged(const char* name, const phantom_paged_cache* c, int total, int dtype, Device* dev, PagedSeqs* s) {
+  if (c == nullptr) return fail(PHANTOM_ATTN_ERR_INVALID, "%s: null cache", name);
+  if (c->batch <= 0 || total <= 0 || c->heads <= 0 || c->num_pages <= 0 || c->table_width <= 0)
+    return fail(PHANTOM_ATTN_ERR_INVALID, "%s: inputs must be non-empty", name);
+  if (c->head_dim != 64 && c->head_dim != 128)
+    return fail(PHANTOM_ATTN_ERR_UNSUPPORTED, "%s: only head dimension 64 and 128 are compiled (got %d)", name, c->head_dim);
+  if (dtype != PHANTOM_ATTN_F16 && dtype != PHANTOM_ATTN_BF16)
+    return fail(PHANTOM_ATTN_ERR_UNSUPPORTED, "%s: float16 or bfloat16 only (got dtype code %d)", name, dtype);
+  if (c->dtype != dtype && c->dtype != PHANTOM_ATTN_I8)
+    return fail(PHANTOM_ATTN_ERR_INVALID, "%s: the cache must have the inputs' dtype, or int8 (got dtype code %d)", name, c->dtype);
+  if (c->page_size < 16 || c->page_size > 1024 || (c->page_size & (c->page_size - 1)) != 0)
+    return fail(PHANTOM_ATTN_ERR_UNSUPPORTED, "%s: page size must be a power of two from 16 to 1024 (got %d)", name, c->page_size);
+  if (c->batch > 65535 || c->heads > 65535)
+    return fail(PHANTOM_ATTN_ERR_UNSUPPORTED, "%s: batch = %d or heads = %d exceeds 65535", name, c->batch, c->heads);
+  if (c->table_stride < c->table_width)
+    return fail(PHANTOM_ATTN_ERR_INVALID, "%s: page table rows overlap (stride %d, width %d)", name, c->table_stride, c->table_width);
+  const bool int8 = c->dtype == PHANTOM_ATTN_I8;
+  for (int i = 0; i < 3; ++i)
+    if (!stride_ok(c->k_stride[i], int8 ? 1 : 2) || !stride_ok(c->v_stride[i], int8 ? 1 : 2))
+      return fail(PHANTOM_ATTN_ERR_INVALID, "%s: cache strides must be multiples of 16 bytes", name);
+  if (int8)
+    for (int i = 0; i < 2; ++i)
+      if (!stride_ok(c->k_scale_stride[i], 4) || !stride_ok(c->v_scale_stride[i], 4))
+        return fail(PHANTOM_ATTN_ERR_INVALID, "%s: scale strides must be multiples of 16 bytes", name);
+  int rc = current_device(name, dev);
+  if (rc != PHANTOM_ATTN_OK) return rc;
+  if (dev->cc != 100)
+    return fail(PHANTOM_ATTN_ERR_UNSUPPORTED, "%s: the paged kernels are compiled for sm_100a (B200); this GPU is sm_%d", name,
+                dev->cc);
+  if ((rc = check_paged_ptr(name, "k_cache", c->k, dev->id, 16)) != PHANTOM_ATTN_OK ||
+      (rc = check_paged_ptr(name, "v_cache", c->v, dev->id, 16)) != PHANTOM_ATTN_OK ||
+      (rc = check_paged_ptr(name, "page_table", c->page_table, dev->id, 4)) != PHANTOM_ATTN_OK ||
+      (rc = check_paged_ptr(name, "kv_lens", c->kv_lens, dev->id, 4)) != PHANTOM_ATTN_OK ||
+      (rc = check_paged_ptr(name, "cu_new", c->cu_new, dev->id, 4)) != PHANTOM_ATTN_OK)
+    return rc;
+  if (int8 && ((rc = check_paged_ptr(name, "k_scale", c->k_scale, dev->id, 16)) != PHANTOM_ATTN_OK ||
+               (rc = check_paged_ptr(name, "v_scale", c->v_scale, dev->id, 16)) != PHANTOM_ATTN_OK))
+    return rc;
+  int page_log2 = 0;
+  while ((1 << page_log2) < c->page_size) ++page_log2;
+  *s = PagedSeqs{c->page_table, c->kv_lens, c->cu_new, c->batch, c->table_width, c->table_stride, total, c->num_pages,
+                 page_log2, c->heads, dev->status};
+  return PHANTOM_ATTN_OK;
+}
+
+int paged_copy(const char* name, const phantom_paged_cache* c, const void* k, const void* v, long long k_token,
+               long long k_head, long long v_token, long long v_head, int total, int dtype, void* stream,
+               cudaError_t (*launch)(const PagedCopyArgs&)) {
+  Device dev;
+  PagedCopyArgs a{};
+  int rc = check_paged(name, c, total, dtype, &dev, &a.s);
+  if (rc != PHANTOM_ATTN_OK) return rc;
+  if (!stride_ok(k_token, 2) || !stride_ok(k_head, 2) || !stride_ok(v_token, 2) || !stride_ok(v_head, 2))
+    return fail(PHANTOM_ATTN_ERR_INVALID, "%s: strides of k and v must be multiples of 16 bytes", name);
+  if ((rc = check_paged_ptr(name, "k", k, dev.id, 16)) != PHANTOM_ATTN_OK ||
+      (rc = check_paged_ptr(name, "v", v, dev.id, 16)) != PHANTOM_ATTN_OK)
+    return rc;
+  a.k = const_cast<void*>(k), a.v = const_cast<void*>(v);
+  a.k_token = k_token, a.k_head = k_head, a.v_token = v_token, a.v_head = v_head;
+  a.kc = c->k, a.vc = c->v, a.ks = c->k_scale, a.vs = c->v_scale;
+  a.kcs = Strides3{c->k_stride[0], c->k_stride[1], c->k_stride[2]};
+  a.vcs = Strides3{c->v_stride[0], c->v_stride[1], c->v_stride[2]};
+  a.kss = Strides3{c->k_scale_stride[0], c->k_scale_stride[1], 1};
+  a.vss = Strides3{c->v_scale_stride[0], c->v_scale_stride[1], 1};
+  a.d = c->head_dim;
+  a.bf16 = dtype == PHANTOM_ATTN_BF16;
+  a.int8 = c->dtype == PHANTOM_ATTN_I8;
+  a.stream = static_cast<cudaStream_t>(stream);
+  const cudaError_t e = launch(a);
+  if (e != cudaSuccess) return cuda_fail(name, e);
+  g_last_error.clear();
+  return PHANTOM_ATTN_OK;
+}
+
 // Reads and clears one status word (the device is already synchronised). Returns the CUDA error.
 cudaError_t take_status_word(int* word, int* out) {
   *out = 0;
@@ -244,7 +342,7 @@ using namespace phantom;
 
 extern "C" {
 
-int phantom_attn_version(void) { return 10000; }
+int phantom_attn_version(void) { return 10100; }
 
 const char* phantom_attn_last_error(void) { return g_last_error.c_str(); }
 
@@ -323,6 +421,52 @@ int phantom_attn_fused_tc_noalloc(const void* q, const void* k, const void* v, v
   return PHANTOM_ATTN_OK;
 }
 
+int phantom_attn_paged_append(const phantom_paged_cache* cache, const void* k, const void* v, long long k_token,
+                              long long k_head, long long v_token, long long v_head, int total_new, int dtype, void* stream) {
+  return paged_copy("paged_append", cache, k, v, k_token, k_head, v_token, v_head, total_new, dtype, stream, launch_paged_append);
+}
+
+int phantom_attn_paged_read(const phantom_paged_cache* cache, void* k, void* v, int total_new, int dtype, void* stream) {
+  const long long d = cache ? cache->head_dim : 0, token = cache ? cache->heads * d : 0;
+  return paged_copy("paged_read", cache, k, v, token, d, token, d, total_new, dtype, stream, launch_paged_read);
+}
+
+int phantom_attn_paged(const phantom_paged_cache* cache, const void* q, long long q_token, long long q_head, void* o,
+                       int total_new, int q_heads, int dtype, int causal, float scale, int max_new, void* stream) {
+  const char* name = "paged_attn";
+  Device dev;
+  PagedAttnArgs a{};
+  int rc = check_paged(name, cache, total_new, dtype, &dev, &a.s);
+  if (rc != PHANTOM_ATTN_OK) return rc;
+  if (q_heads <= 0 || q_heads % cache->heads != 0 || q_heads / cache->heads > 128)
+    return fail(PHANTOM_ATTN_ERR_INVALID, "%s: query heads must be 1 to 128 times the key heads (got %d and %d)", name, q_heads,
+                cache->heads);
+  if (max_new < 0 || !(scale - scale == 0.f))
+    return fail(PHANTOM_ATTN_ERR_INVALID, "%s: max_new must not be negative and scale must be finite", name);
+  if (!stride_ok(q_token, 2) || !stride_ok(q_head, 2))
+    return fail(PHANTOM_ATTN_ERR_INVALID, "%s: strides of q must be multiples of 16 bytes", name);
+  if ((rc = check_paged_ptr(name, "q", q, dev.id, 16)) != PHANTOM_ATTN_OK ||
+      (rc = check_paged_ptr(name, "o", o, dev.id, 16)) != PHANTOM_ATTN_OK)
+    return rc;
+  a.q = q, a.q_token = q_token, a.q_head = q_head, a.o = o;
+  a.kc = cache->k, a.vc = cache->v, a.ks = cache->k_scale, a.vs = cache->v_scale;
+  a.kcs = Strides3{cache->k_stride[0], cache->k_stride[1], cache->k_stride[2]};
+  a.vcs = Strides3{cache->v_stride[0], cache->v_stride[1], cache->v_stride[2]};
+  a.kss = Strides3{cache->k_scale_stride[0], cache->k_scale_stride[1], 1};
+  a.vss = Strides3{cache->v_scale_stride[0], cache->v_scale_stride[1], 1};
+  a.group = q_heads / cache->heads;
+  a.d = cache->head_dim;
+  a.bf16 = dtype == PHANTOM_ATTN_BF16;
+  a.int8 = cache->dtype == PHANTOM_ATTN_I8;
+  a.causal = causal != 0;
+  a.scale = scale != 0.f ? scale : 1.f / sqrtf((float)cache->head_dim);
+  a.stream = static_cast<cudaStream_t>(stream);
+  const cudaError_t e = launch_paged_attn_rows(a, dev.id);
+  if (e != cudaSuccess) return cuda_fail(name, e);
+  g_last_error.clear();
+  return PHANTOM_ATTN_OK;
+}
+
 int phantom_attn_device_status(int* status) {
   if (status == nullptr) return fail(PHANTOM_ATTN_ERR_INVALID, "device_status: null output pointer");
   *status = 0;
@@ -349,7 +493,9 @@ int phantom_attn_device_status(int* status) {
   const int v = v_main | (v_noalloc != 0 ? v_noalloc | PHANTOM_ATTN_STATUS_NOALLOC : 0);
   *status = v;
   g_last_error.clear();
-  return v == 0 ? PHANTOM_ATTN_OK : fail(PHANTOM_ATTN_ERR_DEVICE, "device status 0x%x: a bounded wait expired", v);
+  return v == 0 ? PHANTOM_ATTN_OK : fail(PHANTOM_ATTN_ERR_DEVICE, "device status 0x%x: %s", v,
+                                           v == PHANTOM_ATTN_STATUS_PAGE ? "a paged call's length, offset or page id was out of range"
+                                                                         : "a bounded wait expired");
 }
 
 int phantom_attn_wait_expiry_probe(void* stream) {

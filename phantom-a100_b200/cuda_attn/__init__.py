@@ -11,6 +11,8 @@ Same names, signatures and error behaviour as the reference API (cuda_attn/__ini
   reference                                    fp32 math-backend SDPA, the ground truth of the tests.
   fused_tc_host                                fused_tc for host (pinned) tensors: head chunks streamed
                                                through the GPU with copies overlapping the kernel.
+  paged_append, paged_read, paged_attn         serving: a paged key/value cache (16-bit, or int8 with scales) of
+                                               ragged sequences, and attention of their new tokens over it.
 
 The kernels live in libphantom_attn.so (C ABI: include/phantom_attn.h); `_C` is the PyTorch
 extension over it. There is no CPU fallback: if the extension is missing, every kernel call raises.
@@ -90,6 +92,7 @@ def device_status() -> int:
     return _ext().device_status()
 
 
+from .paged import paged_append, paged_attn, paged_read  # noqa: E402  (paged key/value cache)
 from .pipeline import fused_tc_host  # noqa: E402  (host-resident inputs, copies overlapped with compute)
 
 # Every version, in the order the reference builds them.
@@ -99,4 +102,5 @@ KERNELS = {"naive": naive, "tiled": tiled, "fused": fused,
 FP16_ONLY = {"fused_vec", "fused_db", "fused_tc"}
 
 __all__ = ["naive", "tiled", "fused", "fused_tuned", "fused_vec", "fused_db", "fused_tc",
-           "reference", "KERNELS", "FP16_ONLY", "device_status", "fused_tc_host"]
+           "reference", "KERNELS", "FP16_ONLY", "device_status", "fused_tc_host",
+           "paged_append", "paged_read", "paged_attn"]

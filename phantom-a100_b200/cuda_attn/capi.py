@@ -17,8 +17,22 @@ LIB_PATH = os.path.join(HERE, "libphantom_attn.so")
 F32, F16, BF16 = 0, 1, 2
 OK, ERR_INVALID, ERR_UNSUPPORTED, ERR_CUDA, ERR_DEVICE = 0, 1, 2, 3, 4
 
+I8 = 3  # cache dtype of the paged entry points
+
 _P = ctypes.c_void_p
 _I = ctypes.c_int
+_L = ctypes.c_longlong
+
+
+class PagedCache(ctypes.Structure):
+    """phantom_paged_cache of include/phantom_attn.h."""
+    _fields_ = [("k", _P), ("v", _P), ("k_scale", _P), ("v_scale", _P), ("k_stride", _L * 3), ("v_stride", _L * 3),
+                ("k_scale_stride", _L * 2), ("v_scale_stride", _L * 2), ("page_table", _P), ("kv_lens", _P), ("cu_new", _P),
+                ("batch", _I), ("table_width", _I), ("table_stride", _I), ("num_pages", _I), ("page_size", _I),
+                ("heads", _I), ("head_dim", _I), ("dtype", _I)]
+
+
+_C = ctypes.POINTER(PagedCache)
 # name -> (restype, argtypes); mirrors include/phantom_attn.h
 SIGNATURES = {
     "phantom_attn_version": (_I, []),
@@ -29,6 +43,9 @@ SIGNATURES = {
     "phantom_attn_fused": (_I, [_P, _P, _P, _P, _I, _I, _I, _I, _I, _P]),
     "phantom_attn_naive": (_I, [_P, _P, _P, _P, _I, _I, _I, _I, _I, _P]),
     "phantom_attn_tiled": (_I, [_P, _P, _P, _P, _I, _I, _I, _I, _I, _P]),
+    "phantom_attn_paged_append": (_I, [_C, _P, _P, _L, _L, _L, _L, _I, _I, _P]),
+    "phantom_attn_paged_read": (_I, [_C, _P, _P, _I, _I, _P]),
+    "phantom_attn_paged": (_I, [_C, _P, _L, _L, _P, _I, _I, _I, _I, ctypes.c_float, _I, _P]),
     "phantom_attn_device_status": (_I, [ctypes.POINTER(ctypes.c_int)]),
     "phantom_attn_wait_expiry_probe": (_I, [_P]),
     "phantom_attn_launch_count": (ctypes.c_longlong, [_I]),
