@@ -33,7 +33,7 @@ NVCC = os.path.join(CUDA_HOME, "bin", "nvcc")
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 NVCC_FLAGS = ["-O3", "-lineinfo", "-std=c++17", "-Xcompiler", "-fPIC", "-Xcompiler", "-Wall"] + ARCH
 
-KERNEL_SOURCES = ["attn_tc_sm100.cu", "attn_simt.cu", "attn_paged.cu", "paged_cache.cu", "capi.cu"]
+KERNEL_SOURCES = ["attn_tc_sm100.cu", "attn_simt.cu", "attn_paged.cu", "attn_paged_tc_sm100.cu", "paged_cache.cu", "capi.cu"]
 HEADERS = ["sm100_ptx.cuh", "launchers.h", "paged.h", "paged_dev.cuh"]
 LIB_NAME = "libphantom_attn.so"
 

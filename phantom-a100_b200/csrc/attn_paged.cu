@@ -58,6 +58,21 @@ struct Cfg {
   static_assert(SMEM <= 227 * 1024, "shared memory plan exceeds 227 KB");
 };
 
+
+// ------------------------------------------------------------------------------------------------ units and tiles
+// Units of 16 rows; tiles of 64 keys.
+struct RowBlocks {
+  int group, causal, heads;
+  static constexpr int kTile = BN;
+  __device__ int count(const Seq& x) const { return (x.n * group + BR - 1) / BR; }
+  __device__ int key_end(const Seq& x, int rb) const {
+    if (!causal) return x.len;
+    const int last = min(x.n * group - 1, rb * BR + BR - 1) / group;
+    return min(max(x.len - x.n + last + 1, 0), x.len);
+  }
+  __device__ long long head_tiles(const Seq& x) const { return sum_tiles(*this, x); }
+};
+
 struct Params {
   PagedSeqs s;
   const uint16_t* q;
@@ -65,92 +80,10 @@ struct Params {
   uint16_t* o;
   const float *ks, *vs;
   Strides3 kss, vss;
-  int group, causal;
+  RowBlocks blocks;
   float scale_log2;
   float* part;  // partial results, [CTA][2][BR] rows of D sums of values
   float2* ml;   // their (reference maximum, sum)
-};
-
-// ------------------------------------------------------------------------------------------------ units and tiles
-__device__ __forceinline__ int key_end(const Seq& x, int rb, int group, int causal) {
-  if (!causal) return x.len;
-  const int last = min(x.n * group - 1, rb * BR + BR - 1) / group;
-  return min(max(x.len - x.n + last + 1, 0), x.len);
-}
-// At least one tile, so that rows without any key are written too (as zeros).
-__device__ __forceinline__ int tiles_of(const Seq& x, int rb, int group, int causal) {
-  return max(1, (key_end(x, rb, group, causal) + BN - 1) / BN);
-}
-__device__ __forceinline__ int row_blocks(const Seq& x, int group) { return (x.n * group + BR - 1) / BR; }
-__device__ __forceinline__ long long head_tiles(const Seq& x, int group, int causal) {
-  long long w = 0;
-  for (int rb = row_blocks(x, group) - 1; rb >= 0; --rb) w += tiles_of(x, rb, group, causal);
-  return w;
-}
-
-// A whole warp walks the units in order; every value is uniform over the warp.
-struct Walk {
-  long long total, cur, end;
-  long long head;  // tiles of one head of sequence b
-  Seq x;
-  int b, h, rb, tile, nt;
-
-  __device__ void load(const Params& p) {
-    x = seq_of(p.s, b);
-    head = head_tiles(x, p.group, p.causal);
-  }
-  __device__ void start(const Params& p, int cta, int ctas) {
-    const int lane = threadIdx.x & 31;
-    total = 0;
-    for (int i0 = 0; i0 < p.s.batch; i0 += 32)
-      if (i0 + lane < p.s.batch) total += head_tiles(seq_of(p.s, i0 + lane), p.group, p.causal) * p.s.heads;
-    for (int m = 16; m > 0; m >>= 1) total += __shfl_xor_sync(0xffffffffu, total, m);
-    cur = total * cta / ctas;
-    end = total * (cta + 1) / ctas;
-    if (cur >= end) return;
-    long long before = 0;
-    for (int i0 = 0;; i0 += 32) {
-      long long w = i0 + lane < p.s.batch ? head_tiles(seq_of(p.s, i0 + lane), p.group, p.causal) * p.s.heads : 0;
-      for (int m = 1; m < 32; m <<= 1) {
-        const long long y = __shfl_up_sync(0xffffffffu, w, m);
-        if (lane >= m) w += y;
-      }
-      const unsigned past = __ballot_sync(0xffffffffu, before + w > cur);
-      if (past) {
-        const int at = __ffs(past) - 1;
-        const long long up_to = __shfl_sync(0xffffffffu, w, at > 0 ? at - 1 : 0);
-        b = i0 + at;
-        if (at > 0) before += up_to;
-        break;
-      }
-      before += __shfl_sync(0xffffffffu, w, 31);
-    }
-    load(p);
-    long long r = cur - before;
-    h = (int)(r / head);
-    r -= (long long)h * head;
-    for (rb = 0; r >= (nt = tiles_of(x, rb, p.group, p.causal)); ++rb) r -= nt;
-    tile = (int)r;
-  }
-  // tiles of the current segment: the current unit's that this CTA has
-  __device__ int count() const { return (int)min((long long)(nt - tile), end - cur); }
-  __device__ void advance(const Params& p) {
-    const int c = count();
-    cur += c;
-    if (cur >= end) return;
-    tile = 0;
-    if (++rb == row_blocks(x, p.group)) {
-      rb = 0;
-      if (++h == p.s.heads) {
-        h = 0;
-        do {
-          ++b;
-          load(p);
-        } while (head == 0);
-      }
-    }
-    nt = tiles_of(x, rb, p.group, p.causal);
-  }
 };
 
 // ------------------------------------------------------------------------------------------------ matrix instructions
@@ -174,38 +107,7 @@ __device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], 
                  : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
-// Untiled bulk copy into shared memory (16-byte aligned, a multiple of 16 bytes).
-__device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
-  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst),
-               "l"(src), "r"(bytes), "r"(bar)
-               : "memory");
-}
-__device__ __forceinline__ void tma_load_4d(uint32_t dst, const void* tmap, uint32_t bar, int c0, int c1, int c2, int c3) {
-  asm volatile(
-      "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
-      " [%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(dst),
-      "l"(reinterpret_cast<uint64_t>(tmap)), "r"(c0), "r"(c1), "r"(c2), "r"(c3), "r"(bar)
-      : "memory");
-}
 __device__ __forceinline__ void consumers_meet() { asm volatile("bar.sync 1, 256;" ::: "memory"); }
-
-// Two signed bytes of w (chosen by sel: result bytes [lo, 4, hi, 4], byte 4 = 0x64) as exact fp16 pairs; w already has its
-// sign bits flipped, so a byte u = b + 128 gives the fp16 number 1024 + u.
-template <uint32_t SEL>
-__device__ __forceinline__ uint32_t bytes_f16(uint32_t w) {
-  const uint32_t r = __byte_perm(w, 0x64646464u, SEL);
-  const __half2 x = __hsub2(*reinterpret_cast<const __half2*>(&r), __half2half2(__ushort_as_half(0x6480)));
-  return *reinterpret_cast<const uint32_t*>(&x);
-}
-// Two signed bytes as exact bf16 pairs (SEL: result bytes [lo, 0, hi, 0]): with sign bit s and low bits u, 128 + u and
-// 128 + 128 s are both bf16 numbers, and b is their difference.
-template <uint32_t SEL>
-__device__ __forceinline__ uint32_t bytes_bf16(uint32_t w) {
-  const uint32_t r = __byte_perm(w, 0, SEL);
-  const uint32_t lo = (r & 0x007F007Fu) | 0x43004300u, hi = (r & 0x00800080u) | 0x43004300u;
-  const __nv_bfloat162 x = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&lo), *reinterpret_cast<const __nv_bfloat162*>(&hi));
-  return *reinterpret_cast<const uint32_t*>(&x);
-}
 
 template <int D, bool BF16, bool INT8>
 __global__ void __launch_bounds__(kThreads, 1)
@@ -231,8 +133,9 @@ attn_rows(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUten
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   asm volatile("griddepcontrol.wait;" ::: "memory");
 
-  Walk w;
-  w.start(p, blockIdx.x, gridDim.x);
+  Walk<RowBlocks> w;
+  w.start(p.s, p.blocks, blockIdx.x, gridDim.x);
+  const int group = p.blocks.group, causal = p.blocks.causal;
   const long long begin = w.cur;
 
   if (warp == kConsumers) {
@@ -244,7 +147,7 @@ attn_rows(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUten
     int t = 0;
     bool ok = true;
     while (ok && w.cur < w.end) {
-      const int end = key_end(w.x, w.rb, p.group, p.causal), cnt = w.count();
+      const int end = p.blocks.key_end(w.x, w.blk), cnt = w.count();
       const int page = 1 << p.s.page_log2, box = min(page, BN);
       for (int i = 0; i < cnt; ++i, ++t) {
         const int s = t % C::SLOTS, round = t / C::SLOTS;
@@ -273,7 +176,7 @@ attn_rows(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUten
         }
         __syncwarp();
       }
-      w.advance(p);
+      w.advance(p.s, p.blocks);
     }
     // every issued copy lands before this CTA's shared memory is released
     for (int i = max(0, t - C::SLOTS); i < t; ++i) mbar_wait_drain(full(i % C::SLOTS), (i / C::SLOTS) & 1);
@@ -288,17 +191,17 @@ attn_rows(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUten
   bool ok = true;
   while (w.cur < w.end) {
     const Seq x = w.x;
-    const int cnt = w.count(), R = x.n * p.group, row0 = w.rb * BR, off = x.len - x.n;
-    const int end = key_end(x, w.rb, p.group, p.causal);
+    const int cnt = w.count(), R = x.n * group, row0 = w.blk * BR, off = x.len - x.n;
+    const int end = p.blocks.key_end(x, w.blk);
     // the A operand of the rows g, g + 8; 8-bit caches: columns in the order that their bytes come in (4 t4 ... + 3 of 16)
     uint32_t qa[D / 16][4];
     int lim[2];
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
       const int r = row0 + g + 8 * i;
-      lim[i] = r >= R ? 0 : p.causal ? min(x.len, off + r / p.group + 1) : x.len;
-      const uint16_t* src = p.q + (x.tok0 + (r < R ? r / p.group : 0)) * p.q_token +
-                            (w.h * p.group + (r < R ? r % p.group : 0)) * p.q_head;
+      lim[i] = r >= R ? 0 : causal ? min(x.len, off + r / group + 1) : x.len;
+      const uint16_t* src = p.q + (x.tok0 + (r < R ? r / group : 0)) * p.q_token +
+                            (w.h * group + (r < R ? r % group : 0)) * p.q_head;
 #pragma unroll
       for (int k = 0; k < D / 16; ++k) {
         if constexpr (INT8) {
@@ -311,7 +214,7 @@ attn_rows(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUten
         }
       }
     }
-    const int lim_least = p.causal ? max(0, min(x.len, off + row0 / p.group + 1)) : x.len;  // of the block's rows
+    const int lim_least = causal ? max(0, min(x.len, off + row0 / group + 1)) : x.len;  // of the block's rows
     float m[2] = {-CUDART_INF_F, -CUDART_INF_F}, l[2] = {0.f, 0.f};
     float o[D / 8][4];
 #pragma unroll
@@ -549,7 +452,7 @@ attn_rows(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUten
           uint32_t out[PER / 2];
 #pragma unroll
           for (int i = 0; i < PER / 2; ++i) out[i] = pack2<BF16>(acc[2 * i] * inv, acc[2 * i + 1] * inv);
-          uint16_t* dst = p.o + ((long long)(x.tok0 + row / p.group) * p.s.heads * p.group + w.h * p.group + row % p.group) * D + col;
+          uint16_t* dst = p.o + ((long long)(x.tok0 + row / group) * p.s.heads * group + w.h * group + row % group) * D + col;
           if constexpr (PER == 8)
             *reinterpret_cast<uint4*>(dst) = make_uint4(out[0], out[1], out[2], out[3]);
           else
@@ -565,62 +468,48 @@ attn_rows(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUten
       }
     }
     consumers_meet();
-    w.advance(p);
+    w.advance(p.s, p.blocks);
   }
 }
 
-// Joins the parts of the units that several CTAs of attn_rows shared. Block (key head, sequence, four rows), one thread
-// to a column. Also zeroes the rows of packed tokens that belong to no sequence.
+// Joins the parts of the units that several CTAs of attn_rows shared: block (c, four rows) those of the unit that CTA c
+// continues, if c is the first to continue it; one thread to a column, the parts in the order of the CTAs. Block (0, 0)
+// also zeroes the rows of packed tokens that belong to no sequence.
 template <int D, bool BF16>
-__global__ void __launch_bounds__(D) merge_rows(const Params p, int ctas) {
+__global__ void __launch_bounds__(D) merge_rows(const Params p, int grid) {
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  const int h = blockIdx.x, b = blockIdx.y, lane = threadIdx.x & 31;
-  if (b == 0 && h == 0 && blockIdx.z == 0) {
-    const int first = min(max(p.s.cu_new[p.s.batch], 0), p.s.total);
-    for (long long i = (long long)first * p.s.heads * p.group * D + threadIdx.x; i < (long long)p.s.total * p.s.heads * p.group * D; i += D)
-      p.o[i] = 0;
-  }
-  const Seq x = seq_of(p.s, b);
-  const int R = x.n * p.group;
-  if ((int)blockIdx.z * 4 >= R) return;
-  long long total = 0, w0 = 0;
-  for (int i0 = 0; i0 < p.s.batch; i0 += 32)
-    if (i0 + lane < p.s.batch) {
-      const long long y = head_tiles(seq_of(p.s, i0 + lane), p.group, p.causal) * p.s.heads;
-      total += y;
-      if (i0 + lane < b) w0 += y;
+  const int group = p.blocks.group, c0 = blockIdx.x - 1;
+  if (c0 < 0) {
+    if (blockIdx.y == 0) {
+      const int first = min(max(p.s.cu_new[p.s.batch], 0), p.s.total);
+      const long long row = (long long)p.s.heads * group * D;
+      for (long long i = first * row + threadIdx.x; i < p.s.total * row; i += D) p.o[i] = 0;
     }
-  for (int m = 16; m > 0; m >>= 1) {
-    total += __shfl_xor_sync(0xffffffffu, total, m);
-    w0 += __shfl_xor_sync(0xffffffffu, w0, m);
+    return;
   }
-  w0 += h * head_tiles(x, p.group, p.causal);
-  for (int rb = 0; rb < row_blocks(x, p.group); ++rb) {
-    const int nt = tiles_of(x, rb, p.group, p.causal);
-    const int c0 = (int)(((w0 + 1) * ctas - 1) / total), c1 = (int)(((w0 + nt) * ctas - 1) / total);
-    if (c1 > c0) {
-      for (int r = blockIdx.z * 4; r < blockIdx.z * 4 + 4 && rb * BR + r < R; ++r) {
-        float M = -CUDART_INF_F, L = 0.f, acc = 0.f;
-        auto slot = [&](int c) { return (2LL * c + (c > c0 ? 0 : 1)) * BR + r; };
-        for (int c = c0; c <= c1; ++c)
-          if (total * c / ctas < total * (c + 1) / ctas) M = fmaxf(M, p.ml[slot(c)].x);
-        const float ref = M == -CUDART_INF_F ? 0.f : M;
+  Walk<RowBlocks> w;
+  w.start(p.s, p.blocks, c0 + 1, grid);
+  const long long w0 = w.cur - w.tile;
+  if (w.cur >= w.end || w.tile == 0 || w.first(c0) > w0) return;
+  const int R = w.x.n * group;
+  for (int r = blockIdx.y * 4; r < blockIdx.y * 4 + 4 && w.blk * BR + r < R; ++r) {
+    auto slot = [&](int c) { return (2LL * c + (c > c0 ? 0 : 1)) * BR + r; };
+    float M = -CUDART_INF_F, L = 0.f, acc = 0.f;
+    int c1 = c0;
+    for (; c1 < w.ctas && w.first(c1) < w0 + w.nt; ++c1) M = fmaxf(M, p.ml[slot(c1)].x);
+    const float ref = M == -CUDART_INF_F ? 0.f : M;
 #pragma unroll 4
-        for (int c = c0; c <= c1; ++c) {
-          if (total * c / ctas == total * (c + 1) / ctas) continue;  // that CTA had no tile
-          const float2 y = p.ml[slot(c)];
-          const float wt = ex2(y.x - ref);
-          L = fmaf(wt, y.y, L);
-          acc = fmaf(wt, p.part[slot(c) * D + threadIdx.x], acc);
-        }
-        const int row = rb * BR + r;
-        const float out = M == -CUDART_INF_F ? 0.f : acc / L;
-        p.o[((long long)(x.tok0 + row / p.group) * p.s.heads * p.group + h * p.group + row % p.group) * D + threadIdx.x] =
-            (uint16_t)pack2<BF16>(out, 0.f);
-      }
+    for (int c = c0; c < c1; ++c) {
+      const float2 y = p.ml[slot(c)];
+      const float wt = ex2(y.x - ref);
+      L = fmaf(wt, y.y, L);
+      acc = fmaf(wt, p.part[slot(c) * D + threadIdx.x], acc);
     }
-    w0 += nt;
+    const int row = w.blk * BR + r;
+    const float out = M == -CUDART_INF_F ? 0.f : acc / L;
+    p.o[((long long)(w.x.tok0 + row / group) * p.s.heads * group + w.h * group + row % group) * D + threadIdx.x] =
+        (uint16_t)pack2<BF16>(out, 0.f);
   }
 }
 
@@ -640,15 +529,15 @@ cudaError_t launch(const PagedAttnArgs& a, int dev) {
   }
   CUtensorMap mk, mv;
   const int page = 1 << a.s.page_log2, box = std::min(page, BN), elem = INT8 ? 1 : 2, cols = INT8 ? D : 64;
-  if (!make_paged_map(&mk, a.kc, a.s.num_pages, a.s.heads, page, D, a.kcs, elem, BF16, box, cols) ||
-      !make_paged_map(&mv, a.vc, a.s.num_pages, a.s.heads, page, D, a.vcs, elem, BF16, box, cols))
+  if (!make_paged_map(&mk, a.kc, a.s.num_pages, a.s.heads, page, D, a.kcs, elem, BF16, box, cols, 1) ||
+      !make_paged_map(&mv, a.vc, a.s.num_pages, a.s.heads, page, D, a.vcs, elem, BF16, box, cols, 1))
     return cudaErrorInvalidValue;
   const int ctas = sms;
   const size_t ml_bytes = (size_t)ctas * 2 * BR * sizeof(float2);
   void* block = nullptr;
   if ((e = scratch_alloc(dev, ml_bytes + (size_t)ctas * 2 * BR * D * sizeof(float), a.stream, &block)) != cudaSuccess) return e;
   Params p{a.s, static_cast<const uint16_t*>(a.q), a.q_token, a.q_head, static_cast<uint16_t*>(a.o), a.ks, a.vs, a.kss, a.vss,
-           a.group, a.causal ? 1 : 0, a.scale * 1.4426950408889634f,
+           RowBlocks{a.group, a.causal ? 1 : 0, a.s.heads}, a.scale * 1.4426950408889634f,
            reinterpret_cast<float*>(static_cast<char*>(block) + ml_bytes), static_cast<float2*>(block)};
   cudaLaunchConfig_t cfg = {};
   cudaLaunchAttribute pdl[1];
@@ -663,7 +552,7 @@ cudaError_t launch(const PagedAttnArgs& a, int dev) {
   e = cudaLaunchKernelEx(&cfg, attn_rows<D, BF16, INT8>, mk, mv, p);
   if (e == cudaSuccess) {
     note_launch();
-    cfg.gridDim = dim3((unsigned)a.s.heads, (unsigned)a.s.batch, BR / 4);
+    cfg.gridDim = dim3((unsigned)ctas, BR / 4);
     cfg.blockDim = dim3(D);
     cfg.dynamicSmemBytes = 0;
     if ((e = cudaLaunchKernelEx(&cfg, merge_rows<D, BF16>, p, ctas)) == cudaSuccess) note_launch();

@@ -1,0 +1,676 @@
+// Attention of many query rows over a paged cache (chunks of prompts), on the 5th-generation tensor cores: the operator of
+// attn_paged.cu for units of up to 256 query rows, with the pipeline of attn_tc_sm100.cu (TMA, tcgen05.mma, scores and
+// outputs in TMEM, a softmax thread per query row). What is different here:
+//
+//   * A unit is two tiles of 128 / group new tokens with all `group` query heads of one key head (one TMA box each; with
+//     a group that does not divide 128 the tile's last rows stay unused), so shared heads cost no more key traffic.
+//   * Keys and values come page by page, a TMA box each, into tiles of 128 keys.
+//   * Work is cut evenly over the CTAs (paged_dev.cuh): ragged batches and single long prompts leave no partial wave. The
+//     units that CTAs share leave partial results for merge_chunk.
+//   * Rows of the last tile past the keys that the unit sees may hold anything (the page's stale rest, or what an earlier
+//     tile left): their scores are masked by selection, and their values are zeroed, since 0 * NaN is NaN in a product.
+//
+// The probabilities are rounded to the cache's 16-bit type, as tcgen05.mma wants P and V of one type: half an ulp of each,
+// which adds to the output an error of the size of its own rounding (sqrt(2) times in all).
+#include <cuda.h>
+#include <math_constants.h>
+
+#include <algorithm>
+#include <atomic>
+
+#include "launchers.h"
+#include "paged_dev.cuh"
+#include "sm100_ptx.cuh"
+
+namespace phantom {
+namespace chunk {
+
+constexpr int BM = 128;  // rows of a query tile = TMEM lanes
+constexpr int BN = 128;  // keys of a tile
+constexpr int MMA_WARP = 8, TMA_WARP = 9, PV_WARP = 10;
+constexpr int kThreads = 384;
+// Register split, as in attn_tc_sm100.cu: 384 threads launch with 168 each; 128 * (168 - 72) = 2 * 128 * (216 - 168).
+constexpr int kRegsProducer = 72, kRegsSoftmax = 216;
+constexpr float kRescaleThreshold = 8.0f;  // log2 units: rescale O only when the maximum grows by more than 2^8
+constexpr int kErrTmaWait = 1, kErrMmaWait = 2, kErrSoftmaxWait = 4, kErrEpilogueWait = 8;
+constexpr int kUnitRing = 4;
+
+template <int D>
+struct Cfg {
+  static constexpr bool SHARED_S = D == 128;       // one S region for both query tiles (d = 128), or one each
+  static constexpr int KBLK = D / 64;              // 64-column (128-byte) swizzle blocks across d
+  static constexpr int SUB = BN * 128;             // one such block of a tile of 128 rows
+  static constexpr int TILE = BN * D * 2;
+  static constexpr int STAGES = D == 128 ? 4 : 8;  // ring slots, keys and values in turn
+  static constexpr int OFF_Q = 0;
+  static constexpr int OFF_KV = 2 * TILE;
+  static constexpr int OFF_OST = OFF_KV + STAGES * TILE;  // output staging: per softmax warp 32 rows of 64 bytes
+  static constexpr int OST_WARP = 32 * 64;
+  static constexpr int OFF_BAR = OFF_OST + 8 * OST_WARP;
+  static constexpr int NUM_BARS = 2 * STAGES + 7 * 2 + 3;
+  static constexpr int OFF_MISC = (OFF_BAR + NUM_BARS * 8 + 15) / 16 * 16;  // TMEM base, abort flag, unit ring
+  static constexpr int SMEM = OFF_MISC + 16 + 48 * kUnitRing + 1024;
+  static_assert(SMEM <= 227 * 1024, "shared memory plan exceeds 227 KB");
+  // TMEM columns, as in attn_tc_sm100.cu: P never shares columns with S
+  static constexpr uint32_t T_S0 = SHARED_S ? 0 : 2 * D, T_S1 = SHARED_S ? 0 : 2 * D + BN;
+  static constexpr uint32_t T_P0 = SHARED_S ? BN : 2 * D + 2 * BN, T_P1 = T_P0 + BN / 2;
+  static constexpr uint32_t T_O0 = SHARED_S ? 2 * BN : 0, T_O1 = T_O0 + D;
+  static_assert(T_P1 + BN / 2 <= 512 && T_O1 + D <= 512, "TMEM plan exceeds 512 columns");
+};
+
+// Units of `per` new tokens; tiles of 128 keys.
+struct TokenBlocks {
+  int per, causal, heads;
+  static constexpr int kTile = BN;
+  __device__ int count(const Seq& x) const { return (x.n + per - 1) / per; }
+  __device__ int key_end(const Seq& x, int blk) const {
+    return causal ? min(max(x.len - x.n + min(x.n, (blk + 1) * per), 0), x.len) : x.len;
+  }
+  __device__ long long head_tiles(const Seq& x) const {
+    const int c = count(x), off = x.len - x.n;
+    if (c < 3) return sum_tiles(*this, x);
+    if (!causal) return (long long)c * tiles_of(*this, x, 0);
+    if (off < 0) return sum_tiles(*this, x);
+    // sum over the c - 1 whole blocks of ceil((off + i per) / 128), i = 1 ... c - 1, and the last: a sum of
+    // floor((a i + r) / m), taken by the Euclidean descent on (a, m)
+    long long w = tiles_of(*this, x, c - 1), n = c - 1, a = per, r = off + per + kTile - 1, m = kTile;
+    for (;;) {
+      w += n * (n - 1) / 2 * (a / m) + n * (r / m);
+      a %= m;
+      r %= m;
+      const long long y = a * n + r;
+      if (y < m) break;
+      n = y / m;
+      r = y % m;
+      const long long t = m;
+      m = a;
+      a = t;
+    }
+    return w;
+  }
+};
+
+struct Params {
+  PagedSeqs s;
+  TokenBlocks blocks;
+  int group, tile_tokens;  // query heads of a key head; new tokens of a query tile
+  uint16_t* o;
+  float scale_log2;        // of the scores' size; their sign is in the instruction (negate)
+  int negate;
+  float4* part;            // partial results: [CTA][2][query tile][D / 4][row], fp32
+  float2* ml;              // their (reference maximum, sum): [CTA][2][query tile][row]
+};
+
+// What the producer tells the other roles of a unit (48 bytes).
+struct Unit {
+  int cnt, tile0, end, has_b;  // its tiles here, the first of them; the keys it sees; whether it has a second query tile
+  int len, n, tok, tok0;       // the sequence: cached and new tokens; its new token that the unit begins with; packed place
+  int h, slot, id, b;          // key head; place of the partial result (-1: the unit is whole); id -1 ends the roles
+};
+
+template <int N>
+__device__ __forceinline__ float row_max(const float (&s)[N]) {
+  float a[8];
+#pragma unroll
+  for (int k = 0; k < 8; ++k) a[k] = fmaxf(s[k], s[k + 8]);
+#pragma unroll
+  for (int i = 16; i < N; i += 16)
+#pragma unroll
+    for (int k = 0; k < 8; ++k) a[k] = max3(a[k], s[i + k], s[i + 8 + k]);
+  return fmaxf(max3(a[0], a[1], a[2]), max3(a[3], a[4], max3(a[5], a[6], a[7])));
+}
+
+// p = exp2(s * scale - sub) of 64 scores as packed 16-bit pairs; returns the sum of the unrounded values. Every fourth pair
+// by the FMA pipe's polynomial, as in attn_tc_sm100.cu, with an exact zero where bf16 could hold its 2^-125.
+template <bool BF16, int OFF>
+__device__ __forceinline__ float softmax64(const float (&s)[BN], float scale_log2, float sub, uint32_t (&p)[32]) {
+  const float2 sc = make_float2(scale_log2, scale_log2), nm = make_float2(-sub, -sub);
+  float2 acc[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+#pragma unroll
+  for (int c = 0; c < 32; ++c) {
+    float2 x = fma2(make_float2(s[OFF + 2 * c], s[OFF + 2 * c + 1]), sc, nm);
+    if ((0x09 >> (c & 7)) & 1) {
+      const float2 arg = x;
+      x = exp2_fma2(x);
+      if constexpr (BF16) {
+        x.x = arg.x < -125.f ? 0.f : x.x;
+        x.y = arg.y < -125.f ? 0.f : x.y;
+      }
+    } else {
+      x.x = ex2(x.x);
+      x.y = ex2(x.y);
+    }
+    acc[c & 1] = add2(acc[c & 1], x);
+    p[c] = pack2<BF16>(x.x, x.y);
+  }
+  const float2 t = add2(acc[0], acc[1]);
+  return t.x + t.y;
+}
+
+template <int D, bool BF16>
+__global__ void __launch_bounds__(kThreads, 1)
+attn_chunk(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
+           const __grid_constant__ CUtensorMap tmV, const Params p) {
+  using C = Cfg<D>;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  const uint32_t sbase = smem_u32(smem);
+  const uint32_t bar0 = sbase + C::OFF_BAR;
+  auto kv_full = [&](int s) { return bar0 + 8u * s; };
+  auto kv_empty = [&](int s) { return bar0 + 8u * (C::STAGES + s); };
+  constexpr int B0 = 2 * C::STAGES;
+  // q_full[u & 1]: unit u is published and its queries have landed. unit_read[u & 1]: every role has read unit u's record;
+  // the producer waits for that before it publishes unit u + 2, so no role is ever two phases of q_full behind.
+  auto q_full = [&](int u) { return bar0 + 8u * (B0 + (u & 1)); };
+  auto unit_read = [&](int u) { return bar0 + 8u * (B0 + 2 + (u & 1)); };
+  auto s_full = [&](int g) { return bar0 + 8u * (B0 + 4 + g); };
+  auto s_free = [&](int g) { return bar0 + 8u * (B0 + 6 + g); };
+  auto p_ready = [&](int g) { return bar0 + 8u * (B0 + 8 + g); };
+  auto o_done = [&](int g) { return bar0 + 8u * (B0 + 10 + g); };
+  auto o_free = [&](int g) { return bar0 + 8u * (B0 + 12 + g); };
+  const uint32_t q_free = bar0 + 8u * (B0 + 14), drain_bar = bar0 + 8u * (B0 + 15), drain_pv_bar = bar0 + 8u * (B0 + 16);
+  uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(smem + C::OFF_MISC);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + C::OFF_MISC + 4);
+  int4* ring = reinterpret_cast<int4*>(smem + C::OFF_MISC + 16);  // [kUnitRing][3]
+  int* status = p.s.status;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < C::STAGES; ++s) {
+      mbar_init(kv_full(s), 1);
+      mbar_init(kv_empty(s), 1);
+    }
+    for (int g = 0; g < 2; ++g) {
+      mbar_init(q_full(g), 1);
+      mbar_init(unit_read(g), 10);  // eight softmax warps, the two MMA warps
+      mbar_init(s_full(g), 1);
+      mbar_init(s_free(g), 128);
+      mbar_init(p_ready(g), 128);
+      mbar_init(o_done(g), 1);
+      mbar_init(o_free(g), 128);
+    }
+    mbar_init(q_free, 1);
+    mbar_init(drain_bar, 1);
+    mbar_init(drain_pv_bar, 1);
+    *abort_flag = 0;
+    fence_mbar_init();
+  }
+  if (warp == MMA_WARP) {
+    tmem_alloc(smem_u32(tmem_holder), 512);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_holder;
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+
+  auto publish = [&](int u, const Unit& x) {
+    int4* r = ring + 3 * (u % kUnitRing);
+    r[0] = make_int4(x.cnt, x.tile0, x.end, x.has_b);
+    r[1] = make_int4(x.len, x.n, x.tok, x.tok0);
+    r[2] = make_int4(x.h, x.slot, x.id, x.b);
+  };
+  auto record = [&](int u) {
+    const int4* r = ring + 3 * (u % kUnitRing);
+    const int4 a = r[0], b = r[1], c = r[2];
+    Unit x;
+    x.cnt = a.x, x.tile0 = a.y, x.end = a.z, x.has_b = a.w;
+    x.len = b.x, x.n = b.y, x.tok = b.z, x.tok0 = b.w;
+    x.h = c.x, x.slot = c.y, x.id = c.z, x.b = c.w;
+    return x;
+  };
+  auto wait = [&](uint32_t bar, int parity, int code) {
+    return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag, status, code)) != 0;
+  };
+  // Next unit of a consuming role (its id is -1 at the end, or when a wait gave up).
+  auto next_unit = [&](int u, bool& ok) -> Unit {
+    Unit x;
+    x.id = -1;
+    if ((ok = wait(q_full(u), (u >> 1) & 1, kErrMmaWait))) {
+      x = record(u);
+      __syncwarp();
+      if (lane == 0) mbar_arrive(unit_read(u));
+    }
+    return x;
+  };
+
+  if (warp == TMA_WARP) {
+    setmaxnreg_dec<kRegsProducer>();
+    // Producer, per unit: its record and queries, then keys and values of its tiles in turn.
+    if (lane == 0) {
+      tma_prefetch_desc(&tmQ);
+      tma_prefetch_desc(&tmK);
+      tma_prefetch_desc(&tmV);
+    }
+    __syncwarp();
+    Walk<TokenBlocks> w;
+    w.start(p.s, p.blocks, blockIdx.x, gridDim.x);
+    const long long begin = w.cur;
+    const int page = 1 << p.s.page_log2, box = min(page, BN);
+    int t = 0, nu = 0, nq = 0;  // copies, units, phases of q_full begun
+    bool ok = true;
+    for (;;) {
+      if (nu > 0 && !(ok = wait(q_free, (nu - 1) & 1, kErrTmaWait))) break;
+      if (nu > 1 && !(ok = wait(unit_read(nu), ((nu >> 1) - 1) & 1, kErrTmaWait))) break;
+      Unit x = {};
+      x.id = -1;
+      if (w.cur >= w.end) {
+        if (lane == 0) {
+          publish(nu, x);
+          mbar_arrive(q_full(nu));
+        }
+        __syncwarp();
+        ++nq;
+        break;
+      }
+      x.id = nu;
+      x.b = w.b;
+      x.h = w.h;
+      x.cnt = w.count();
+      x.tile0 = w.tile;
+      x.end = p.blocks.key_end(w.x, w.blk);
+      x.tok = w.blk * p.blocks.per;
+      x.len = w.x.len, x.n = w.x.n, x.tok0 = w.x.tok0;
+      x.has_b = x.tok + p.tile_tokens < x.n;
+      x.slot = x.cnt == w.nt ? -1 : 2 * (int)blockIdx.x + (begin > w.cur - w.tile ? 0 : 1);
+      if (lane == 0) {
+        publish(nu, x);
+        const int tiles = x.has_b ? 2 : 1;
+        mbar_arrive_expect_tx(q_full(nu), tiles * C::KBLK * p.tile_tokens * p.group * 128);
+        for (int g = 0; g < tiles; ++g)
+          for (int c = 0; c < C::KBLK; ++c)
+            tma_load_4d(sbase + C::OFF_Q + g * C::TILE + c * C::SUB, &tmQ, q_full(nu), c * 64, 0, x.h,
+                        x.tok0 + x.tok + g * p.tile_tokens);
+      }
+      __syncwarp();
+      ++nu;
+      ++nq;
+      for (int jt = 0; jt < 2 * x.cnt; ++jt, ++t) {
+        const int s = t % C::STAGES, round = t / C::STAGES;
+        const int j0 = (x.tile0 + (jt >> 1)) * BN;
+        const int boxes = max(0, (min(j0 + BN, x.end) - j0 + box - 1) / box);
+        const int pg = lane / C::KBLK, blk = lane % C::KBLK;
+        int id = 0;
+        if (lane < boxes * C::KBLK) id = page_of(p.s, x.b, (j0 >> p.s.page_log2) + pg);
+        if (round > 0 && !(ok = wait(kv_empty(s), (round - 1) & 1, kErrTmaWait))) break;
+        if (lane == 0) mbar_arrive_expect_tx(kv_full(s), boxes * box * D * 2);
+        __syncwarp();
+        if (lane < boxes * C::KBLK)  // an id that is out of range reads as zeros
+          tma_load_4d(sbase + C::OFF_KV + s * C::TILE + blk * C::SUB + pg * box * 128, (jt & 1) ? &tmV : &tmK, kv_full(s),
+                      blk * 64, j0 & (page - 1), x.h, id);
+        __syncwarp();
+      }
+      if (!ok) break;
+      w.advance(p.s, p.blocks);
+    }
+    // every issued copy lands before this CTA's shared memory can be released
+    for (int a = max(0, nq - 2); a < nq; ++a) mbar_wait_drain(q_full(a), (a >> 1) & 1);
+    if (!ok) *abort_flag = 1;
+    for (int i = max(0, t - C::STAGES); i < t; ++i) mbar_wait_drain(kv_full(i % C::STAGES), (i / C::STAGES) & 1);
+  } else if (warp == PV_WARP + 1) {
+    setmaxnreg_dec<kRegsProducer>();  // completes the warpgroup
+  } else if (warp == MMA_WARP || warp == PV_WARP) {
+    setmaxnreg_dec<kRegsProducer>();
+    const uint64_t dq = smem_desc_sw128(sbase + C::OFF_Q, 16, 1024);
+    const uint64_t dk = smem_desc_sw128(sbase + C::OFF_KV, 16, 1024);
+    const uint64_t dv = smem_desc_sw128(sbase + C::OFF_KV, C::SUB, 1024);
+    auto kv_wait = [&](int t) { return wait(kv_full(t % C::STAGES), (t / C::STAGES) & 1, kErrMmaWait); };
+    if (warp == MMA_WARP) {
+      // S_g = Q_g K^T, per key tile for query tile A, then B (see attn_tc_sm100.cu).
+      const uint32_t idesc = idesc_f16(BF16, BM, BN, false) | (p.negate ? 1u << 13 : 0u);
+      auto issue = [&](int g, int stage) {
+        const uint32_t a_off = (uint32_t)(g * C::TILE) >> 4, b_off = (uint32_t)(stage * C::TILE) >> 4;
+        const uint32_t d_t = tmem + (g ? C::T_S1 : C::T_S0);
+#pragma unroll
+        for (int kk = 0; kk < D / 16; ++kk) {
+          const uint32_t o = ((kk >> 2) * C::SUB + (kk & 3) * 32) >> 4;
+          mma_ss(d_t, dq + (a_off + o), dk + (b_off + o), idesc, kk > 0 ? 1u : 0u);
+        }
+      };
+      int tb = 0, nu = 0, ks = 0;
+      int qc[2] = {0, 0};
+      bool ok = true;
+      for (;;) {
+        const Unit x = next_unit(nu, ok);
+        if (x.id < 0) break;
+        for (int q = 0; ok && q < x.cnt; ++q) {
+          const int tk = tb + 2 * q, sk = tk % C::STAGES;
+          if (!(ok = kv_wait(tk))) break;
+#pragma unroll
+          for (int g = 0; g < 2; ++g) {
+            if (g == 1 && !x.has_b) continue;
+            const int n_prev = C::SHARED_S ? ks : qc[g];
+            if (n_prev > 0 && !(ok = wait(s_free(C::SHARED_S ? 0 : g), (n_prev - 1) & 1, kErrMmaWait))) break;
+            tc_fence_after();
+            if (elect_one()) {
+              issue(g, sk);
+              mma_commit(s_full(g));
+              if (g == x.has_b) mma_commit(kv_empty(sk));
+            }
+            __syncwarp();
+            if (C::SHARED_S) ++ks; else ++qc[g];
+          }
+        }
+        if (!ok) break;
+        if (elect_one()) mma_commit(q_free);
+        __syncwarp();
+        tb += 2 * x.cnt;
+        ++nu;
+      }
+      if (elect_one()) mma_commit(drain_bar);
+      __syncwarp();
+      mbar_wait_drain(drain_bar, 0);
+    } else {
+      // O_g += P_g V: P from TMEM, V as an MN-major operand.
+      constexpr uint32_t idesc = idesc_f16(BF16, BM, D, true);
+      auto issue = [&](int g, int stage, bool acc) {
+        const uint32_t b_off = (uint32_t)(stage * C::TILE) >> 4;
+        const uint32_t d_t = tmem + (g ? C::T_O1 : C::T_O0), p_t = tmem + (g ? C::T_P1 : C::T_P0);
+#pragma unroll
+        for (int kk = 0; kk < BN / 16; ++kk)
+          mma_ts(d_t, p_t + kk * 8, dv + (b_off + kk * (2048 >> 4)), idesc, (acc || kk > 0) ? 1u : 0u);
+      };
+      int tb = 0, nu = 0;
+      int pc[2] = {0, 0}, uc[2] = {0, 0};
+      bool ok = true;
+      for (;; ++nu) {
+        const Unit x = next_unit(nu, ok);
+        if (x.id < 0) break;
+        for (int q = 0; ok && q < x.cnt; ++q) {
+          const int tv = tb + 2 * q + 1, sv = tv % C::STAGES;
+          if (!(ok = kv_wait(tv))) break;
+          const int j0 = (x.tile0 + q) * BN;
+          if (j0 + BN > x.end) {  // zero the values of keys past the unit's end
+            for (int i = max(0, x.end - j0) * 8 + lane; i < BN * 8; i += 32)
+              for (int c = 0; c < C::KBLK; ++c)
+                st_shared_v4(sbase + C::OFF_KV + sv * C::TILE + c * C::SUB + i * 16, 0, 0, 0, 0);
+            fence_proxy_async_smem();
+            __syncwarp();
+          }
+          for (int g = 0; g <= x.has_b; ++g) {
+            if (q == 0 && uc[g] > 0 && !(ok = wait(o_free(g), (uc[g] - 1) & 1, kErrMmaWait))) break;
+            if (!(ok = wait(p_ready(g), pc[g] & 1, kErrMmaWait))) break;
+            tc_fence_after();
+            if (elect_one()) {
+              issue(g, sv, q > 0);
+              mma_commit(o_done(g));
+              if (g == x.has_b) mma_commit(kv_empty(sv));
+            }
+            __syncwarp();
+            ++pc[g];
+          }
+        }
+        if (!ok) break;
+        for (int g = 0; g <= x.has_b; ++g) ++uc[g];
+        tb += 2 * x.cnt;
+      }
+      if (elect_one()) mma_commit(drain_pv_bar);
+      __syncwarp();
+      mbar_wait_drain(drain_pv_bar, 0);
+    }
+  } else {
+    // Softmax warpgroups: warps 0-3 query tile A, 4-7 tile B; thread = query row = TMEM lane (see attn_tc_sm100.cu).
+    setmaxnreg_inc<kRegsSoftmax>();
+    const int g = warp >> 2, r_local = threadIdx.x & 127;
+    const uint32_t lane_off = (uint32_t)((warp & 3) * 32) << 16;
+    const uint32_t t_s = tmem + lane_off + (g ? C::T_S1 : C::T_S0);
+    const uint32_t t_p = tmem + lane_off + (g ? C::T_P1 : C::T_P0);
+    const uint32_t t_o = tmem + lane_off + (g ? C::T_O1 : C::T_O0);
+    uint8_t* stage = smem + C::OFF_OST + warp * C::OST_WARP;
+    const int row_tok = r_local / p.group;  // this row's token within the query tile
+    int sc = 0, oc = 0;
+    bool ok = true;
+    for (int nu = 0;; ++nu) {
+      Unit x = next_unit(nu, ok);
+      if (x.id < 0) break;
+      if (g == 1 && !x.has_b) continue;
+      const int tile_tok = x.tok + g * p.tile_tokens;
+      const int see = x.len - x.n + tile_tok + 1;  // causal: keys that the tile's first row sees
+      const bool causal = p.blocks.causal;
+      const int lim = causal ? min(x.len, see + row_tok) : x.len;
+      const int lim_least = causal ? min(x.len, see) : x.len;
+      const int cnt = x.cnt, jb = x.tile0 * BN;
+      float m_used = -CUDART_INF_F, l = 0.f;
+      bool s_ready = false;
+      for (int j = 0; j < cnt; ++j) {
+        if (!s_ready && !(ok = wait(s_full(g), sc & 1, kErrSoftmaxWait))) break;
+        ++sc;
+        tc_fence_after();
+        float s[BN];
+        {
+          uint32_t r[BN];
+          tmem_ld128_wait(t_s, r);
+#pragma unroll
+          for (int i = 0; i < BN; ++i) s[i] = __uint_as_float(r[i]);
+        }
+        tc_fence_before();
+        mbar_arrive(s_free(C::SHARED_S ? 0 : g));
+        const int j0 = jb + j * BN;
+        if (j0 + BN > lim_least) {
+          const int left = lim - j0;
+#pragma unroll
+          for (int c = 0; c < BN; ++c) s[c] = c < left ? s[c] : -CUDART_INF_F;
+        }
+        const float m_new = row_max<BN>(s) * p.scale_log2;
+        float alpha = 1.f;
+        bool need = false;
+        if (j == 0) {
+          m_used = m_new;
+        } else {
+          need = m_new > m_used + kRescaleThreshold;
+          if (need) {
+            alpha = ex2(m_used - m_new);
+            m_used = m_new;
+          }
+          if (!(ok = wait(o_done(g), oc & 1, kErrSoftmaxWait))) break;
+          ++oc;
+          tc_fence_after();
+          if (__any_sync(0xffffffffu, need)) {
+            const float2 a2 = make_float2(alpha, alpha);
+#pragma unroll
+            for (int c = 0; c < D / 32; ++c) {
+              uint32_t rr[32];
+              tmem_ld32_wait(t_o + c * 32, rr);
+#pragma unroll
+              for (int i = 0; i < 16; ++i) {
+                const float2 y = mul2(make_float2(__uint_as_float(rr[2 * i]), __uint_as_float(rr[2 * i + 1])), a2);
+                rr[2 * i] = __float_as_uint(y.x);
+                rr[2 * i + 1] = __float_as_uint(y.y);
+              }
+              tmem_st32(t_o + c * 32, rr);
+            }
+          }
+        }
+        const float sub = m_used == -CUDART_INF_F ? 0.f : m_used;
+        uint32_t pk[32];
+        float psum = softmax64<BF16, 0>(s, p.scale_log2, sub, pk);
+        tmem_st32(t_p, pk);
+        bool next_test = false;
+        if constexpr (!C::SHARED_S) next_test = j + 1 < cnt && mbar_test(s_full(g), sc & 1);
+        psum += softmax64<BF16, 64>(s, p.scale_log2, sub, pk);
+        tmem_st32(t_p + 32, pk);
+        tmem_wait_st();
+        tc_fence_before();
+        mbar_arrive(p_ready(g));
+        if constexpr (!C::SHARED_S) s_ready = __all_sync(0xffffffffu, next_test);
+        l = l * alpha + psum;
+      }
+      if (!ok) break;
+      if (!(ok = wait(o_done(g), oc & 1, kErrEpilogueWait))) break;
+      ++oc;
+      tc_fence_after();
+      x = record(nu);  // read again: fewer registers live across the tile loop
+      if (x.slot < 0) {
+        // O / l, 32 columns at a time through shared memory (16-byte chunk k of row r at k ^ (r / 2 % 4): conflict-free)
+        // so that four lanes write 64 consecutive bytes of a row
+        const float inv_l = m_used == -CUDART_INF_F ? 0.f : 1.f / l;
+        const int rows = min(p.tile_tokens, x.n - (x.tok + g * p.tile_tokens)) * p.group;
+        const long long at = (long long)(x.tok0 + x.tok + g * p.tile_tokens) * p.s.heads;
+#pragma unroll
+        for (int cb = 0; cb < D / 32; ++cb) {
+          uint32_t rr[32], w[16];
+          tmem_ld32_wait(t_o + cb * 32, rr);
+#pragma unroll
+          for (int i = 0; i < 16; ++i)
+            w[i] = pack2<BF16>(__uint_as_float(rr[2 * i]) * inv_l, __uint_as_float(rr[2 * i + 1]) * inv_l);
+          __syncwarp();
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            *reinterpret_cast<uint4*>(stage + lane * 64 + ((k ^ ((lane >> 1) & 3)) << 4)) =
+                make_uint4(w[4 * k], w[4 * k + 1], w[4 * k + 2], w[4 * k + 3]);
+          __syncwarp();
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int r = i * 8 + (lane >> 2), k = lane & 3, row = (warp & 3) * 32 + r;
+            if (row < rows) {
+              const uint4 v = *reinterpret_cast<const uint4*>(stage + r * 64 + ((k ^ ((r >> 1) & 3)) << 4));
+              const int tok = row / p.group;
+              *reinterpret_cast<uint4*>(p.o + ((at + (long long)tok * p.s.heads + x.h) * p.group + (row - tok * p.group)) * D +
+                                        cb * 32 + k * 8) = v;
+            }
+          }
+        }
+      } else {
+        float4* po = p.part + ((long long)x.slot * 2 + g) * (D / 4) * BM + r_local;
+#pragma unroll
+        for (int c = 0; c < D / 32; ++c) {
+          uint32_t rr[32];
+          tmem_ld32_wait(t_o + c * 32, rr);
+#pragma unroll
+          for (int i = 0; i < 8; ++i)
+            po[(c * 8 + i) * BM] = make_float4(__uint_as_float(rr[4 * i]), __uint_as_float(rr[4 * i + 1]),
+                                               __uint_as_float(rr[4 * i + 2]), __uint_as_float(rr[4 * i + 3]));
+        }
+        p.ml[((long long)x.slot * 2 + g) * BM + r_local] = make_float2(m_used, l);
+      }
+      tc_fence_before();
+      mbar_arrive(o_free(g));
+    }
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  if (warp == MMA_WARP) {
+    tc_fence_after();
+    tmem_dealloc(tmem, 512);
+  }
+}
+
+// Joins the parts of the units that several CTAs of attn_chunk shared. Block (c, query tile, 16 columns): the unit that CTA
+// c continues, if c is the first to continue it; thread = query row; the parts in the order of the CTAs. Block (0, 0, 0)
+// also zeroes the rows of packed tokens that belong to no sequence.
+constexpr int kMergeCols = 16;
+template <int D, bool BF16>
+__global__ void __launch_bounds__(BM) merge_chunk(const Params p, int grid) {
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const int g = blockIdx.y, col = blockIdx.z * kMergeCols, r = threadIdx.x, c0 = blockIdx.x - 1;
+  if (c0 < 0) {
+    if (g == 0 && col == 0) {
+      const int first = min(max(p.s.cu_new[p.s.batch], 0), p.s.total);
+      const long long row = (long long)p.s.heads * p.group * D;
+      for (long long i = first * row + r; i < p.s.total * row; i += BM) p.o[i] = 0;
+    }
+    return;
+  }
+  Walk<TokenBlocks> w;
+  w.start(p.s, p.blocks, c0 + 1, grid);
+  const long long w0 = w.cur - w.tile;
+  if (w.cur >= w.end || w.tile == 0 || w.first(c0) > w0) return;
+  const int tok = w.blk * p.blocks.per + g * p.tile_tokens;
+  if (r >= min(p.tile_tokens, w.x.n - tok) * p.group) return;
+  auto slot = [&](int c) { return ((2LL * c + (c > c0 ? 0 : 1)) * 2 + g) * BM + r; };
+  float M = -CUDART_INF_F, L = 0.f, acc[kMergeCols];
+#pragma unroll
+  for (int i = 0; i < kMergeCols; ++i) acc[i] = 0.f;
+  int c1 = c0;
+  for (; c1 < w.ctas && w.first(c1) < w0 + w.nt; ++c1) M = fmaxf(M, p.ml[slot(c1)].x);
+  const float ref = M == -CUDART_INF_F ? 0.f : M;
+#pragma unroll 2
+  for (int c = c0; c < c1; ++c) {
+    const float2 y = p.ml[slot(c)];
+    const float wt = ex2(y.x - ref);
+    L = fmaf(wt, y.y, L);
+    const float4* src = p.part + (slot(c) - r) * (D / 4) + (col / 4) * BM + r;
+#pragma unroll
+    for (int i = 0; i < kMergeCols / 4; ++i) {
+      const float4 v = src[i * BM];
+      acc[4 * i] = fmaf(wt, v.x, acc[4 * i]);
+      acc[4 * i + 1] = fmaf(wt, v.y, acc[4 * i + 1]);
+      acc[4 * i + 2] = fmaf(wt, v.z, acc[4 * i + 2]);
+      acc[4 * i + 3] = fmaf(wt, v.w, acc[4 * i + 3]);
+    }
+  }
+  const float inv = M == -CUDART_INF_F ? 0.f : 1.f / L;
+  uint32_t out[kMergeCols / 2];
+#pragma unroll
+  for (int i = 0; i < kMergeCols / 2; ++i) out[i] = pack2<BF16>(acc[2 * i] * inv, acc[2 * i + 1] * inv);
+  const int t = r / p.group;
+  uint4* dst = reinterpret_cast<uint4*>(
+      p.o + (((long long)(w.x.tok0 + tok + t) * p.s.heads + w.h) * p.group + (r - t * p.group)) * D + col);
+  dst[0] = make_uint4(out[0], out[1], out[2], out[3]);
+  dst[1] = make_uint4(out[4], out[5], out[6], out[7]);
+}
+
+std::atomic<bool> g_attr[2][2][64];
+
+template <int D, bool BF16>
+cudaError_t launch(const PagedAttnArgs& a, int dev) {
+  using C = Cfg<D>;
+  int ctas = 0;
+  cudaError_t e = sm_count(dev, &ctas);
+  if (e != cudaSuccess) return e;
+  std::atomic<bool>& attr = g_attr[D / 128][BF16][dev];
+  if (!attr.load(std::memory_order_acquire)) {
+    if ((e = cudaFuncSetAttribute(attn_chunk<D, BF16>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM)) != cudaSuccess)
+      return e;
+    attr.store(true, std::memory_order_release);
+  }
+  const int page = 1 << a.s.page_log2, box = std::min(page, BN), tile_tokens = BM / a.group;
+  CUtensorMap mq, mk, mv;
+  // queries as (packed token, key head, query head of it, d), boxes of one key head's rows of a tile
+  const Strides3 qs{a.q_token, a.q_head * a.group, a.q_head};
+  if (!make_paged_map(&mk, a.kc, a.s.num_pages, a.s.heads, page, D, a.kcs, 2, BF16, box, 64, 1) ||
+      !make_paged_map(&mv, a.vc, a.s.num_pages, a.s.heads, page, D, a.vcs, 2, BF16, box, 64, 1) ||
+      !make_paged_map(&mq, a.q, a.s.total, a.s.heads, a.group, D, qs, 2, BF16, a.group, 64, tile_tokens))
+    return cudaErrorInvalidValue;
+  const size_t ml_bytes = (size_t)ctas * 4 * BM * sizeof(float2);
+  void* block = nullptr;
+  if ((e = scratch_alloc(dev, ml_bytes + (size_t)ctas * 4 * BM * D * sizeof(float), a.stream, &block)) != cudaSuccess) return e;
+  Params p{a.s, TokenBlocks{2 * tile_tokens, a.causal ? 1 : 0, a.s.heads}, a.group, tile_tokens, static_cast<uint16_t*>(a.o),
+           fabsf(a.scale) * 1.4426950408889634f, a.scale < 0.f ? 1 : 0,
+           reinterpret_cast<float4*>(static_cast<char*>(block) + ml_bytes), static_cast<float2*>(block)};
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute pdl[1];
+  pdl[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  pdl[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = pdl;
+  cfg.numAttrs = 1;
+  cfg.stream = a.stream;
+  cfg.gridDim = dim3((unsigned)ctas);
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = C::SMEM;
+  e = cudaLaunchKernelEx(&cfg, attn_chunk<D, BF16>, mq, mk, mv, p);
+  if (e == cudaSuccess) {
+    note_launch();
+    cfg.gridDim = dim3((unsigned)ctas, 2, D / kMergeCols);
+    cfg.blockDim = dim3(BM);
+    cfg.dynamicSmemBytes = 0;
+    if ((e = cudaLaunchKernelEx(&cfg, merge_chunk<D, BF16>, p, ctas)) == cudaSuccess) note_launch();
+  }
+  if (e == cudaSuccess) e = cudaGetLastError();
+  const cudaError_t ef = cudaFreeAsync(block, a.stream);
+  return e != cudaSuccess ? e : ef;
+}
+
+}  // namespace chunk
+
+cudaError_t launch_paged_attn_chunk(const PagedAttnArgs& a, int dev) {
+  using namespace chunk;
+  if (a.d == 64) return a.bf16 ? launch<64, true>(a, dev) : launch<64, false>(a, dev);
+  return a.bf16 ? launch<128, true>(a, dev) : launch<128, false>(a, dev);
+}
+
+}  // namespace phantom

@@ -1395,7 +1395,7 @@ namespace {
 struct PagedMapEntry {
   CUtensorMap map;
   const void* base = nullptr;
-  int pages = 0, heads = 0, page = 0, d = 0, elem = 0, rows = 0, cols = 0;
+  int pages = 0, heads = 0, page = 0, d = 0, elem = 0, rows = 0, cols = 0, per_box = 0;
   Strides3 st{};
   bool bf16 = false, valid = false;
 };
@@ -1405,11 +1405,11 @@ thread_local int g_paged_next = 0;
 }  // namespace
 
 bool make_paged_map(void* out, const void* base, int num_pages, int heads, int page, int d, const Strides3& st, int elem,
-                    bool bf16, int rows, int cols) {
+                    bool bf16, int rows, int cols, int pages_per_box) {
   CUtensorMap* m = static_cast<CUtensorMap*>(out);
   for (const PagedMapEntry& e : g_paged_maps)
     if (e.valid && e.base == base && e.pages == num_pages && e.heads == heads && e.page == page && e.d == d &&
-        e.elem == elem && e.rows == rows && e.cols == cols && e.bf16 == bf16 && e.st.page == st.page &&
+        e.elem == elem && e.rows == rows && e.cols == cols && e.per_box == pages_per_box && e.bf16 == bf16 && e.st.page == st.page &&
         e.st.head == st.head && e.st.token == st.token) {
       *m = e.map;
       return true;
@@ -1418,7 +1418,7 @@ bool make_paged_map(void* out, const void* base, int num_pages, int heads, int p
   if (!fn) return false;
   const cuuint64_t dims[4] = {(cuuint64_t)d, (cuuint64_t)page, (cuuint64_t)heads, (cuuint64_t)num_pages};
   const cuuint64_t strides[3] = {(cuuint64_t)st.token * elem, (cuuint64_t)st.head * elem, (cuuint64_t)st.page * elem};
-  const cuuint32_t box[4] = {(cuuint32_t)cols, (cuuint32_t)rows, 1, 1};
+  const cuuint32_t box[4] = {(cuuint32_t)cols, (cuuint32_t)rows, 1, (cuuint32_t)pages_per_box};
   const cuuint32_t estr[4] = {1, 1, 1, 1};
   const CUtensorMapDataType type = elem == 1 ? CU_TENSOR_MAP_DATA_TYPE_UINT8
                                    : bf16    ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
@@ -1431,7 +1431,7 @@ bool make_paged_map(void* out, const void* base, int num_pages, int heads, int p
   g_paged_next = (g_paged_next + 1) % kMapCache;
   e.map = *m;
   e.base = base;
-  e.pages = num_pages, e.heads = heads, e.page = page, e.d = d, e.elem = elem, e.rows = rows, e.cols = cols;
+  e.pages = num_pages, e.heads = heads, e.page = page, e.d = d, e.elem = elem, e.rows = rows, e.cols = cols, e.per_box = pages_per_box;
   e.st = st;
   e.bf16 = bf16;
   e.valid = true;

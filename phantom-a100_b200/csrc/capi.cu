@@ -461,7 +461,11 @@ int phantom_attn_paged(const phantom_paged_cache* cache, const void* q, long lon
   a.causal = causal != 0;
   a.scale = scale != 0.f ? scale : 1.f / sqrtf((float)cache->head_dim);
   a.stream = static_cast<cudaStream_t>(stream);
-  const cudaError_t e = launch_paged_attn_rows(a, dev.id);
+  // Query rows of one key head in one sequence, as expected: up to one 16-row block the rows kernel reads the keys once
+  // and is bound by that; above, its blocks would each read them, and the chunk kernel takes up to 256 rows at a time.
+  const long long new_tokens = max_new > 0 ? max_new : (total_new + cache->batch - 1) / cache->batch;
+  const bool few = new_tokens * a.group <= 16 || a.int8;
+  const cudaError_t e = few ? launch_paged_attn_rows(a, dev.id) : launch_paged_attn_chunk(a, dev.id);
   if (e != cudaSuccess) return cuda_fail(name, e);
   g_last_error.clear();
   return PHANTOM_ATTN_OK;

@@ -3,6 +3,7 @@
 // that no value of theirs makes a kernel read or write outside the arrays it was given. What is out of range is recorded
 // in the status word (PHANTOM_ATTN_STATUS_PAGE).
 #include "paged.h"
+#include "sm100_ptx.cuh"
 
 namespace phantom {
 
@@ -41,6 +42,136 @@ __device__ __forceinline__ int seq_index(const PagedSeqs& s, int tok) {
     b += __popc(__ballot_sync(0xffffffffu, i < s.batch && s.cu_new[min(i, s.batch - 1) + 1] <= tok));
   }
   return b;
+}
+
+// ------------------------------------------------------------------------------------------------ even shares of work
+// An attention call's work: units (sequence, key head, block of query rows) in a row, each of as many tiles of keys as its
+// rows see. CTA c of G takes the tiles [c W / G, (c + 1) W / G) of all W, so a unit may be shared by several CTAs.
+// `Blocks` says how the rows are cut: kTile keys to a tile; count(x) blocks; the keys key_end(x, blk) that a block sees;
+// head_tiles(x) tiles in all of one head.
+
+// At least one tile, so that rows without any key are written too (as zeros).
+template <typename Blocks>
+__device__ __forceinline__ int tiles_of(const Blocks& k, const Seq& x, int blk) {
+  return max(1, (k.key_end(x, blk) + Blocks::kTile - 1) / Blocks::kTile);
+}
+template <typename Blocks>
+__device__ __forceinline__ long long sum_tiles(const Blocks& k, const Seq& x) {
+  long long w = 0;
+  for (int i = k.count(x) - 1; i >= 0; --i) w += tiles_of(k, x, i);
+  return w;
+}
+
+// A whole warp walks one CTA's share; every value is uniform over the warp.
+template <typename Blocks>
+struct Walk {
+  long long total, cur, end;
+  int ctas;  // that share the work: no more than there are tiles, so that each has one
+  Seq x;
+  int b, h, blk, tile, nt;  // the unit, its tile at `cur`, its tiles
+
+  __device__ static long long scan(long long w, int lane) {
+    for (int m = 1; m < 32; m <<= 1) {
+      const long long y = __shfl_up_sync(0xffffffffu, w, m);
+      if (lane >= m) w += y;
+    }
+    return w;
+  }
+  __device__ void start(const PagedSeqs& s, const Blocks& k, int cta, int grid) {
+    const int lane = threadIdx.x & 31;
+    auto seq_tiles = [&](int i) { return i < s.batch ? k.head_tiles(seq_of(s, i)) * s.heads : 0LL; };
+    // (up to 32 sequences: one scan gives the total and the place)
+    long long w = scan(seq_tiles(lane), lane);
+    total = __shfl_sync(0xffffffffu, w, 31);
+    for (int i0 = 32; i0 < s.batch; i0 += 32) total += __shfl_sync(0xffffffffu, scan(seq_tiles(i0 + lane), lane), 31);
+    ctas = (int)min((long long)grid, total);
+    cur = cta < ctas ? first(cta) : 0;
+    end = cta < ctas ? first(cta + 1) : 0;
+    if (cur >= end) return;
+    long long before = 0;
+    for (int i0 = 0;; i0 += 32) {
+      if (i0 > 0) w = scan(seq_tiles(i0 + lane), lane);
+      const unsigned past = __ballot_sync(0xffffffffu, before + w > cur);
+      if (past) {
+        const int at = __ffs(past) - 1;
+        const long long up_to = __shfl_sync(0xffffffffu, w, max(at - 1, 0));
+        b = i0 + at;
+        before += at > 0 ? up_to : 0;
+        break;
+      }
+      before += __shfl_sync(0xffffffffu, w, 31);
+    }
+    x = seq_of(s, b);
+    const long long head = k.head_tiles(x);
+    long long r = cur - before;
+    h = (int)(r / head);
+    r -= h * head;
+    const int count = k.count(x);
+    for (int i0 = 0;; i0 += 32) {
+      w = scan(i0 + lane < count ? tiles_of(k, x, i0 + lane) : 0, lane);
+      const unsigned past = __ballot_sync(0xffffffffu, w > r);
+      if (past) {
+        const int at = __ffs(past) - 1;
+        const long long up_to = __shfl_sync(0xffffffffu, w, max(at - 1, 0));
+        blk = i0 + at;
+        r -= at > 0 ? up_to : 0;
+        break;
+      }
+      r -= __shfl_sync(0xffffffffu, w, 31);
+    }
+    nt = tiles_of(k, x, blk);
+    tile = (int)r;
+  }
+  // The first tile of a CTA's share.
+  __device__ long long first(int cta) const { return total * cta / ctas; }
+  // The tiles of the unit that this CTA has.
+  __device__ int count() const { return (int)min((long long)(nt - tile), end - cur); }
+  __device__ void advance(const PagedSeqs& s, const Blocks& k) {
+    cur += count();
+    if (cur >= end) return;
+    tile = 0;
+    if (++blk == k.count(x)) {
+      blk = 0;
+      if (++h == s.heads) {
+        h = 0;
+        do x = seq_of(s, ++b);
+        while (x.n == 0);
+      }
+    }
+    nt = tiles_of(k, x, blk);
+  }
+};
+
+// ------------------------------------------------------------------------------------------------ copies, 8-bit values
+// Untiled bulk copy into shared memory (16-byte aligned, a multiple of 16 bytes).
+__device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst),
+               "l"(src), "r"(bytes), "r"(bar)
+               : "memory");
+}
+__device__ __forceinline__ void tma_load_4d(uint32_t dst, const void* tmap, uint32_t bar, int c0, int c1, int c2, int c3) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
+      " [%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(dst),
+      "l"(reinterpret_cast<uint64_t>(tmap)), "r"(c0), "r"(c1), "r"(c2), "r"(c3), "r"(bar)
+      : "memory");
+}
+// Two signed bytes of w (chosen by sel: result bytes [lo, 4, hi, 4], byte 4 = 0x64) as exact fp16 pairs; w already has its
+// sign bits flipped, so a byte u = b + 128 gives the fp16 number 1024 + u.
+template <uint32_t SEL>
+__device__ __forceinline__ uint32_t bytes_f16(uint32_t w) {
+  const uint32_t r = __byte_perm(w, 0x64646464u, SEL);
+  const __half2 x = __hsub2(*reinterpret_cast<const __half2*>(&r), __half2half2(__ushort_as_half(0x6480)));
+  return *reinterpret_cast<const uint32_t*>(&x);
+}
+// Two signed bytes as exact bf16 pairs (SEL: result bytes [lo, 0, hi, 0]): with sign bit s and low bits u, 128 + u and
+// 128 + 128 s are both bf16 numbers, and b is their difference.
+template <uint32_t SEL>
+__device__ __forceinline__ uint32_t bytes_bf16(uint32_t w) {
+  const uint32_t r = __byte_perm(w, 0, SEL);
+  const uint32_t lo = (r & 0x007F007Fu) | 0x43004300u, hi = (r & 0x00800080u) | 0x43004300u;
+  const __nv_bfloat162 x = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&lo), *reinterpret_cast<const __nv_bfloat162*>(&hi));
+  return *reinterpret_cast<const uint32_t*>(&x);
 }
 
 }  // namespace phantom
