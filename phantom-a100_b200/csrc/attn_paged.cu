@@ -13,8 +13,8 @@
 //     [c W / G, (c + 1) W / G) of all W. Ragged lengths then cost nothing, and one long sequence spreads over the GPU. A
 //     unit that several CTAs share leaves partial results (fp32 rows, reference maximum, sum), which merge_rows joins in
 //     the order of the CTAs: the result depends on the lengths and the GPU's SM count alone.
-//   * One producer warp reads the page table and keeps a ring of tiles in flight by TMA (a box per page, swizzled, so that
-//     pages of 16 tokens land as one conflict-free tile); 160 KB in flight for each SM.
+//   * Two producer warps read the page table and keep a ring of tiles in flight by TMA (a box per page, swizzled, so that
+//     pages of 16 tokens land as one conflict-free tile); 128 KB in flight for each SM.
 //   * Eight consumer warps work without meeting: two to a tile, 32 keys each, every warp with its own running maximum,
 //     sum and output; they are joined through shared memory at the end of a unit.
 //
@@ -39,7 +39,7 @@ namespace rows {
 constexpr int BR = 16;        // query rows of a unit
 constexpr int BN = 64;        // keys of a tile
 constexpr int kConsumers = 8; // warps; pairs of them take the tiles in turn
-constexpr int kThreads = 32 * (kConsumers + 1);
+constexpr int kThreads = 32 * (kConsumers + 2);  // and two producers, of keys and of values
 constexpr int kErrCopyWait = 1, kErrTileWait = 4;
 
 template <int D, bool INT8>
@@ -48,7 +48,10 @@ struct Cfg {
   static constexpr int BLOCKS = INT8 ? 1 : D / 64;        // such blocks across d
   static constexpr int HALF = BN * D * (INT8 ? 1 : 2);    // keys (or values) of a tile
   static constexpr int SLOT = 2 * HALF;
-  static constexpr int SLOTS = INT8 ? (D == 128 ? 9 : 16) : (D == 128 ? 5 : 10);
+  // A multiple of the four pairs: a slot's tiles then all go to one pair, which sees every phase of its barriers. (With a
+  // slot passed between pairs, a pair could wait for a phase whose predecessor was still open, and parity would let it by.)
+  static constexpr int SLOTS = INT8 ? (D == 128 ? 8 : 16) : (D == 128 ? 4 : 8);
+  static_assert(SLOTS % 4 == 0, "each ring slot belongs to one pair of warps");
   static constexpr int OFF_MERGE = SLOTS * SLOT;          // [kConsumers][BR][D] fp32
   static constexpr int OFF_ML = OFF_MERGE + kConsumers * BR * D * 4;
   static constexpr int OFF_SCALE = OFF_ML + kConsumers * BR * 8;
@@ -123,8 +126,8 @@ attn_rows(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUten
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < C::SLOTS; ++s) {
-      mbar_init(full(s), 1);
-      mbar_init(empty(s), 2);
+      mbar_init(full(s), 2);   // the producers
+      mbar_init(empty(s), 2);  // the consuming pair
     }
     *abort_flag = 0;
     fence_mbar_init();
@@ -137,42 +140,46 @@ attn_rows(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUten
   w.start(p.s, p.blocks, blockIdx.x, gridDim.x);
   const int group = p.blocks.group, causal = p.blocks.causal;
   const long long begin = w.cur;
+  // Where token `row` of a tile has its column block `blk`: boxes of min(page, 64) tokens, each [block][token][ROW bytes].
+  const int box_log2 = min(p.s.page_log2, 6);
+  auto place_of = [&](int row, int blk) {
+    return C::BLOCKS == 1 ? row * C::ROW
+                          : ((((row >> box_log2) * C::BLOCKS + blk) << box_log2) + (row & ((1 << box_log2) - 1))) * C::ROW;
+  };
 
-  if (warp == kConsumers) {
-    // Producer: a tile's boxes (one per page and 64-column block, keys then values), and an 8-bit cache's scales.
-    if (lane == 0) {
-      tma_prefetch_desc(&tmK);
-      tma_prefetch_desc(&tmV);
-    }
+  if (warp >= kConsumers) {
+    // Producers, one of the keys and one of the values: a tile's boxes, one to a page, and an 8-bit cache's scales. One
+    // elected lane of warp-uniform code issues the copies; the issue is what limits pages of 16 tokens, hence two warps.
+    const bool vals = warp > kConsumers;
+    const CUtensorMap* map = vals ? &tmV : &tmK;
+    if (lane == 0) tma_prefetch_desc(map);
     int t = 0;
     bool ok = true;
+    const int page = 1 << p.s.page_log2, box = min(page, BN);
+    const Strides3 st = vals ? p.vss : p.kss;
+    const float* scale = vals ? p.vs : p.ks;
     while (ok && w.cur < w.end) {
       const int end = p.blocks.key_end(w.x, w.blk), cnt = w.count();
-      const int page = 1 << p.s.page_log2, box = min(page, BN);
       for (int i = 0; i < cnt; ++i, ++t) {
         const int s = t % C::SLOTS, round = t / C::SLOTS;
-        if (round > 0 && !(ok = __all_sync(0xffffffffu, mbar_wait(empty(s), (round - 1) & 1, abort_flag, p.s.status, kErrCopyWait))))
-          break;
         const int j0 = (w.tile + i) * BN;
         const int boxes = max(0, (min(j0 + BN, end) - j0 + box - 1) / box);  // pages of the tile that hold keys
-        constexpr int NC = 2 * C::BLOCKS;
-        int pg = lane < 16 ? lane / NC : (lane - 16) >> 1;
-        const bool copies = lane < boxes * NC, scales = INT8 && lane >= 16 && lane < 16 + 2 * boxes;
         int id = 0;
-        if (copies || scales) id = page_of(p.s, w.b, (j0 >> p.s.page_log2) + pg);
-        if (lane == 0) mbar_arrive_expect_tx(full(s), boxes * box * (2 * D * (INT8 ? 1 : 2) + (INT8 ? 8 : 0)));
-        __syncwarp();
+        if (lane < boxes) id = page_of(p.s, w.b, (j0 >> p.s.page_log2) + lane);
+        if (round > 0 && !(ok = __all_sync(0xffffffffu, mbar_wait(empty(s), (round - 1) & 1, abort_flag, p.s.status, kErrCopyWait))))
+          break;
         const int place = j0 & (page - 1);
-        if (copies) {
-          // an id that is out of range reads as zeros (the map's bounds)
-          const int c = lane % NC, blk = c >> 1;
-          const uint32_t dst = sbase + s * C::SLOT + (c & 1) * C::HALF + blk * BN * C::ROW + pg * box * C::ROW;
-          tma_load_4d(dst, (c & 1) ? &tmV : &tmK, full(s), blk * 64, place, w.h, id);
-        } else if (scales) {
-          const int v = lane & 1;
-          const Strides3& st = v ? p.vss : p.kss;
-          bulk_load(sbase + C::OFF_SCALE + (s * 2 + v) * BN * 4 + pg * box * 4,
-                    (v ? p.vs : p.ks) + max(id, 0) * st.page + w.h * st.head + place, box * 4, full(s));
+        const uint32_t dst = sbase + s * C::SLOT + (vals ? C::HALF : 0);
+        if (elect_one()) mbar_arrive_expect_tx(full(s), boxes * box * (D * (INT8 ? 1 : 2) + (INT8 ? 4 : 0)));
+        for (int pg = 0; pg < boxes; ++pg) {
+          const int from = __shfl_sync(0xffffffffu, id, pg);
+          if (elect_one()) {
+            // an id that is out of range reads as zeros (the map's bounds)
+            tma_load_5d(dst + pg * box * C::BLOCKS * C::ROW, map, full(s), 0, place, 0, w.h, from);
+            if constexpr (INT8)
+              bulk_load(sbase + C::OFF_SCALE + (s * 2 + vals) * BN * 4 + pg * box * 4,
+                        scale + max(from, 0) * st.page + w.h * st.head + place, box * 4, full(s));
+          }
         }
         __syncwarp();
       }
@@ -258,7 +265,7 @@ attn_rows(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUten
           for (int k = 0; k < D / 32; ++k) {
             uint32_t r[4];
             const int chunk = k * 4 + (lane >> 3);
-            ldsm4(kb + (chunk >> 3) * BN * 128 + row * 128 + (((chunk & 7) ^ (row & 7)) << 4), r);
+            ldsm4(kb + place_of(row, chunk >> 3) + (((chunk & 7) ^ (row & 7)) << 4), r);
             mma16816<BF16>(sc[n], qa[2 * k], r[0], r[1]);
             mma16816<BF16>(sc[n], qa[2 * k + 1], r[2], r[3]);
           }
@@ -383,7 +390,7 @@ attn_rows(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUten
           for (int c = 0; c < D / 16; ++c) {
             uint32_t r[4];
             const int chunk = 2 * c + (lane >> 4);
-            ldsm4_t(vb + (chunk >> 3) * BN * 128 + row * 128 + (((chunk & 7) ^ (row & 7)) << 4), r);
+            ldsm4_t(vb + place_of(row, chunk >> 3) + (((chunk & 7) ^ (row & 7)) << 4), r);
             if (tail) {
               r[0] &= keep[0];
               r[1] &= keep[1];
@@ -529,8 +536,8 @@ cudaError_t launch(const PagedAttnArgs& a, int dev) {
   }
   CUtensorMap mk, mv;
   const int page = 1 << a.s.page_log2, box = std::min(page, BN), elem = INT8 ? 1 : 2, cols = INT8 ? D : 64;
-  if (!make_paged_map(&mk, a.kc, a.s.num_pages, a.s.heads, page, D, a.kcs, elem, BF16, box, cols, 1) ||
-      !make_paged_map(&mv, a.vc, a.s.num_pages, a.s.heads, page, D, a.vcs, elem, BF16, box, cols, 1))
+  if (!make_paged_map(&mk, a.kc, a.s.num_pages, a.s.heads, page, D, a.kcs, elem, BF16, cols, box, C::BLOCKS, 1) ||
+      !make_paged_map(&mv, a.vc, a.s.num_pages, a.s.heads, page, D, a.vcs, elem, BF16, cols, box, C::BLOCKS, 1))
     return cudaErrorInvalidValue;
   const int ctas = sms;
   const size_t ml_bytes = (size_t)ctas * 2 * BR * sizeof(float2);

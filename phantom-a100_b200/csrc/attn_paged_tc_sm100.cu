@@ -27,7 +27,7 @@ namespace chunk {
 
 constexpr int BM = 128;  // rows of a query tile = TMEM lanes
 constexpr int BN = 128;  // keys of a tile
-constexpr int MMA_WARP = 8, TMA_WARP = 9, PV_WARP = 10;
+constexpr int MMA_WARP = 8, TMA_WARP = 9, PV_WARP = 10, V_WARP = 11;
 constexpr int kThreads = 384;
 // Register split, as in attn_tc_sm100.cu: 384 threads launch with 168 each; 128 * (168 - 72) = 2 * 128 * (216 - 168).
 constexpr int kRegsProducer = 72, kRegsSoftmax = 216;
@@ -236,86 +236,106 @@ attn_chunk(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUte
     return x;
   };
 
-  if (warp == TMA_WARP) {
+  if (warp == TMA_WARP || warp == V_WARP) {
     setmaxnreg_dec<kRegsProducer>();
-    // Producer, per unit: its record and queries, then keys and values of its tiles in turn.
-    if (lane == 0) {
-      tma_prefetch_desc(&tmQ);
-      tma_prefetch_desc(&tmK);
-      tma_prefetch_desc(&tmV);
+    // Producers: V_WARP copies the values, TMA_WARP the keys, and the units' records and queries. Each walks the CTA's
+    // share by itself. One elected lane of warp-uniform code issues the copies; their issue is what limits pages of 16
+    // tokens, hence two warps and, for the values, boxes of all columns (the tensor core takes V 16 keys at a time from
+    // anywhere, but K's 128 keys at one stride).
+    const bool vals = warp == V_WARP;
+    if (elect_one()) {
+      if (!vals) tma_prefetch_desc(&tmQ);
+      tma_prefetch_desc(vals ? &tmV : &tmK);
     }
     __syncwarp();
     Walk<TokenBlocks> w;
     w.start(p.s, p.blocks, blockIdx.x, gridDim.x);
     const long long begin = w.cur;
     const int page = 1 << p.s.page_log2, box = min(page, BN);
-    int t = 0, nu = 0, nq = 0;  // copies, units, phases of q_full begun
+    int t = vals, nu = 0, nq = 0;  // copies (keys even, values odd), units, phases of q_full begun
     bool ok = true;
-    for (;;) {
-      if (nu > 0 && !(ok = wait(q_free, (nu - 1) & 1, kErrTmaWait))) break;
-      if (nu > 1 && !(ok = wait(unit_read(nu), ((nu >> 1) - 1) & 1, kErrTmaWait))) break;
-      Unit x = {};
-      x.id = -1;
-      if (w.cur >= w.end) {
-        if (lane == 0) {
+    auto copy_tile = [&](int j0, int end) {
+      const int s = t % C::STAGES, round = t / C::STAGES;
+      const int boxes = max(0, (min(j0 + BN, end) - j0 + box - 1) / box);  // pages of the tile that hold keys
+      int id = 0;
+      if (lane < boxes) id = page_of(p.s, w.b, (j0 >> p.s.page_log2) + lane);
+      if (round > 0 && !(ok = wait(kv_empty(s), (round - 1) & 1, kErrTmaWait))) return;
+      const uint32_t dst = sbase + C::OFF_KV + s * C::TILE;
+      if (elect_one()) mbar_arrive_expect_tx(kv_full(s), boxes * box * D * 2);
+      for (int pg = 0; pg < boxes; ++pg) {
+        const int from = __shfl_sync(0xffffffffu, id, pg);
+        if (elect_one()) {  // an id that is out of range reads as zeros
+          if (vals) {
+            tma_load_5d(dst + pg * box * D * 2, &tmV, kv_full(s), 0, j0 & (page - 1), 0, w.h, from);
+          } else {
+#pragma unroll
+            for (int c = 0; c < C::KBLK; ++c)
+              tma_load_5d(dst + c * C::SUB + pg * box * 128, &tmK, kv_full(s), 0, j0 & (page - 1), c, w.h, from);
+          }
+        }
+      }
+      __syncwarp();
+      t += 2;
+    };
+    while (ok && w.cur < w.end) {
+      const int cnt = w.count(), end = p.blocks.key_end(w.x, w.blk);
+      int i = 0;
+      if (!vals) {
+        copy_tile(w.tile * BN, end);  // before the wait for the last unit's queries to be done with
+        i = 1;
+        if (ok && nu > 0) ok = wait(q_free, (nu - 1) & 1, kErrTmaWait);
+        if (ok && nu > 1) ok = wait(unit_read(nu), ((nu >> 1) - 1) & 1, kErrTmaWait);
+        if (!ok) break;
+        Unit x;
+        x.id = nu;
+        x.b = w.b;
+        x.h = w.h;
+        x.cnt = cnt;
+        x.tile0 = w.tile;
+        x.end = end;
+        x.tok = w.blk * p.blocks.per;
+        x.len = w.x.len, x.n = w.x.n, x.tok0 = w.x.tok0;
+        x.has_b = x.tok + p.tile_tokens < x.n;
+        x.slot = cnt == w.nt ? -1 : 2 * (int)blockIdx.x + (begin > w.cur - w.tile ? 0 : 1);
+        if (elect_one()) {
+          publish(nu, x);
+          const int tiles = x.has_b ? 2 : 1;
+          mbar_arrive_expect_tx(q_full(nu), tiles * C::KBLK * p.tile_tokens * p.group * 128);
+          for (int g = 0; g < tiles; ++g)
+            for (int c = 0; c < C::KBLK; ++c)
+              tma_load_5d(sbase + C::OFF_Q + g * C::TILE + c * C::SUB, &tmQ, q_full(nu), 0, 0, c, x.h,
+                          x.tok0 + x.tok + g * p.tile_tokens);
+        }
+        __syncwarp();
+        ++nu;
+        ++nq;
+      }
+      for (; ok && i < cnt; ++i) copy_tile((w.tile + i) * BN, end);
+      w.advance(p.s, p.blocks);
+    }
+    if (!vals && ok) {
+      // the end of the units
+      if (nu > 0) ok = wait(q_free, (nu - 1) & 1, kErrTmaWait);
+      if (ok && nu > 1) ok = wait(unit_read(nu), ((nu >> 1) - 1) & 1, kErrTmaWait);
+      if (ok) {
+        Unit x = {};
+        x.id = -1;
+        if (elect_one()) {
           publish(nu, x);
           mbar_arrive(q_full(nu));
         }
         __syncwarp();
         ++nq;
-        break;
       }
-      x.id = nu;
-      x.b = w.b;
-      x.h = w.h;
-      x.cnt = w.count();
-      x.tile0 = w.tile;
-      x.end = p.blocks.key_end(w.x, w.blk);
-      x.tok = w.blk * p.blocks.per;
-      x.len = w.x.len, x.n = w.x.n, x.tok0 = w.x.tok0;
-      x.has_b = x.tok + p.tile_tokens < x.n;
-      x.slot = x.cnt == w.nt ? -1 : 2 * (int)blockIdx.x + (begin > w.cur - w.tile ? 0 : 1);
-      if (lane == 0) {
-        publish(nu, x);
-        const int tiles = x.has_b ? 2 : 1;
-        mbar_arrive_expect_tx(q_full(nu), tiles * C::KBLK * p.tile_tokens * p.group * 128);
-        for (int g = 0; g < tiles; ++g)
-          for (int c = 0; c < C::KBLK; ++c)
-            tma_load_4d(sbase + C::OFF_Q + g * C::TILE + c * C::SUB, &tmQ, q_full(nu), c * 64, 0, x.h,
-                        x.tok0 + x.tok + g * p.tile_tokens);
-      }
-      __syncwarp();
-      ++nu;
-      ++nq;
-      for (int jt = 0; jt < 2 * x.cnt; ++jt, ++t) {
-        const int s = t % C::STAGES, round = t / C::STAGES;
-        const int j0 = (x.tile0 + (jt >> 1)) * BN;
-        const int boxes = max(0, (min(j0 + BN, x.end) - j0 + box - 1) / box);
-        const int pg = lane / C::KBLK, blk = lane % C::KBLK;
-        int id = 0;
-        if (lane < boxes * C::KBLK) id = page_of(p.s, x.b, (j0 >> p.s.page_log2) + pg);
-        if (round > 0 && !(ok = wait(kv_empty(s), (round - 1) & 1, kErrTmaWait))) break;
-        if (lane == 0) mbar_arrive_expect_tx(kv_full(s), boxes * box * D * 2);
-        __syncwarp();
-        if (lane < boxes * C::KBLK)  // an id that is out of range reads as zeros
-          tma_load_4d(sbase + C::OFF_KV + s * C::TILE + blk * C::SUB + pg * box * 128, (jt & 1) ? &tmV : &tmK, kv_full(s),
-                      blk * 64, j0 & (page - 1), x.h, id);
-        __syncwarp();
-      }
-      if (!ok) break;
-      w.advance(p.s, p.blocks);
     }
+    if (!ok) *abort_flag = 1;
     // every issued copy lands before this CTA's shared memory can be released
     for (int a = max(0, nq - 2); a < nq; ++a) mbar_wait_drain(q_full(a), (a >> 1) & 1);
-    if (!ok) *abort_flag = 1;
-    for (int i = max(0, t - C::STAGES); i < t; ++i) mbar_wait_drain(kv_full(i % C::STAGES), (i / C::STAGES) & 1);
-  } else if (warp == PV_WARP + 1) {
-    setmaxnreg_dec<kRegsProducer>();  // completes the warpgroup
+    for (int i = max((int)vals, t - C::STAGES); i < t; i += 2) mbar_wait_drain(kv_full(i % C::STAGES), (i / C::STAGES) & 1);
   } else if (warp == MMA_WARP || warp == PV_WARP) {
     setmaxnreg_dec<kRegsProducer>();
     const uint64_t dq = smem_desc_sw128(sbase + C::OFF_Q, 16, 1024);
     const uint64_t dk = smem_desc_sw128(sbase + C::OFF_KV, 16, 1024);
-    const uint64_t dv = smem_desc_sw128(sbase + C::OFF_KV, C::SUB, 1024);
     auto kv_wait = [&](int t) { return wait(kv_full(t % C::STAGES), (t / C::STAGES) & 1, kErrMmaWait); };
     if (warp == MMA_WARP) {
       // S_g = Q_g K^T, per key tile for query tile A, then B (see attn_tc_sm100.cu).
@@ -365,12 +385,18 @@ attn_chunk(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUte
     } else {
       // O_g += P_g V: P from TMEM, V as an MN-major operand.
       constexpr uint32_t idesc = idesc_f16(BF16, BM, D, true);
+      // V lies as boxes of `box` keys, [64-column block][key][128 bytes]
+      const int box_log2 = min(p.s.page_log2, 7), box = 1 << box_log2;
+      const uint64_t dv = smem_desc_sw128(sbase + C::OFF_KV, box * 128, 1024);
+      auto place_of = [&](int key, int blk) {
+        return ((((key >> box_log2) * C::KBLK + blk) << box_log2) + (key & (box - 1))) * 128;
+      };
       auto issue = [&](int g, int stage, bool acc) {
         const uint32_t b_off = (uint32_t)(stage * C::TILE) >> 4;
         const uint32_t d_t = tmem + (g ? C::T_O1 : C::T_O0), p_t = tmem + (g ? C::T_P1 : C::T_P0);
 #pragma unroll
         for (int kk = 0; kk < BN / 16; ++kk)
-          mma_ts(d_t, p_t + kk * 8, dv + (b_off + kk * (2048 >> 4)), idesc, (acc || kk > 0) ? 1u : 0u);
+          mma_ts(d_t, p_t + kk * 8, dv + (b_off + (place_of(kk * 16, 0) >> 4)), idesc, (acc || kk > 0) ? 1u : 0u);
       };
       int tb = 0, nu = 0;
       int pc[2] = {0, 0}, uc[2] = {0, 0};
@@ -385,7 +411,7 @@ attn_chunk(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUte
           if (j0 + BN > x.end) {  // zero the values of keys past the unit's end
             for (int i = max(0, x.end - j0) * 8 + lane; i < BN * 8; i += 32)
               for (int c = 0; c < C::KBLK; ++c)
-                st_shared_v4(sbase + C::OFF_KV + sv * C::TILE + c * C::SUB + i * 16, 0, 0, 0, 0);
+                st_shared_v4(sbase + C::OFF_KV + sv * C::TILE + place_of(i >> 3, c) + (i & 7) * 16, 0, 0, 0, 0);
             fence_proxy_async_smem();
             __syncwarp();
           }
@@ -632,9 +658,9 @@ cudaError_t launch(const PagedAttnArgs& a, int dev) {
   CUtensorMap mq, mk, mv;
   // queries as (packed token, key head, query head of it, d), boxes of one key head's rows of a tile
   const Strides3 qs{a.q_token, a.q_head * a.group, a.q_head};
-  if (!make_paged_map(&mk, a.kc, a.s.num_pages, a.s.heads, page, D, a.kcs, 2, BF16, box, 64, 1) ||
-      !make_paged_map(&mv, a.vc, a.s.num_pages, a.s.heads, page, D, a.vcs, 2, BF16, box, 64, 1) ||
-      !make_paged_map(&mq, a.q, a.s.total, a.s.heads, a.group, D, qs, 2, BF16, a.group, 64, tile_tokens))
+  if (!make_paged_map(&mk, a.kc, a.s.num_pages, a.s.heads, page, D, a.kcs, 2, BF16, 64, box, 1, 1) ||
+      !make_paged_map(&mv, a.vc, a.s.num_pages, a.s.heads, page, D, a.vcs, 2, BF16, 64, box, C::KBLK, 1) ||
+      !make_paged_map(&mq, a.q, a.s.total, a.s.heads, a.group, D, qs, 2, BF16, 64, a.group, 1, tile_tokens))
     return cudaErrorInvalidValue;
   const size_t ml_bytes = (size_t)ctas * 4 * BM * sizeof(float2);
   void* block = nullptr;

@@ -46,6 +46,7 @@
 
 #include <algorithm>
 #include <atomic>
+#include <cstring>
 #include <mutex>
 
 #include "launchers.h"
@@ -1392,12 +1393,15 @@ cudaError_t scratch_alloc(int dev, size_t bytes, cudaStream_t stream, void** out
 namespace {
 
 // Per-thread cache of the paged maps, as for the contiguous ones above (a map is a pure function of its key).
+struct PagedMapKey {
+  const void* base;
+  long long st[3];
+  int num[4], box[4], elem, bf16;
+};
 struct PagedMapEntry {
   CUtensorMap map;
-  const void* base = nullptr;
-  int pages = 0, heads = 0, page = 0, d = 0, elem = 0, rows = 0, cols = 0, per_box = 0;
-  Strides3 st{};
-  bool bf16 = false, valid = false;
+  PagedMapKey key;
+  bool valid = false;
 };
 thread_local PagedMapEntry g_paged_maps[kMapCache];
 thread_local int g_paged_next = 0;
@@ -1405,35 +1409,34 @@ thread_local int g_paged_next = 0;
 }  // namespace
 
 bool make_paged_map(void* out, const void* base, int num_pages, int heads, int page, int d, const Strides3& st, int elem,
-                    bool bf16, int rows, int cols, int pages_per_box) {
+                    bool bf16, int cols, int rows, int blocks, int pages) {
   CUtensorMap* m = static_cast<CUtensorMap*>(out);
+  PagedMapKey key;
+  memset(&key, 0, sizeof(key));  // compared as bytes
+  key = PagedMapKey{base, {st.page, st.head, st.token}, {num_pages, heads, page, d}, {cols, rows, blocks, pages}, elem, bf16};
   for (const PagedMapEntry& e : g_paged_maps)
-    if (e.valid && e.base == base && e.pages == num_pages && e.heads == heads && e.page == page && e.d == d &&
-        e.elem == elem && e.rows == rows && e.cols == cols && e.per_box == pages_per_box && e.bf16 == bf16 && e.st.page == st.page &&
-        e.st.head == st.head && e.st.token == st.token) {
+    if (e.valid && memcmp(&e.key, &key, sizeof(key)) == 0) {
       *m = e.map;
       return true;
     }
   EncodeTiledFn fn = encode_fn();
   if (!fn) return false;
-  const cuuint64_t dims[4] = {(cuuint64_t)d, (cuuint64_t)page, (cuuint64_t)heads, (cuuint64_t)num_pages};
-  const cuuint64_t strides[3] = {(cuuint64_t)st.token * elem, (cuuint64_t)st.head * elem, (cuuint64_t)st.page * elem};
-  const cuuint32_t box[4] = {(cuuint32_t)cols, (cuuint32_t)rows, 1, (cuuint32_t)pages_per_box};
-  const cuuint32_t estr[4] = {1, 1, 1, 1};
+  const cuuint64_t dims[5] = {(cuuint64_t)cols, (cuuint64_t)page, (cuuint64_t)(d / cols), (cuuint64_t)heads, (cuuint64_t)num_pages};
+  const cuuint64_t strides[4] = {(cuuint64_t)st.token * elem, (cuuint64_t)cols * elem, (cuuint64_t)st.head * elem,
+                                 (cuuint64_t)st.page * elem};
+  const cuuint32_t box[5] = {(cuuint32_t)cols, (cuuint32_t)rows, (cuuint32_t)blocks, 1, (cuuint32_t)pages};
+  const cuuint32_t estr[5] = {1, 1, 1, 1, 1};
   const CUtensorMapDataType type = elem == 1 ? CU_TENSOR_MAP_DATA_TYPE_UINT8
                                    : bf16    ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
                                              : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
-  if (fn(m, type, 4, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+  if (fn(m, type, 5, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
          cols * elem == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
          CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
     return false;
   PagedMapEntry& e = g_paged_maps[g_paged_next];
   g_paged_next = (g_paged_next + 1) % kMapCache;
   e.map = *m;
-  e.base = base;
-  e.pages = num_pages, e.heads = heads, e.page = page, e.d = d, e.elem = elem, e.rows = rows, e.cols = cols, e.per_box = pages_per_box;
-  e.st = st;
-  e.bf16 = bf16;
+  memcpy(&e.key, &key, sizeof(key));
   e.valid = true;
   return true;
 }

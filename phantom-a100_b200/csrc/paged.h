@@ -62,9 +62,10 @@ cudaError_t launch_paged_attn_chunk(const PagedAttnArgs& a, int dev);
 cudaError_t sm_count(int dev, int* n);
 // Stream-ordered scratch from the library's pool of device `dev`, released with cudaFreeAsync on the same stream.
 cudaError_t scratch_alloc(int dev, size_t bytes, cudaStream_t stream, void** out);
-// TMA map of a (page, head, token, d) cache: boxes of `pages_per_box` pages, one head, `rows` tokens and `cols` elements of
-// `elem` bytes, swizzled over the box's inner `cols * elem` bytes (64 or 128).
+// TMA map of a (page, head, token, d) cache as (columns of a swizzled row, token, block of such columns, head, page): boxes
+// of `cols` elements of `elem` bytes (64 or 128 bytes, the swizzle's width) by `rows` tokens by `blocks` column blocks of
+// one head and `pages` pages.
 bool make_paged_map(void* map, const void* base, int num_pages, int heads, int page, int d, const Strides3& st, int elem,
-                    bool bf16, int rows, int cols, int pages_per_box);
+                    bool bf16, int cols, int rows, int blocks, int pages);
 
 }  // namespace phantom
