@@ -7,12 +7,15 @@
 // values once: 2 len d elements for each key head against 2 * 2 len d operations for each query row, so with up to 16 rows
 // it is bound by memory, and everything here serves the reads:
 //
-//   * The rows of one key head (new tokens x its query heads, token-major) are taken 16 at a time, the height of a warp's
-//     matrix instruction: the keys are read once for all of them.
-//   * Work is cut evenly: all (sequence, head, row block) units in a row, tiles of 64 keys, and CTA c of G takes tiles
-//     [c W / G, (c + 1) W / G) of all W. Ragged lengths then cost nothing, and one long sequence spreads over the GPU. A
-//     unit that several CTAs share leaves partial results (fp32 rows, reference maximum, sum), which merge_rows joins in
-//     the order of the CTAs: the result depends on the lengths and the GPU's SM count alone.
+//   * Queries are the narrow operand. The matrix instruction takes 16 keys by 16 of d from shared memory against 8 query
+//     rows (new tokens x query heads of one key head, token-major) held in registers: scores come out as keys x queries,
+//     are turned around by movmatrix, and meet V^T the same way. With queries as the 16-high operand a group of 4 or 8
+//     heads left half of every instruction and of the softmax unused (16 contexts of 4096 tokens, 8 key heads: 812
+//     instructions for each 32 keys and warp, against 310).
+//   * Work is cut evenly: all (sequence, head, row block) units in a row, tiles of 64 keys, and every CTA takes its share
+//     (paged_dev.cuh). Ragged lengths then cost nothing, and one long sequence spreads over the GPU. The parts of a unit
+//     that several CTAs share (fp32 rows, reference maximum, sum) are joined in the order of the CTAs by the one that
+//     finishes last: the result depends on the lengths and the GPU's SM count alone.
 //   * Two producer warps read the page table and keep a ring of tiles in flight by TMA (a box per page, swizzled, so that
 //     pages of 16 tokens land as one conflict-free tile); 128 KB in flight for each SM.
 //   * Eight consumer warps work without meeting: two to a tile, 32 keys each, every warp with its own running maximum,
@@ -36,14 +39,15 @@
 namespace phantom {
 namespace rows {
 
-constexpr int BR = 16;        // query rows of a unit
+// A unit has 8 NT query rows (NT = 1, 2).
 constexpr int BN = 64;        // keys of a tile
 constexpr int kConsumers = 8; // warps; pairs of them take the tiles in turn
 constexpr int kThreads = 32 * (kConsumers + 2);  // and two producers, of keys and of values
 constexpr int kErrCopyWait = 1, kErrTileWait = 4;
 
-template <int D, bool INT8>
+template <int D, bool INT8, int NT>
 struct Cfg {
+  static constexpr int BR = 8 * NT;
   static constexpr int ROW = INT8 ? D : 128;              // bytes of a swizzled row (16-bit: 64 columns)
   static constexpr int BLOCKS = INT8 ? 1 : D / 64;        // such blocks across d
   static constexpr int HALF = BN * D * (INT8 ? 1 : 2);    // keys (or values) of a tile
@@ -63,10 +67,11 @@ struct Cfg {
 
 
 // ------------------------------------------------------------------------------------------------ units and tiles
-// Units of 16 rows; tiles of 64 keys.
+// Units of 8 NT rows; tiles of 64 keys.
+template <int NT>
 struct RowBlocks {
   int group, causal, heads;
-  static constexpr int kTile = BN;
+  static constexpr int kTile = BN, BR = 8 * NT;
   __device__ int count(const Seq& x) const { return (x.n * group + BR - 1) / BR; }
   __device__ int key_end(const Seq& x, int rb) const {
     if (!causal) return x.len;
@@ -76,6 +81,7 @@ struct RowBlocks {
   __device__ long long head_tiles(const Seq& x) const { return sum_tiles(*this, x); }
 };
 
+template <int NT>
 struct Params {
   PagedSeqs s;
   const uint16_t* q;
@@ -83,10 +89,13 @@ struct Params {
   uint16_t* o;
   const float *ks, *vs;
   Strides3 kss, vss;
-  RowBlocks blocks;
-  float scale_log2;
-  float* part;  // partial results, [CTA][2][BR] rows of D sums of values
-  float2* ml;   // their (reference maximum, sum)
+  RowBlocks<NT> blocks;
+  float scale_log2;  // of the scores' size
+  uint32_t flip;     // sign bits to flip in the queries (a negative scale)
+  float* part;       // parts of shared units, [place][8 NT] rows of D sums of values
+  float2* ml;        // their (reference maximum, sum)
+  unsigned long long* flags;
+  unsigned long long call;
 };
 
 // ------------------------------------------------------------------------------------------------ matrix instructions
@@ -111,11 +120,18 @@ __device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], 
 }
 
 __device__ __forceinline__ void consumers_meet() { asm volatile("bar.sync 1, 256;" ::: "memory"); }
+// Transposes the 8 x 8 matrix of 16-bit numbers that a warp holds (lane 4 r + c: row r, columns 2 c and 2 c + 1).
+__device__ __forceinline__ uint32_t turn(uint32_t x) {
+  uint32_t y;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
+}
 
-template <int D, bool BF16, bool INT8>
+template <int D, bool BF16, bool INT8, int NT>
 __global__ void __launch_bounds__(kThreads, 1)
-attn_rows(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV, const Params p) {
-  using C = Cfg<D, INT8>;
+attn_rows(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV, const Params<NT> p) {
+  using C = Cfg<D, INT8, NT>;
+  constexpr int BR = C::BR;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   const uint32_t sbase = smem_u32(smem);
@@ -136,17 +152,10 @@ attn_rows(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUten
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   asm volatile("griddepcontrol.wait;" ::: "memory");
 
-  Walk<RowBlocks> w;
+  Walk<RowBlocks<NT>> w;
   w.start(p.s, p.blocks, blockIdx.x, gridDim.x);
   const int group = p.blocks.group, causal = p.blocks.causal;
   const long long begin = w.cur;
-  // Where token `row` of a tile has its column block `blk`: boxes of min(page, 64) tokens, each [block][token][ROW bytes].
-  const int box_log2 = min(p.s.page_log2, 6);
-  auto place_of = [&](int row, int blk) {
-    return C::BLOCKS == 1 ? row * C::ROW
-                          : ((((row >> box_log2) * C::BLOCKS + blk) << box_log2) + (row & ((1 << box_log2) - 1))) * C::ROW;
-  };
-
   if (warp >= kConsumers) {
     // Producers, one of the keys and one of the values: a tile's boxes, one to a page, and an 8-bit cache's scales. One
     // elected lane of warp-uniform code issues the copies; the issue is what limits pages of 16 tokens, hence two warps.
@@ -194,40 +203,64 @@ attn_rows(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUten
   const int pair = warp >> 1, kr = (warp & 1) * 32;  // this warp's keys of its pair's tiles
   float* merge = reinterpret_cast<float*>(smem + C::OFF_MERGE);
   float2* ml = reinterpret_cast<float2*>(smem + C::OFF_ML);
+  // Where this lane's rows for ldmatrix lie in a tile: 16 keys from kr + 16 mt, matrices (keys 0-7, 8-15) x (first, second
+  // 16-byte chunk of a pair); V^T of 16-bit values has the two the other way around. Boxes of min(page, 64) tokens, each
+  // [64-column block][token][ROW bytes]; a chunk lies at its number ^ the row's swizzle, so stepping over pairs of chunks
+  // is an XOR with 32 times the pair's number.
+  const int box_log2 = min(p.s.page_log2, 6), blk_stride = C::ROW << box_log2;
+  uint32_t at_k[2], at_v[2];
+#pragma unroll
+  for (int mt = 0; mt < 2; ++mt) {
+    auto place_of = [&](int key, int chunk) {
+      const int row = C::BLOCKS == 1 ? key : (((key >> box_log2) * C::BLOCKS) << box_log2) + (key & ((1 << box_log2) - 1));
+      const int sw = C::ROW == 128 ? key & 7 : (key >> 1) & 3;
+      return (uint32_t)(row * C::ROW + ((chunk ^ sw) << 4));
+    };
+    const int key = kr + mt * 16 + (lane & 7);
+    at_k[mt] = place_of(key + ((lane >> 3) & 1) * 8, lane >> 4);
+    at_v[mt] = INT8 ? at_k[mt] : place_of(key + (lane >> 4) * 8, (lane >> 3) & 1);
+  }
   int t = 0;
   bool ok = true;
   while (w.cur < w.end) {
     const Seq x = w.x;
     const int cnt = w.count(), R = x.n * group, row0 = w.blk * BR, off = x.len - x.n;
     const int end = p.blocks.key_end(x, w.blk);
-    // the A operand of the rows g, g + 8; 8-bit caches: columns in the order that their bytes come in (4 t4 ... + 3 of 16)
-    uint32_t qa[D / 16][4];
-    int lim[2];
+    // the queries as B operands: of row 8 nt + g; 8-bit caches: columns in the order that their bytes come in (4 t4 ... + 3
+    // of 16). Keys that the rows 8 nt + 2 t4 + e of this lane's scores see.
+    uint32_t qb[NT][D / 16][2];
+    int lim[NT][2];
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const int r = row0 + g + 8 * i;
-      lim[i] = r >= R ? 0 : causal ? min(x.len, off + r / group + 1) : x.len;
+    for (int nt = 0; nt < NT; ++nt) {
+      const int r = row0 + nt * 8 + g;
       const uint16_t* src = p.q + (x.tok0 + (r < R ? r / group : 0)) * p.q_token +
                             (w.h * group + (r < R ? r % group : 0)) * p.q_head;
 #pragma unroll
       for (int k = 0; k < D / 16; ++k) {
         if constexpr (INT8) {
           const uint2 y = *reinterpret_cast<const uint2*>(src + k * 16 + 4 * t4);
-          qa[k][i] = r < R ? y.x : 0u;
-          qa[k][2 + i] = r < R ? y.y : 0u;
+          qb[nt][k][0] = r < R ? y.x : 0u;
+          qb[nt][k][1] = r < R ? y.y : 0u;
         } else {
-          qa[k][i] = r < R ? *reinterpret_cast<const uint32_t*>(src + k * 16 + 2 * t4) : 0u;
-          qa[k][2 + i] = r < R ? *reinterpret_cast<const uint32_t*>(src + k * 16 + 8 + 2 * t4) : 0u;
+          qb[nt][k][0] = r < R ? *reinterpret_cast<const uint32_t*>(src + k * 16 + 2 * t4) ^ p.flip : 0u;
+          qb[nt][k][1] = r < R ? *reinterpret_cast<const uint32_t*>(src + k * 16 + 8 + 2 * t4) ^ p.flip : 0u;
         }
+      }
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const int row = row0 + nt * 8 + 2 * t4 + e;
+        lim[nt][e] = row >= R ? 0 : causal ? min(x.len, off + row / group + 1) : x.len;
       }
     }
     const int lim_least = causal ? max(0, min(x.len, off + row0 / group + 1)) : x.len;  // of the block's rows
-    float m[2] = {-CUDART_INF_F, -CUDART_INF_F}, l[2] = {0.f, 0.f};
-    float o[D / 8][4];
+    float m[NT][2], l[NT][2], o[D / 16][NT][4];
 #pragma unroll
-    for (int n = 0; n < D / 8; ++n)
+    for (int nt = 0; nt < NT; ++nt) {
+      m[nt][0] = m[nt][1] = -CUDART_INF_F;
+      l[nt][0] = l[nt][1] = 0.f;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) o[n][e] = 0.f;
+      for (int c = 0; c < D / 16; ++c) o[c][nt][0] = o[c][nt][1] = o[c][nt][2] = o[c][nt][3] = 0.f;
+    }
 
     for (int i = 0; i < cnt; ++i, ++t) {
       if ((t & 3) != pair) continue;
@@ -237,173 +270,178 @@ attn_rows(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUten
       const uint32_t kb = sbase + s * C::SLOT, vb = kb + C::HALF;
       const int j0 = (w.tile + i) * BN + kr;  // this warp's first key
       if (j0 < end) {
-      // ---- scores: [4 groups of 8 keys][row g: keys 2 t4, + 1; row g + 8: the same]
-      float sc[4][4];
+        // ---- scores: [16 keys][8 rows]: (key g: rows 2 t4, + 1; key g + 8: the same)
+        float sc[2][NT][4];
 #pragma unroll
-      for (int n = 0; n < 4; ++n) {
+        for (int mt = 0; mt < 2; ++mt) {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) sc[n][e] = 0.f;
-        const int row = kr + n * 8 + (lane & 7);
-        if constexpr (INT8) {
-          const int sw = D == 128 ? row & 7 : (row >> 1) & 3;
+          for (int nt = 0; nt < NT; ++nt) sc[mt][nt][0] = sc[mt][nt][1] = sc[mt][nt][2] = sc[mt][nt][3] = 0.f;
+          if constexpr (INT8) {
 #pragma unroll
-          for (int k = 0; k < D / 64; ++k) {
-            uint32_t r[4];
-            ldsm4(kb + row * C::ROW + (((k * 4 + (lane >> 3)) ^ sw) << 4), r);
+            for (int k = 0; k < D / 32; ++k) {
+              uint32_t r[4], a[2][4];
+              ldsm4(kb + (at_k[mt] ^ (k << 5)), r);
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              if constexpr (BF16) {
-                mma16816<true>(sc[n], qa[k * 4 + e], bytes_bf16<0x4140>(r[e]), bytes_bf16<0x4342>(r[e]));
-              } else {
-                const uint32_t u = r[e] ^ 0x80808080u;
-                mma16816<false>(sc[n], qa[k * 4 + e], bytes_f16<0x4140>(u), bytes_f16<0x4342>(u));
+              for (int e = 0; e < 4; ++e) {  // r: (keys 0-7, 8-15) of chunk 2 k, then of 2 k + 1
+                if constexpr (BF16) {
+                  a[e >> 1][e & 1] = bytes_bf16<0x4140>(r[e]);
+                  a[e >> 1][2 + (e & 1)] = bytes_bf16<0x4342>(r[e]);
+                } else {
+                  const uint32_t u = r[e] ^ 0x80808080u;
+                  a[e >> 1][e & 1] = bytes_f16<0x4140>(u);
+                  a[e >> 1][2 + (e & 1)] = bytes_f16<0x4342>(u);
+                }
+              }
+#pragma unroll
+              for (int nt = 0; nt < NT; ++nt) {
+                mma16816<BF16>(sc[mt][nt], a[0], qb[nt][2 * k][0], qb[nt][2 * k][1]);
+                mma16816<BF16>(sc[mt][nt], a[1], qb[nt][2 * k + 1][0], qb[nt][2 * k + 1][1]);
               }
             }
-          }
-        } else {
-#pragma unroll
-          for (int k = 0; k < D / 32; ++k) {
-            uint32_t r[4];
-            const int chunk = k * 4 + (lane >> 3);
-            ldsm4(kb + place_of(row, chunk >> 3) + (((chunk & 7) ^ (row & 7)) << 4), r);
-            mma16816<BF16>(sc[n], qa[2 * k], r[0], r[1]);
-            mma16816<BF16>(sc[n], qa[2 * k + 1], r[2], r[3]);
-          }
-        }
-      }
-      // ---- to the log2 domain; masks
-      float vsc[4][2];  // 8-bit: the values' scales, then their reciprocals
-      if constexpr (INT8) {
-        const float* scl = reinterpret_cast<const float*>(smem + C::OFF_SCALE + s * 2 * BN * 4) + kr + 2 * t4;
-#pragma unroll
-        for (int n = 0; n < 4; ++n) {
-          const float2 a = *reinterpret_cast<const float2*>(scl + n * 8), v = *reinterpret_cast<const float2*>(scl + BN + n * 8);
-          const float k0 = a.x * p.scale_log2, k1 = a.y * p.scale_log2, l0 = __log2f(v.x), l1 = __log2f(v.y);
-          sc[n][0] = fmaf(sc[n][0], k0, l0);
-          sc[n][1] = fmaf(sc[n][1], k1, l1);
-          sc[n][2] = fmaf(sc[n][2], k0, l0);
-          sc[n][3] = fmaf(sc[n][3], k1, l1);
-          vsc[n][0] = v.x;
-          vsc[n][1] = v.y;
-        }
-      } else {
-#pragma unroll
-        for (int n = 0; n < 4; ++n)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) sc[n][e] *= p.scale_log2;
-      }
-      if (j0 + 32 > lim_least) {
-#pragma unroll
-        for (int n = 0; n < 4; ++n)
-#pragma unroll
-          for (int e = 0; e < 4; ++e)
-            if (j0 + n * 8 + 2 * t4 + (e & 1) >= lim[e >> 1]) sc[n][e] = -CUDART_INF_F;
-      }
-      // ---- running maximum
-      float alpha[2], sub[2];
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        float y = -CUDART_INF_F;
-#pragma unroll
-        for (int n = 0; n < 4; ++n) y = fmaxf(y, fmaxf(sc[n][2 * h], sc[n][2 * h + 1]));
-        y = fmaxf(y, __shfl_xor_sync(0xffffffffu, y, 1));
-        y = fmaxf(y, __shfl_xor_sync(0xffffffffu, y, 2));
-        y = fmaxf(y, m[h]);
-        sub[h] = y == -CUDART_INF_F ? 0.f : y;
-        alpha[h] = ex2(m[h] - sub[h]);  // 0 while no key was seen
-        m[h] = y;
-        l[h] *= alpha[h];
-      }
-      if (__any_sync(0xffffffffu, alpha[0] != 1.f || alpha[1] != 1.f)) {
-#pragma unroll
-        for (int n = 0; n < D / 8; ++n) {
-          o[n][0] *= alpha[0];
-          o[n][1] *= alpha[0];
-          o[n][2] *= alpha[1];
-          o[n][3] *= alpha[1];
-        }
-      }
-      // ---- probabilities
-      uint32_t hi[2][4], lo[2][4];
-#pragma unroll
-      for (int n = 0; n < 4; ++n) {
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const float a = ex2(sc[n][2 * h] - sub[h]), c = ex2(sc[n][2 * h + 1] - sub[h]);
-          if constexpr (INT8) {
-            // masked keys: p' = 0 (their scales may be anything)
-            l[h] += (a > 0.f ? __fdividef(a, vsc[n][0]) : a) + (c > 0.f ? __fdividef(c, vsc[n][1]) : c);
-            hi[n >> 1][(n & 1) * 2 + h] = pack2<false>(a, c);
           } else {
-            l[h] += a + c;
-            const uint32_t y = pack2<BF16>(a, c);
-            hi[n >> 1][(n & 1) * 2 + h] = y;
-            float2 f;
-            if constexpr (BF16)
-              f = make_float2(__uint_as_float(y << 16), __uint_as_float(y & 0xFFFF0000u));
-            else
-              f = __half22float2(*reinterpret_cast<const __half2*>(&y));
-            lo[n >> 1][(n & 1) * 2 + h] = pack2<BF16>(a - f.x, c - f.y);
+#pragma unroll
+            for (int k = 0; k < D / 16; ++k) {
+              uint32_t r[4];
+              ldsm4(kb + (k >> 2) * blk_stride + (at_k[mt] ^ ((k & 3) << 5)), r);
+#pragma unroll
+              for (int nt = 0; nt < NT; ++nt) mma16816<BF16>(sc[mt][nt], r, qb[nt][k][0], qb[nt][k][1]);
+            }
           }
         }
-      }
-      // ---- values; those of keys past the end are zeroed (what lies in the page there may be anything)
-      const bool tail = j0 + 32 > end;
-      if constexpr (INT8) {
-        uint32_t keep[4];
+        // ---- 8-bit: to the log2 domain, with the values' scales; masks
+        float inv_vs[2][2];
+        if constexpr (INT8) {
+          const float* scl = reinterpret_cast<const float*>(smem + C::OFF_SCALE + s * 2 * BN * 4) + kr + g;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int j = j0 + e * 8 + 2 * t4;
-          keep[e] = tail ? (j < end ? 0xffffu : 0u) | (j + 1 < end ? 0xffff0000u : 0u) : 0xffffffffu;
+          for (int mt = 0; mt < 2; ++mt)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              const float a = scl[mt * 16 + e * 8] * p.scale_log2, v = scl[BN + mt * 16 + e * 8], lv = __log2f(v);
+              // past the end a scale may be anything; p' is 0 there
+              inv_vs[mt][e] = j0 + mt * 16 + e * 8 + g < end ? __fdividef(1.f, v) : 0.f;
+#pragma unroll
+              for (int nt = 0; nt < NT; ++nt) {
+                sc[mt][nt][2 * e] = fmaf(sc[mt][nt][2 * e], a, lv);
+                sc[mt][nt][2 * e + 1] = fmaf(sc[mt][nt][2 * e + 1], a, lv);
+              }
+            }
         }
-        const int row = kr + (lane >> 3) * 8 + (lane & 7);
-        const int sw = D == 128 ? row & 7 : (row >> 1) & 3;
+        if (j0 + 32 > lim_least) {
 #pragma unroll
-        for (int c = 0; c < D / 16; ++c) {
-          uint32_t r[4];
-          ldsm4_t(vb + row * C::ROW + ((c ^ sw) << 4), r);
-          uint32_t ev[4], od[4];
+          for (int mt = 0; mt < 2; ++mt)
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const uint32_t u = (r[e] & keep[e]) ^ 0x80808080u;
-            ev[e] = bytes_f16<0x4240>(u);
-            od[e] = bytes_f16<0x4341>(u);
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+              for (int e = 0; e < 4; ++e)
+                if (j0 + mt * 16 + (e >> 1) * 8 + g >= lim[nt][e & 1]) sc[mt][nt][e] = -CUDART_INF_F;
+        }
+        // ---- running maximum of each row, over the lanes of one t4
+        const float scale = INT8 ? 1.f : p.scale_log2;
+        float2 sub[NT], alpha[NT];
+        bool grew = false;
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            float y = fmaxf(fmaxf(sc[0][nt][e], sc[0][nt][2 + e]), fmaxf(sc[1][nt][e], sc[1][nt][2 + e]));
+            y = fmaxf(y, __shfl_xor_sync(0xffffffffu, y, 4));
+            y = fmaxf(y, __shfl_xor_sync(0xffffffffu, y, 8));
+            y = fmaxf(y, __shfl_xor_sync(0xffffffffu, y, 16));
+            y = fmaxf(y * scale, m[nt][e]);
+            const float ref = y == -CUDART_INF_F ? 0.f : y, al = ex2(m[nt][e] - ref);  // 0 while no key was seen
+            grew |= y != m[nt][e];
+            m[nt][e] = y;
+            l[nt][e] *= al;
+            if (e == 0) sub[nt].x = -ref, alpha[nt].x = al;
+            else sub[nt].y = -ref, alpha[nt].y = al;
           }
-          mma16816<false>(o[2 * c], hi[0], ev[0], ev[1]);
-          mma16816<false>(o[2 * c], hi[1], ev[2], ev[3]);
-          mma16816<false>(o[2 * c + 1], hi[0], od[0], od[1]);
-          mma16816<false>(o[2 * c + 1], hi[1], od[2], od[3]);
         }
-      } else {
+        if (__any_sync(0xffffffffu, grew)) {
 #pragma unroll
-        for (int ks = 0; ks < 2; ++ks) {
+          for (int c = 0; c < D / 16; ++c)
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+              const float2 a = mul2(make_float2(o[c][nt][0], o[c][nt][1]), alpha[nt]);
+              const float2 b = mul2(make_float2(o[c][nt][2], o[c][nt][3]), alpha[nt]);
+              o[c][nt][0] = a.x, o[c][nt][1] = a.y, o[c][nt][2] = b.x, o[c][nt][3] = b.y;
+            }
+        }
+        // ---- probabilities, turned into B operands (16 keys by 8 rows)
+        uint32_t hi[2][NT][2], lo[2][NT][2];
+#pragma unroll
+        for (int mt = 0; mt < 2; ++mt)
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              float2 y = fma2(make_float2(sc[mt][nt][2 * e], sc[mt][nt][2 * e + 1]), make_float2(scale, scale), sub[nt]);
+              y.x = ex2(y.x);
+              y.y = ex2(y.y);
+              if constexpr (INT8) {
+                l[nt][0] = fmaf(y.x, inv_vs[mt][e], l[nt][0]);
+                l[nt][1] = fmaf(y.y, inv_vs[mt][e], l[nt][1]);
+                hi[mt][nt][e] = turn(pack2<false>(y.x, y.y));
+              } else {
+                l[nt][0] += y.x;
+                l[nt][1] += y.y;
+                const uint32_t h = pack2<BF16>(y.x, y.y);
+                float2 f;
+                if constexpr (BF16)
+                  f = make_float2(__uint_as_float(h << 16), __uint_as_float(h & 0xFFFF0000u));
+                else
+                  f = __half22float2(*reinterpret_cast<const __half2*>(&h));
+                hi[mt][nt][e] = turn(h);
+                lo[mt][nt][e] = turn(pack2<BF16>(y.x - f.x, y.y - f.y));
+              }
+            }
+        // ---- values; those of keys past the end are zeroed (what lies in the page there may be anything)
+        const bool tail = j0 + 32 > end;
+#pragma unroll
+        for (int mt = 0; mt < 2; ++mt) {
           uint32_t keep[2] = {0xffffffffu, 0xffffffffu};
           if (tail) {
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
-              const int j = j0 + ks * 16 + e * 8 + 2 * t4;
+              const int j = j0 + mt * 16 + e * 8 + 2 * t4;
               keep[e] = (j < end ? 0xffffu : 0u) | (j + 1 < end ? 0xffff0000u : 0u);
             }
           }
-          const int row = kr + ks * 16 + ((lane >> 3) & 1) * 8 + (lane & 7);
+          if constexpr (INT8) {
 #pragma unroll
-          for (int c = 0; c < D / 16; ++c) {
-            uint32_t r[4];
-            const int chunk = 2 * c + (lane >> 4);
-            ldsm4_t(vb + place_of(row, chunk >> 3) + (((chunk & 7) ^ (row & 7)) << 4), r);
-            if (tail) {
-              r[0] &= keep[0];
-              r[1] &= keep[1];
-              r[2] &= keep[0];
-              r[3] &= keep[1];
+            for (int c = 0; c < D / 32; ++c) {
+              uint32_t r[4], a[2][4];
+              ldsm4_t(vb + (at_v[mt] ^ (c << 5)), r);
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {  // r: (keys 0-7, 8-15) of columns 32 c ... + 15, then ... + 31; even and odd columns
+                const uint32_t u = (tail ? r[e] & keep[e & 1] : r[e]) ^ 0x80808080u;
+                a[e >> 1][2 * (e & 1)] = bytes_f16<0x4240>(u);
+                a[e >> 1][2 * (e & 1) + 1] = bytes_f16<0x4341>(u);
+              }
+#pragma unroll
+              for (int nt = 0; nt < NT; ++nt) {
+                mma16816<false>(o[2 * c][nt], a[0], hi[mt][nt][0], hi[mt][nt][1]);
+                mma16816<false>(o[2 * c + 1][nt], a[1], hi[mt][nt][0], hi[mt][nt][1]);
+              }
             }
-            mma16816<BF16>(o[2 * c], hi[ks], r[0], r[1]);
-            mma16816<BF16>(o[2 * c + 1], hi[ks], r[2], r[3]);
-            mma16816<BF16>(o[2 * c], lo[ks], r[0], r[1]);
-            mma16816<BF16>(o[2 * c + 1], lo[ks], r[2], r[3]);
+          } else {
+#pragma unroll
+            for (int c = 0; c < D / 16; ++c) {
+              uint32_t r[4];
+              ldsm4_t(vb + (c >> 2) * blk_stride + (at_v[mt] ^ ((c & 3) << 5)), r);
+              if (tail) {
+                r[0] &= keep[0];
+                r[1] &= keep[0];
+                r[2] &= keep[1];
+                r[3] &= keep[1];
+              }
+#pragma unroll
+              for (int nt = 0; nt < NT; ++nt) {
+                mma16816<BF16>(o[c][nt], r, hi[mt][nt][0], hi[mt][nt][1]);
+                mma16816<BF16>(o[c][nt], r, lo[mt][nt][0], lo[mt][nt][1]);
+              }
+            }
           }
         }
-      }
       }
       __syncwarp();
       if (lane == 0) mbar_arrive(empty(s));
@@ -411,127 +449,130 @@ attn_rows(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUten
 
     // ---- join the eight warps: rows in shared memory, columns swizzled by 8 floats with the row (no bank conflicts)
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      l[h] += __shfl_xor_sync(0xffffffffu, l[h], 1);
-      l[h] += __shfl_xor_sync(0xffffffffu, l[h], 2);
-      const int r = g + 8 * h;
-      float* dst = merge + (warp * BR + r) * D;
-      if (t4 == 0) ml[warp * BR + r] = make_float2(m[h], l[h]);
-      if constexpr (INT8) {
+    for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-        for (int c = 0; c < D / 16; ++c)
-          *reinterpret_cast<float4*>(dst + ((16 * c + 4 * t4) ^ ((r & 3) * 8))) =
-              make_float4(o[2 * c][2 * h], o[2 * c + 1][2 * h], o[2 * c][2 * h + 1], o[2 * c + 1][2 * h + 1]);
-      } else {
+      for (int e = 0; e < 2; ++e) {
+        float y = l[nt][e];
+        y += __shfl_xor_sync(0xffffffffu, y, 4);
+        y += __shfl_xor_sync(0xffffffffu, y, 8);
+        y += __shfl_xor_sync(0xffffffffu, y, 16);
+        const int r = nt * 8 + 2 * t4 + e;
+        if (g == 0) ml[warp * BR + r] = make_float2(m[nt][e], y);
+        float* dst = merge + (warp * BR + r) * D;
 #pragma unroll
-        for (int n = 0; n < D / 8; ++n)
-          *reinterpret_cast<float2*>(dst + ((8 * n + 2 * t4) ^ ((r & 3) * 8))) = make_float2(o[n][2 * h], o[n][2 * h + 1]);
-      }
-    }
-    consumers_meet();
-    {
-      constexpr int PER = D / 16;  // columns of a thread: 8 or 4
-      const int r = threadIdx.x >> 4, col = (threadIdx.x & 15) * PER, row = row0 + r;
-      if (row < R) {
-        float M = -CUDART_INF_F, L = 0.f, acc[PER];
-#pragma unroll
-        for (int i = 0; i < PER; ++i) acc[i] = 0.f;
-#pragma unroll
-        for (int v = 0; v < kConsumers; ++v) M = fmaxf(M, ml[v * BR + r].x);
-        const float ref = M == -CUDART_INF_F ? 0.f : M;
-#pragma unroll
-        for (int v = 0; v < kConsumers; ++v) {
-          const float2 y = ml[v * BR + r];
-          const float wt = ex2(y.x - ref);
-          L = fmaf(wt, y.y, L);
-          const float* src = merge + (v * BR + r) * D + (col ^ ((r & 3) * 8));
-#pragma unroll
-          for (int i = 0; i < PER; i += 4) {
-            const float4 f = *reinterpret_cast<const float4*>(src + i);
-            acc[i] = fmaf(wt, f.x, acc[i]);
-            acc[i + 1] = fmaf(wt, f.y, acc[i + 1]);
-            acc[i + 2] = fmaf(wt, f.z, acc[i + 2]);
-            acc[i + 3] = fmaf(wt, f.w, acc[i + 3]);
+        for (int c = 0; c < D / 16; ++c) {
+          if constexpr (INT8) {
+            *reinterpret_cast<float2*>(dst + ((16 * c + 2 * g) ^ (t4 * 8))) = make_float2(o[c][nt][e], o[c][nt][2 + e]);
+          } else {
+            dst[(16 * c + g) ^ (t4 * 8)] = o[c][nt][e];
+            dst[(16 * c + g + 8) ^ (t4 * 8)] = o[c][nt][2 + e];
           }
         }
-        if (cnt == w.nt) {
-          const float inv = M == -CUDART_INF_F ? 0.f : 1.f / L;
-          uint32_t out[PER / 2];
+      }
+    consumers_meet();
+    constexpr int PER = BR * D / 256;  // columns of a thread: 8, 4 or 2
+    const int r = threadIdx.x / (256 / BR), col = (threadIdx.x % (256 / BR)) * PER, row = row0 + r;
+    const bool there = row < R, whole = cnt == w.nt;
+    float M = -CUDART_INF_F, L = 0.f, acc[PER];
 #pragma unroll
-          for (int i = 0; i < PER / 2; ++i) out[i] = pack2<BF16>(acc[2 * i] * inv, acc[2 * i + 1] * inv);
-          uint16_t* dst = p.o + ((long long)(x.tok0 + row / group) * p.s.heads * group + w.h * group + row % group) * D + col;
-          if constexpr (PER == 8)
-            *reinterpret_cast<uint4*>(dst) = make_uint4(out[0], out[1], out[2], out[3]);
-          else
-            *reinterpret_cast<uint2*>(dst) = make_uint2(out[0], out[1]);
-        } else {
-          const long long slot = 2LL * blockIdx.x + (begin > w.cur - w.tile ? 0 : 1);
-          float* dst = p.part + (slot * BR + r) * D + col;
+    for (int i = 0; i < PER; ++i) acc[i] = 0.f;
 #pragma unroll
-          for (int i = 0; i < PER; i += 4)
-            *reinterpret_cast<float4*>(dst + i) = make_float4(acc[i], acc[i + 1], acc[i + 2], acc[i + 3]);
-          if (col == 0) p.ml[slot * BR + r] = make_float2(M, L);
+    for (int v = 0; v < kConsumers; ++v) M = fmaxf(M, ml[v * BR + r].x);
+    const float ref = M == -CUDART_INF_F ? 0.f : M;
+#pragma unroll
+    for (int v = 0; v < kConsumers; ++v) {
+      const float2 y = ml[v * BR + r];
+      const float wt = ex2(y.x - ref);
+      L = fmaf(wt, y.y, L);
+      const float* src = merge + (v * BR + r) * D + (col ^ (((r >> 1) & 3) * 8));
+#pragma unroll
+      for (int i = 0; i < PER; i += 2) {
+        const float2 f = *reinterpret_cast<const float2*>(src + i);
+        acc[i] = fmaf(wt, f.x, acc[i]);
+        acc[i + 1] = fmaf(wt, f.y, acc[i + 1]);
+      }
+    }
+    bool done = whole;
+    if (!whole) {
+      const long long w0 = w.cur - w.tile;
+      const int c0 = w.owner(w0), c1 = w.owner(w0 + w.nt - 1);
+      const long long slot = w.place(blockIdx.x, (int)blockIdx.x == c0);
+      if (there) {
+        float* dst = p.part + (slot * BR + r) * D + col;
+#pragma unroll
+        for (int i = 0; i < PER; i += 2) *reinterpret_cast<float2*>(dst + i) = make_float2(acc[i], acc[i + 1]);
+        if (col == 0) p.ml[slot * BR + r] = make_float2(M, L);
+      }
+      consumers_meet();
+      if (warp == 0) {
+        if (lane == 0 && ok) flag_set(p.flags + slot, p.call);
+        __syncwarp();
+        const bool all = flags_all(p.flags, 1, c0, c1, p.call);
+        if (all) flags_clear(p.flags, 1, c0, c1);
+        if (lane == 0) ml[0].x = all ? 1.f : 0.f;
+      }
+      consumers_meet();
+      done = ml[0].x != 0.f;
+      if (done) {
+        const int parts = c1 - c0 + 1;
+        consumers_meet();  // all have read ml[0]
+        float2* pml = reinterpret_cast<float2*>(merge);  // [part][BR]
+        for (int i = threadIdx.x; i < parts * BR; i += 256)
+          pml[i] = __ldcg(p.ml + (2LL * (c0 + i / BR) + (i < BR)) * BR + i % BR);
+        consumers_meet();
+        M = -CUDART_INF_F;
+        for (int c = 0; c < parts; ++c) M = fmaxf(M, pml[c * BR + r].x);
+        const float ref = M == -CUDART_INF_F ? 0.f : M;
+        L = 0.f;
+#pragma unroll
+        for (int i = 0; i < PER; ++i) acc[i] = 0.f;
+        if (there) {
+#pragma unroll 4
+          for (int c = 0; c < parts; ++c) {
+            const float2 y = pml[c * BR + r];
+            const float wt = ex2(y.x - ref);
+            L = fmaf(wt, y.y, L);
+            const float* src = p.part + ((2LL * (c0 + c) + (c == 0)) * BR + r) * D + col;
+#pragma unroll
+            for (int i = 0; i < PER; i += 2) {
+              const float2 f = __ldcg(reinterpret_cast<const float2*>(src + i));
+              acc[i] = fmaf(wt, f.x, acc[i]);
+              acc[i + 1] = fmaf(wt, f.y, acc[i + 1]);
+            }
+          }
         }
       }
+    }
+    if (done && there) {
+      const float inv = M == -CUDART_INF_F ? 0.f : 1.f / L;
+      uint32_t* dst = reinterpret_cast<uint32_t*>(
+          p.o + ((long long)(x.tok0 + row / group) * p.s.heads * group + w.h * group + row % group) * D + col);
+#pragma unroll
+      for (int i = 0; i < PER / 2; ++i) dst[i] = pack2<BF16>(acc[2 * i] * inv, acc[2 * i + 1] * inv);
     }
     consumers_meet();
     w.advance(p.s, p.blocks);
   }
-}
-
-// Joins the parts of the units that several CTAs of attn_rows shared: block (c, four rows) those of the unit that CTA c
-// continues, if c is the first to continue it; one thread to a column, the parts in the order of the CTAs. Block (0, 0)
-// also zeroes the rows of packed tokens that belong to no sequence.
-template <int D, bool BF16>
-__global__ void __launch_bounds__(D) merge_rows(const Params p, int grid) {
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-  asm volatile("griddepcontrol.wait;" ::: "memory");
-  const int group = p.blocks.group, c0 = blockIdx.x - 1;
-  if (c0 < 0) {
-    if (blockIdx.y == 0) {
-      const int first = min(max(p.s.cu_new[p.s.batch], 0), p.s.total);
-      const long long row = (long long)p.s.heads * group * D;
-      for (long long i = first * row + threadIdx.x; i < p.s.total * row; i += D) p.o[i] = 0;
-    }
-    return;
-  }
-  Walk<RowBlocks> w;
-  w.start(p.s, p.blocks, c0 + 1, grid);
-  const long long w0 = w.cur - w.tile;
-  if (w.cur >= w.end || w.tile == 0 || w.first(c0) > w0) return;
-  const int R = w.x.n * group;
-  for (int r = blockIdx.y * 4; r < blockIdx.y * 4 + 4 && w.blk * BR + r < R; ++r) {
-    auto slot = [&](int c) { return (2LL * c + (c > c0 ? 0 : 1)) * BR + r; };
-    float M = -CUDART_INF_F, L = 0.f, acc = 0.f;
-    int c1 = c0;
-    for (; c1 < w.ctas && w.first(c1) < w0 + w.nt; ++c1) M = fmaxf(M, p.ml[slot(c1)].x);
-    const float ref = M == -CUDART_INF_F ? 0.f : M;
-#pragma unroll 4
-    for (int c = c0; c < c1; ++c) {
-      const float2 y = p.ml[slot(c)];
-      const float wt = ex2(y.x - ref);
-      L = fmaf(wt, y.y, L);
-      acc = fmaf(wt, p.part[slot(c) * D + threadIdx.x], acc);
-    }
-    const int row = w.blk * BR + r;
-    const float out = M == -CUDART_INF_F ? 0.f : acc / L;
-    p.o[((long long)(w.x.tok0 + row / group) * p.s.heads * group + w.h * group + row % group) * D + threadIdx.x] =
-        (uint16_t)pack2<BF16>(out, 0.f);
+  if (blockIdx.x == 0) {
+    // zeroes the rows of packed tokens that belong to no sequence
+    const int first = min(max(p.s.cu_new[p.s.batch], 0), p.s.total);
+    const long long row = (long long)p.s.heads * group * D;
+    for (long long i = first * row + threadIdx.x; i < p.s.total * row; i += 256) p.o[i] = 0;
   }
 }
 
-std::atomic<bool> g_attr[2][2][2][64];
+std::atomic<bool> g_attr[2][2][2][2][64];
 
-template <int D, bool BF16, bool INT8>
+template <int D, bool BF16, bool INT8, int NT>
 cudaError_t launch(const PagedAttnArgs& a, int dev) {
-  using C = Cfg<D, INT8>;
-  int sms = 0;
-  cudaError_t e = sm_count(dev, &sms);
+  using C = Cfg<D, INT8, NT>;
+  int ctas = 0;
+  cudaError_t e = sm_count(dev, &ctas);
   if (e != cudaSuccess) return e;
-  std::atomic<bool>& attr = g_attr[D / 128][BF16][INT8][dev];
+  auto kern = attn_rows<D, BF16, INT8, NT>;
+  std::atomic<bool>& attr = g_attr[D / 128][BF16][INT8][NT - 1][dev];
   if (!attr.load(std::memory_order_acquire)) {
-    if ((e = cudaFuncSetAttribute(attn_rows<D, BF16, INT8>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM)) != cudaSuccess)
-      return e;
+    if ((e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM)) != cudaSuccess) return e;
     attr.store(true, std::memory_order_release);
   }
   CUtensorMap mk, mv;
@@ -539,13 +580,15 @@ cudaError_t launch(const PagedAttnArgs& a, int dev) {
   if (!make_paged_map(&mk, a.kc, a.s.num_pages, a.s.heads, page, D, a.kcs, elem, BF16, cols, box, C::BLOCKS, 1) ||
       !make_paged_map(&mv, a.vc, a.s.num_pages, a.s.heads, page, D, a.vcs, elem, BF16, cols, box, C::BLOCKS, 1))
     return cudaErrorInvalidValue;
-  const int ctas = sms;
-  const size_t ml_bytes = (size_t)ctas * 2 * BR * sizeof(float2);
+  const size_t places = (size_t)ctas * 2, part_bytes = places * C::BR * D * sizeof(float), ml_bytes = places * C::BR * sizeof(float2);
   void* block = nullptr;
-  if ((e = scratch_alloc(dev, ml_bytes + (size_t)ctas * 2 * BR * D * sizeof(float), a.stream, &block)) != cudaSuccess) return e;
-  Params p{a.s, static_cast<const uint16_t*>(a.q), a.q_token, a.q_head, static_cast<uint16_t*>(a.o), a.ks, a.vs, a.kss, a.vss,
-           RowBlocks{a.group, a.causal ? 1 : 0, a.s.heads}, a.scale * 1.4426950408889634f,
-           reinterpret_cast<float*>(static_cast<char*>(block) + ml_bytes), static_cast<float2*>(block)};
+  if ((e = scratch_alloc(dev, part_bytes + ml_bytes + places * 8, a.stream, &block)) != cudaSuccess) return e;
+  char* base = static_cast<char*>(block);
+  Params<NT> p{a.s, static_cast<const uint16_t*>(a.q), a.q_token, a.q_head, static_cast<uint16_t*>(a.o), a.ks, a.vs, a.kss, a.vss,
+               RowBlocks<NT>{a.group, a.causal ? 1 : 0, a.s.heads},
+               (INT8 ? a.scale : fabsf(a.scale)) * 1.4426950408889634f, !INT8 && a.scale < 0.f ? 0x80008000u : 0u,
+               reinterpret_cast<float*>(base), reinterpret_cast<float2*>(base + part_bytes),
+               reinterpret_cast<unsigned long long*>(base + part_bytes + ml_bytes), next_call()};
   cudaLaunchConfig_t cfg = {};
   cudaLaunchAttribute pdl[1];
   pdl[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -556,28 +599,26 @@ cudaError_t launch(const PagedAttnArgs& a, int dev) {
   cfg.gridDim = dim3((unsigned)ctas);
   cfg.blockDim = dim3(kThreads);
   cfg.dynamicSmemBytes = C::SMEM;
-  e = cudaLaunchKernelEx(&cfg, attn_rows<D, BF16, INT8>, mk, mv, p);
-  if (e == cudaSuccess) {
+  if ((e = cudaLaunchKernelEx(&cfg, kern, mk, mv, p)) == cudaSuccess) {
     note_launch();
-    cfg.gridDim = dim3((unsigned)ctas, BR / 4);
-    cfg.blockDim = dim3(D);
-    cfg.dynamicSmemBytes = 0;
-    if ((e = cudaLaunchKernelEx(&cfg, merge_rows<D, BF16>, p, ctas)) == cudaSuccess) note_launch();
+    e = cudaGetLastError();
   }
-  if (e == cudaSuccess) e = cudaGetLastError();
   const cudaError_t ef = cudaFreeAsync(block, a.stream);
   return e != cudaSuccess ? e : ef;
 }
 
+template <int D, int NT>
+cudaError_t launch_d(const PagedAttnArgs& a, int dev) {
+  return a.int8 ? (a.bf16 ? launch<D, true, true, NT>(a, dev) : launch<D, false, true, NT>(a, dev))
+                : (a.bf16 ? launch<D, true, false, NT>(a, dev) : launch<D, false, false, NT>(a, dev));
+}
+
 }  // namespace rows
 
-cudaError_t launch_paged_attn_rows(const PagedAttnArgs& a, int dev) {
+cudaError_t launch_paged_attn_rows(const PagedAttnArgs& a, int dev, int rows) {
   using namespace rows;
-  if (a.d == 64)
-    return a.int8 ? (a.bf16 ? launch<64, true, true>(a, dev) : launch<64, false, true>(a, dev))
-                  : (a.bf16 ? launch<64, true, false>(a, dev) : launch<64, false, false>(a, dev));
-  return a.int8 ? (a.bf16 ? launch<128, true, true>(a, dev) : launch<128, false, true>(a, dev))
-                : (a.bf16 ? launch<128, true, false>(a, dev) : launch<128, false, false>(a, dev));
+  if (rows <= 8) return a.d == 64 ? launch_d<64, 1>(a, dev) : launch_d<128, 1>(a, dev);
+  return a.d == 64 ? launch_d<64, 2>(a, dev) : launch_d<128, 2>(a, dev);
 }
 
 }  // namespace phantom

@@ -1384,6 +1384,8 @@ cudaError_t sm_count(int dev, int* n) {
   return e;
 }
 
+unsigned long long next_call() { return next_generation(); }
+
 cudaError_t scratch_alloc(int dev, size_t bytes, cudaStream_t stream, void** out) {
   cudaMemPool_t pool;
   const cudaError_t e = device_pool(dev, &pool);

@@ -54,7 +54,8 @@ struct PagedAttnArgs {
 };
 
 // Few query rows for each key head (decoding): attn_paged.cu. Right for any number of them.
-cudaError_t launch_paged_attn_rows(const PagedAttnArgs& a, int dev);
+// `rows`: how many to expect.
+cudaError_t launch_paged_attn_rows(const PagedAttnArgs& a, int dev, int rows);
 // Many query rows (chunks of prompts): attn_paged_tc_sm100.cu.
 cudaError_t launch_paged_attn_chunk(const PagedAttnArgs& a, int dev);
 
@@ -62,6 +63,8 @@ cudaError_t launch_paged_attn_chunk(const PagedAttnArgs& a, int dev);
 cudaError_t sm_count(int dev, int* n);
 // Stream-ordered scratch from the library's pool of device `dev`, released with cudaFreeAsync on the same stream.
 cudaError_t scratch_alloc(int dev, size_t bytes, cudaStream_t stream, void** out);
+// A number unique to a call in this process, never 0.
+unsigned long long next_call();
 // TMA map of a (page, head, token, d) cache as (columns of a swizzled row, token, block of such columns, head, page): boxes
 // of `cols` elements of `elem` bytes (64 or 128 bytes, the swizzle's width) by `rows` tokens by `blocks` column blocks of
 // one head and `pages` pages.

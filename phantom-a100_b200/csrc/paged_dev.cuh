@@ -65,8 +65,8 @@ __device__ __forceinline__ long long sum_tiles(const Blocks& k, const Seq& x) {
 // A whole warp walks one CTA's share; every value is uniform over the warp.
 template <typename Blocks>
 struct Walk {
-  long long total, cur, end;
-  int ctas;  // that share the work: no more than there are tiles, so that each has one
+  long long share, cur, end;
+  int more, ctas;           // CTA c has share + (c < more) tiles; CTAs that have any
   Seq x;
   int b, h, blk, tile, nt;  // the unit, its tile at `cur`, its tiles
 
@@ -77,14 +77,19 @@ struct Walk {
     }
     return w;
   }
+  __device__ static long long quotient(long long a, long long b) {  // 64-bit division is a long call
+    return a <= 0x7fffffffLL && b <= 0x7fffffffLL ? (long long)((unsigned)a / (unsigned)b) : a / b;
+  }
   __device__ void start(const PagedSeqs& s, const Blocks& k, int cta, int grid) {
     const int lane = threadIdx.x & 31;
     auto seq_tiles = [&](int i) { return i < s.batch ? k.head_tiles(seq_of(s, i)) * s.heads : 0LL; };
     // (up to 32 sequences: one scan gives the total and the place)
     long long w = scan(seq_tiles(lane), lane);
-    total = __shfl_sync(0xffffffffu, w, 31);
+    long long total = __shfl_sync(0xffffffffu, w, 31);
     for (int i0 = 32; i0 < s.batch; i0 += 32) total += __shfl_sync(0xffffffffu, scan(seq_tiles(i0 + lane), lane), 31);
-    ctas = (int)min((long long)grid, total);
+    ctas = (int)min((long long)grid, total);  // each has a tile then
+    share = ctas > 0 ? quotient(total, ctas) : 0;
+    more = (int)(total - share * ctas);
     cur = cta < ctas ? first(cta) : 0;
     end = cta < ctas ? first(cta + 1) : 0;
     if (cur >= end) return;
@@ -104,11 +109,13 @@ struct Walk {
     x = seq_of(s, b);
     const long long head = k.head_tiles(x);
     long long r = cur - before;
-    h = (int)(r / head);
+    h = (int)quotient(r, head);
     r -= h * head;
+    blk = 0;
     const int count = k.count(x);
-    for (int i0 = 0;; i0 += 32) {
-      w = scan(i0 + lane < count ? tiles_of(k, x, i0 + lane) : 0, lane);
+    for (int i0 = 0; count > 1; i0 += 32) {
+      const int y = i0 + lane < count ? tiles_of(k, x, i0 + lane) : 0;
+      w = scan(y, lane);
       const unsigned past = __ballot_sync(0xffffffffu, w > r);
       if (past) {
         const int at = __ffs(past) - 1;
@@ -123,9 +130,16 @@ struct Walk {
     tile = (int)r;
   }
   // The first tile of a CTA's share.
-  __device__ long long first(int cta) const { return total * cta / ctas; }
+  __device__ long long first(int cta) const { return cta * share + min(cta, more); }
+  // The CTA that has a tile.
+  __device__ int owner(long long at) const {
+    const long long big = more * (share + 1);
+    return (int)(at < big ? quotient(at, share + 1) : more + quotient(at - big, share));
+  }
   // The tiles of the unit that this CTA has.
   __device__ int count() const { return (int)min((long long)(nt - tile), end - cur); }
+  // A unit that several CTAs share: CTA c's part of it lies in the place 2 c + 1 if the unit begins in c's share, else 2 c.
+  __device__ static int place(int cta, bool begins) { return 2 * cta + (begins ? 1 : 0); }
   __device__ void advance(const PagedSeqs& s, const Blocks& k) {
     cur += count();
     if (cur >= end) return;
@@ -141,6 +155,33 @@ struct Walk {
     nt = tiles_of(k, x, blk);
   }
 };
+
+// The parts of a shared unit are joined by the CTA that finds all of them written. Each part has a 64-bit flag that holds
+// the call's number (unique in the process) once the part is in memory. A CTA writes its part, then its flag, then reads
+// all the unit's flags: in the order that fence.sc gives the flags' writes, the CTA of the last one finds them all. (Two
+// may; they write the same result.) It then clears them, so that a call replayed from a graph, whose number is the same
+// each time, finds none set. Flags need no initialisation: what a pool's memory held before does not equal the number.
+__device__ __forceinline__ void flag_set(unsigned long long* flag, unsigned long long call) {
+  asm volatile("fence.sc.gpu;" ::: "memory");
+  asm volatile("st.relaxed.gpu.global.u64 [%0], %1;" ::"l"(flag), "l"(call) : "memory");
+  asm volatile("fence.sc.gpu;" ::: "memory");
+}
+__device__ __forceinline__ unsigned long long flag_get(const unsigned long long* flag) {
+  unsigned long long y;
+  asm volatile("ld.relaxed.gpu.global.u64 %0, [%1];" : "=l"(y) : "l"(flag) : "memory");
+  return y;
+}
+// Whole warp: are the flags of the unit whose parts the CTAs c0 ... c1 have all set? `per` flags to a place.
+__device__ __forceinline__ bool flags_all(const unsigned long long* flags, int per, int c0, int c1, unsigned long long call) {
+  bool all = true;
+  for (int c = c0 + (int)(threadIdx.x & 31); c <= c1; c += 32) all &= flag_get(flags + (2LL * c + (c == c0)) * per) == call;
+  all = __all_sync(0xffffffffu, all);
+  asm volatile("fence.sc.gpu;" ::: "memory");
+  return all;
+}
+__device__ __forceinline__ void flags_clear(unsigned long long* flags, int per, int c0, int c1) {
+  for (int c = c0 + (int)(threadIdx.x & 31); c <= c1; c += 32) flags[(2LL * c + (c == c0)) * per] = 0;
+}
 
 // ------------------------------------------------------------------------------------------------ copies, 8-bit values
 // Untiled bulk copy into shared memory (16-byte aligned, a multiple of 16 bytes).
