@@ -19,7 +19,9 @@
 //   * Two producer warps read the page table and keep a ring of tiles in flight by TMA (a box per page, swizzled, so that
 //     pages of 16 tokens land as one conflict-free tile); 128 KB in flight for each SM.
 //   * Eight consumer warps work without meeting: two to a tile, 32 keys each, every warp with its own running maximum,
-//     sum and output; they are joined through shared memory at the end of a unit.
+//     sum and output. At the end of a unit they leave these in shared memory and go on to the next, whose queries a
+//     producer has brought there; four further warps join and write them. (With the consumers doing this themselves a
+//     unit cost them 3.9 us besides its tiles.)
 //
 // Precision: scores and sums are fp32. 16-bit caches: P enters the second product as hi + lo (two 16-bit numbers), so its
 // rounding (which alone would be as large as the output's) is gone; the tensor cores idle here and the second product is
@@ -42,8 +44,13 @@ namespace rows {
 // A unit has 8 NT query rows (NT = 1, 2).
 constexpr int BN = 64;        // keys of a tile
 constexpr int kConsumers = 8; // warps; pairs of them take the tiles in turn
-constexpr int kThreads = 32 * (kConsumers + 2);  // and two producers, of keys and of values
-constexpr int kErrCopyWait = 1, kErrTileWait = 4;
+constexpr int kJoiners = 4;
+constexpr int K_WARP = kConsumers + kJoiners, V_WARP = K_WARP + 1;  // producers; two idle warps complete their warpgroup
+constexpr int kThreads = 32 * 16;
+// Registers: 512 threads launch with 128 each; 2 * 168 + 104 + 72 = 4 * 128 (setmaxnreg, by warpgroup).
+constexpr int kRegsConsumer = 168, kRegsJoiner = 104, kRegsProducer = 72;
+constexpr int kUnitRing = 4;
+constexpr int kErrCopyWait = 1, kErrTileWait = 4, kErrJoinWait = 8;
 
 template <int D, bool INT8, int NT>
 struct Cfg {
@@ -58,9 +65,12 @@ struct Cfg {
   static_assert(SLOTS % 4 == 0, "each ring slot belongs to one pair of warps");
   static constexpr int OFF_MERGE = SLOTS * SLOT;          // [kConsumers][BR][D] fp32
   static constexpr int OFF_ML = OFF_MERGE + kConsumers * BR * D * 4;
-  static constexpr int OFF_SCALE = OFF_ML + kConsumers * BR * 8;
-  static constexpr int OFF_BAR = OFF_SCALE + (INT8 ? SLOTS * 2 * BN * 4 : 0);
-  static constexpr int OFF_FLAG = OFF_BAR + 2 * SLOTS * 8;
+  static constexpr int Q_ROW = 2 * D + 16;                // padded: lanes of 8 rows and 4 words read without conflicts
+  static constexpr int OFF_Q = OFF_ML + kConsumers * BR * 8;
+  static constexpr int OFF_SCALE = OFF_Q + kUnitRing * BR * Q_ROW;
+  static constexpr int OFF_UNIT = OFF_SCALE + (INT8 ? SLOTS * 2 * BN * 4 : 0);
+  static constexpr int OFF_BAR = OFF_UNIT + kUnitRing * 48;
+  static constexpr int OFF_FLAG = OFF_BAR + (2 * SLOTS + 2 * kUnitRing + 2) * 8;
   static constexpr int SMEM = OFF_FLAG + 16 + 1024;       // + slack to align the base
   static_assert(SMEM <= 227 * 1024, "shared memory plan exceeds 227 KB");
 };
@@ -119,13 +129,26 @@ __device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], 
                  : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
-__device__ __forceinline__ void consumers_meet() { asm volatile("bar.sync 1, 256;" ::: "memory"); }
+__device__ __forceinline__ void joiners_meet() { asm volatile("bar.sync 1, 128;" ::: "memory"); }
+__device__ __forceinline__ bool joiners_all(bool x) {
+  uint32_t y;
+  asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %1, 0;\n\tbar.red.and.pred q, 1, 128, p;\n\tselp.u32 %0, 1, 0, q;\n\t}"
+               : "=r"(y) : "r"((uint32_t)x) : "memory");
+  return y != 0;
+}
 // Transposes the 8 x 8 matrix of 16-bit numbers that a warp holds (lane 4 r + c: row r, columns 2 c and 2 c + 1).
 __device__ __forceinline__ uint32_t turn(uint32_t x) {
   uint32_t y;
   asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
   return y;
 }
+
+// What the key producer tells the others of a unit (48 bytes).
+struct Unit {
+  int cnt, tile0, end, id;    // its tiles here, the first of them; the keys that its rows see; id -1 ends the roles
+  int len, n, row0, tok0;     // the sequence: cached and new tokens; the unit's first row; packed place of its first token
+  int h, c0, c1, pad;         // key head; the first and the last CTA that have tiles of it
+};
 
 template <int D, bool BF16, bool INT8, int NT>
 __global__ void __launch_bounds__(kThreads, 1)
@@ -134,17 +157,30 @@ attn_rows(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUten
   constexpr int BR = C::BR;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  const uint32_t sbase = smem_u32(smem);
-  auto full = [&](int s) { return sbase + C::OFF_BAR + 8u * s; };
-  auto empty = [&](int s) { return sbase + C::OFF_BAR + 8u * (C::SLOTS + s); };
+  const uint32_t sbase = smem_u32(smem), bars = sbase + C::OFF_BAR;
+  auto full = [&](int s) { return bars + 8u * s; };
+  auto empty = [&](int s) { return bars + 8u * (C::SLOTS + s); };
+  auto q_full = [&](int u) { return bars + 8u * (2 * C::SLOTS + u % kUnitRing); };
+  auto q_empty = [&](int u) { return bars + 8u * (2 * C::SLOTS + kUnitRing + u % kUnitRing); };
+  const uint32_t join_full = bars + 8u * (2 * C::SLOTS + 2 * kUnitRing), join_empty = join_full + 8;
   volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + C::OFF_FLAG);
+  volatile int* joined = reinterpret_cast<volatile int*>(smem + C::OFF_FLAG + 4);
+  int4* ring = reinterpret_cast<int4*>(smem + C::OFF_UNIT);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int group = p.blocks.group, causal = p.blocks.causal;
+  int* status = p.s.status;
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < C::SLOTS; ++s) {
       mbar_init(full(s), 2);   // the producers
       mbar_init(empty(s), 2);  // the consuming pair
     }
+    for (int u = 0; u < kUnitRing; ++u) {
+      mbar_init(q_full(u), 1);
+      mbar_init(q_empty(u), kConsumers + kJoiners);
+    }
+    mbar_init(join_full, kConsumers);
+    mbar_init(join_empty, kJoiners);
     *abort_flag = 0;
     fence_mbar_init();
   }
@@ -152,31 +188,70 @@ attn_rows(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUten
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   asm volatile("griddepcontrol.wait;" ::: "memory");
 
-  Walk<RowBlocks<NT>> w;
-  w.start(p.s, p.blocks, blockIdx.x, gridDim.x);
-  const int group = p.blocks.group, causal = p.blocks.causal;
-  const long long begin = w.cur;
-  if (warp >= kConsumers) {
-    // Producers, one of the keys and one of the values: a tile's boxes, one to a page, and an 8-bit cache's scales. One
-    // elected lane of warp-uniform code issues the copies; the issue is what limits pages of 16 tokens, hence two warps.
-    const bool vals = warp > kConsumers;
+  auto wait = [&](uint32_t bar, int parity, int code) {
+    return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag, status, code)) != 0;
+  };
+  // A consuming role's next unit (id -1 at the end, or when a wait gave up).
+  auto next_unit = [&](int u) {
+    Unit x;
+    x.id = -1;
+    if (wait(q_full(u), (u / kUnitRing) & 1, kErrTileWait)) {
+      const int4* r = ring + 3 * (u % kUnitRing);
+      const int4 a = r[0], b = r[1], c = r[2];
+      x.cnt = a.x, x.tile0 = a.y, x.end = a.z, x.id = a.w;
+      x.len = b.x, x.n = b.y, x.row0 = b.z, x.tok0 = b.w;
+      x.h = c.x, x.c0 = c.y, x.c1 = c.z;
+    }
+    return x;
+  };
+
+  if (warp >= K_WARP) {
+    setmaxnreg_dec<kRegsProducer>();
+    if (warp > V_WARP) return;
+    // Producers, one of the keys (and of the units' records and queries) and one of the values: a tile's boxes, one to a
+    // page, and an 8-bit cache's scales. Each walks the CTA's share by itself. One elected lane of warp-uniform code issues
+    // the copies; the issue is what limits pages of 16 tokens, hence two warps.
+    const bool vals = warp == V_WARP;
     const CUtensorMap* map = vals ? &tmV : &tmK;
-    if (lane == 0) tma_prefetch_desc(map);
-    int t = 0;
+    if (elect_one()) tma_prefetch_desc(map);
+    __syncwarp();
+    Walk<RowBlocks<NT>> w;
+    w.start(p.s, p.blocks, blockIdx.x, gridDim.x);
+    int t = 0, nu = 0;
     bool ok = true;
     const int page = 1 << p.s.page_log2, box = min(page, BN);
     const Strides3 st = vals ? p.vss : p.kss;
     const float* scale = vals ? p.vs : p.ks;
-    while (ok && w.cur < w.end) {
+    while (w.cur < w.end) {
       const int end = p.blocks.key_end(w.x, w.blk), cnt = w.count();
+      if (!vals) {
+        if (nu >= kUnitRing && !(ok = wait(q_empty(nu), (nu / kUnitRing - 1) & 1, kErrCopyWait))) break;
+        const int row0 = w.blk * BR, rows = min(BR, w.x.n * group - row0);
+        const long long w0 = w.cur - w.tile;
+        const int c0 = w.owner(w0), c1 = w.owner(w0 + w.nt - 1);
+        if (elect_one()) {
+          int4* r = ring + 3 * (nu % kUnitRing);
+          r[0] = make_int4(cnt, w.tile, end, nu);
+          r[1] = make_int4(w.x.len, w.x.n, row0, w.x.tok0);
+          r[2] = make_int4(w.h, c0, c1, 0);
+          mbar_arrive_expect_tx(q_full(nu), rows * D * 2);
+        }
+        __syncwarp();
+        if (lane < rows) {
+          const int tok = (row0 + lane) / group;
+          bulk_load(sbase + C::OFF_Q + ((nu % kUnitRing) * BR + lane) * C::Q_ROW,
+                    p.q + (w.x.tok0 + tok) * p.q_token + (w.h * group + (row0 + lane - tok * group)) * p.q_head, D * 2, q_full(nu));
+        }
+        __syncwarp();
+        ++nu;
+      }
       for (int i = 0; i < cnt; ++i, ++t) {
         const int s = t % C::SLOTS, round = t / C::SLOTS;
         const int j0 = (w.tile + i) * BN;
         const int boxes = max(0, (min(j0 + BN, end) - j0 + box - 1) / box);  // pages of the tile that hold keys
         int id = 0;
         if (lane < boxes) id = page_of(p.s, w.b, (j0 >> p.s.page_log2) + lane);
-        if (round > 0 && !(ok = __all_sync(0xffffffffu, mbar_wait(empty(s), (round - 1) & 1, abort_flag, p.s.status, kErrCopyWait))))
-          break;
+        if (round > 0 && !(ok = wait(empty(s), (round - 1) & 1, kErrCopyWait))) break;
         const int place = j0 & (page - 1);
         const uint32_t dst = sbase + s * C::SLOT + (vals ? C::HALF : 0);
         if (elect_one()) mbar_arrive_expect_tx(full(s), boxes * box * (D * (INT8 ? 1 : 2) + (INT8 ? 4 : 0)));
@@ -192,17 +267,144 @@ attn_rows(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUten
         }
         __syncwarp();
       }
+      if (!ok) break;
       w.advance(p.s, p.blocks);
     }
+    if (!vals) {
+      if (ok && nu >= kUnitRing) ok = wait(q_empty(nu), (nu / kUnitRing - 1) & 1, kErrCopyWait);
+      if (ok) {
+        if (elect_one()) {
+          ring[3 * (nu % kUnitRing)] = make_int4(0, 0, 0, -1);
+          mbar_arrive(q_full(nu));
+        }
+        __syncwarp();
+        ++nu;
+      }
+      for (int u = max(0, nu - kUnitRing); u < nu; ++u) mbar_wait_drain(q_full(u), (u / kUnitRing) & 1);
+    }
+    if (!ok) *abort_flag = 1;
     // every issued copy lands before this CTA's shared memory is released
     for (int i = max(0, t - C::SLOTS); i < t; ++i) mbar_wait_drain(full(i % C::SLOTS), (i / C::SLOTS) & 1);
     return;
   }
 
-  const int g = lane >> 2, t4 = lane & 3;
-  const int pair = warp >> 1, kr = (warp & 1) * 32;  // this warp's keys of its pair's tiles
   float* merge = reinterpret_cast<float*>(smem + C::OFF_MERGE);
   float2* ml = reinterpret_cast<float2*>(smem + C::OFF_ML);
+  if (warp >= kConsumers) {
+    setmaxnreg_dec<kRegsJoiner>();
+    // Joiners: a unit's rows from the eight warps' sums, to the output or to the parts of a shared unit.
+    constexpr int PER = BR * D / 128;  // columns of a thread: 16, 8 or 4
+    const int tid = threadIdx.x - 32 * kConsumers;
+    const int r = tid / (128 / BR), col = (tid % (128 / BR)) * PER;
+    for (int u = 0;; ++u) {
+      const Unit x = next_unit(u);
+      __syncwarp();
+      if (x.id >= 0 && lane == 0) mbar_arrive(q_empty(u));
+      // all four warps go on, or none (a wait that gave up ends the roles; no warp may be left at a barrier)
+      if (!joiners_all(x.id >= 0 && wait(join_full, u & 1, kErrJoinWait))) break;
+      const int row = x.row0 + r;
+      const bool there = row < x.n * group;
+      float M = -CUDART_INF_F, L = 0.f, acc[PER];
+#pragma unroll
+      for (int i = 0; i < PER; ++i) acc[i] = 0.f;
+#pragma unroll
+      for (int v = 0; v < kConsumers; ++v) M = fmaxf(M, ml[v * BR + r].x);
+      {
+        const float ref = M == -CUDART_INF_F ? 0.f : M;
+#pragma unroll 2
+        for (int v = 0; v < kConsumers; ++v) {
+          const float2 y = ml[v * BR + r];
+          if (y.x == -CUDART_INF_F && y.y == 0.f) continue;  // no key seen, and maybe nothing written
+          const float wt = ex2(y.x - ref);
+          L = fmaf(wt, y.y, L);
+          const float* src = merge + (v * BR + r) * D;
+#pragma unroll
+          for (int i = 0; i < PER; i += 4) {
+            const float4 f = *reinterpret_cast<const float4*>(src + ((col + i) ^ (((r >> 1) & 3) * 8)));
+            acc[i] = fmaf(wt, f.x, acc[i]);
+            acc[i + 1] = fmaf(wt, f.y, acc[i + 1]);
+            acc[i + 2] = fmaf(wt, f.z, acc[i + 2]);
+            acc[i + 3] = fmaf(wt, f.w, acc[i + 3]);
+          }
+        }
+      }
+      bool done = x.c0 == x.c1;
+      if (done) {
+        __syncwarp();
+        if (lane == 0) mbar_arrive(join_empty);
+      } else {
+        const long long slot = Walk<RowBlocks<NT>>::place(blockIdx.x, (int)blockIdx.x == x.c0);
+        if (there) {
+          float* dst = p.part + (slot * BR + r) * D + col;
+#pragma unroll
+          for (int i = 0; i < PER; i += 4)
+            *reinterpret_cast<float4*>(dst + i) = make_float4(acc[i], acc[i + 1], acc[i + 2], acc[i + 3]);
+          if (col == 0) p.ml[slot * BR + r] = make_float2(M, L);
+        }
+        joiners_meet();
+        if (warp == kConsumers) {
+          if (lane == 0) flag_set(p.flags + slot, p.call);
+          __syncwarp();
+          const bool all = flags_all(p.flags, 1, x.c0, x.c1, p.call);
+          if (all) flags_clear(p.flags, 1, x.c0, x.c1);
+          if (lane == 0) *joined = all;
+        }
+        joiners_meet();
+        done = *joined != 0;
+        if (done) {
+          const int parts = x.c1 - x.c0 + 1;
+          float2* pml = reinterpret_cast<float2*>(merge);  // [part][BR]
+          for (int i = tid; i < parts * BR; i += 128) pml[i] = __ldcg(p.ml + (2LL * (x.c0 + i / BR) + (i < BR)) * BR + i % BR);
+          joiners_meet();
+          M = -CUDART_INF_F;
+          for (int c = 0; c < parts; ++c) M = fmaxf(M, pml[c * BR + r].x);
+          const float ref = M == -CUDART_INF_F ? 0.f : M;
+          L = 0.f;
+#pragma unroll
+          for (int i = 0; i < PER; ++i) acc[i] = 0.f;
+          if (there) {
+#pragma unroll 4
+            for (int c = 0; c < parts; ++c) {
+              const float2 y = pml[c * BR + r];
+              const float wt = ex2(y.x - ref);
+              L = fmaf(wt, y.y, L);
+              const float* src = p.part + ((2LL * (x.c0 + c) + (c == 0)) * BR + r) * D + col;
+#pragma unroll
+              for (int i = 0; i < PER; i += 4) {
+                const float4 f = __ldcg(reinterpret_cast<const float4*>(src + i));
+                acc[i] = fmaf(wt, f.x, acc[i]);
+                acc[i + 1] = fmaf(wt, f.y, acc[i + 1]);
+                acc[i + 2] = fmaf(wt, f.z, acc[i + 2]);
+                acc[i + 3] = fmaf(wt, f.w, acc[i + 3]);
+              }
+            }
+          }
+          joiners_meet();
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(join_empty);
+      }
+      if (done && there) {
+        const float inv = M == -CUDART_INF_F ? 0.f : 1.f / L;
+        uint2* dst = reinterpret_cast<uint2*>(
+            p.o + ((long long)(x.tok0 + row / group) * p.s.heads * group + x.h * group + row % group) * D + col);
+#pragma unroll
+        for (int i = 0; i < PER / 4; ++i)
+          dst[i] = make_uint2(pack2<BF16>(acc[4 * i] * inv, acc[4 * i + 1] * inv), pack2<BF16>(acc[4 * i + 2] * inv, acc[4 * i + 3] * inv));
+      }
+    }
+    if (blockIdx.x == 0) {
+      // zeroes the rows of packed tokens that belong to no sequence
+      const int first = min(max(p.s.cu_new[p.s.batch], 0), p.s.total);
+      const long long row = (long long)p.s.heads * group * D;
+      for (long long i = first * row + tid; i < p.s.total * row; i += 128) p.o[i] = 0;
+    }
+    return;
+  }
+
+  setmaxnreg_inc<kRegsConsumer>();
+  const int g = lane >> 2, t4 = lane & 3;
+  const int pair = warp >> 1, kr = (warp & 1) * 32;  // this warp's keys of its pair's tiles
   // Where this lane's rows for ldmatrix lie in a tile: 16 keys from kr + 16 mt, matrices (keys 0-7, 8-15) x (first, second
   // 16-byte chunk of a pair); V^T of 16-bit values has the two the other way around. Boxes of min(page, 64) tokens, each
   // [64-column block][token][ROW bytes]; a chunk lies at its number ^ the row's swizzle, so stepping over pairs of chunks
@@ -221,29 +423,27 @@ attn_rows(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUten
     at_v[mt] = INT8 ? at_k[mt] : place_of(key + (lane >> 4) * 8, (lane >> 3) & 1);
   }
   int t = 0;
-  bool ok = true;
-  while (w.cur < w.end) {
-    const Seq x = w.x;
-    const int cnt = w.count(), R = x.n * group, row0 = w.blk * BR, off = x.len - x.n;
-    const int end = p.blocks.key_end(x, w.blk);
+  for (int u = 0;; ++u) {
+    const Unit x = next_unit(u);
+    if (x.id < 0) break;
+    const int R = x.n * group, row0 = x.row0, off = x.len - x.n, end = x.end;
     // the queries as B operands: of row 8 nt + g; 8-bit caches: columns in the order that their bytes come in (4 t4 ... + 3
-    // of 16). Keys that the rows 8 nt + 2 t4 + e of this lane's scores see.
+    // of 16). Keys that the rows 8 nt + 2 t4 + e of this lane's scores see. (Rows past the last hold anything; no row's
+    // numbers meet another's.)
     uint32_t qb[NT][D / 16][2];
     int lim[NT][2];
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
-      const int r = row0 + nt * 8 + g;
-      const uint16_t* src = p.q + (x.tok0 + (r < R ? r / group : 0)) * p.q_token +
-                            (w.h * group + (r < R ? r % group : 0)) * p.q_head;
+      const uint8_t* src = smem + C::OFF_Q + ((u % kUnitRing) * BR + nt * 8 + g) * C::Q_ROW;
 #pragma unroll
       for (int k = 0; k < D / 16; ++k) {
         if constexpr (INT8) {
-          const uint2 y = *reinterpret_cast<const uint2*>(src + k * 16 + 4 * t4);
-          qb[nt][k][0] = r < R ? y.x : 0u;
-          qb[nt][k][1] = r < R ? y.y : 0u;
+          const uint2 y = *reinterpret_cast<const uint2*>(src + k * 32 + 8 * t4);
+          qb[nt][k][0] = y.x;
+          qb[nt][k][1] = y.y;
         } else {
-          qb[nt][k][0] = r < R ? *reinterpret_cast<const uint32_t*>(src + k * 16 + 2 * t4) ^ p.flip : 0u;
-          qb[nt][k][1] = r < R ? *reinterpret_cast<const uint32_t*>(src + k * 16 + 8 + 2 * t4) ^ p.flip : 0u;
+          qb[nt][k][0] = *reinterpret_cast<const uint32_t*>(src + k * 32 + 4 * t4) ^ p.flip;
+          qb[nt][k][1] = *reinterpret_cast<const uint32_t*>(src + k * 32 + 16 + 4 * t4) ^ p.flip;
         }
       }
 #pragma unroll
@@ -252,6 +452,8 @@ attn_rows(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUten
         lim[nt][e] = row >= R ? 0 : causal ? min(x.len, off + row / group + 1) : x.len;
       }
     }
+    __syncwarp();
+    if (lane == 0) mbar_arrive(q_empty(u));
     const int lim_least = causal ? max(0, min(x.len, off + row0 / group + 1)) : x.len;  // of the block's rows
     float m[NT][2], l[NT][2], o[D / 16][NT][4];
 #pragma unroll
@@ -262,13 +464,12 @@ attn_rows(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUten
       for (int c = 0; c < D / 16; ++c) o[c][nt][0] = o[c][nt][1] = o[c][nt][2] = o[c][nt][3] = 0.f;
     }
 
-    for (int i = 0; i < cnt; ++i, ++t) {
-      if ((t & 3) != pair) continue;
-      const int s = t % C::SLOTS;
-      if (ok) ok = __all_sync(0xffffffffu, mbar_wait(full(s), (t / C::SLOTS) & 1, abort_flag, p.s.status, kErrTileWait));
-      if (!ok) continue;
+    bool ok = true;
+    for (int i = (pair - t) & 3; i < x.cnt; i += 4) {  // every fourth tile
+      const int s = (t + i) % C::SLOTS;
+      if (!(ok = wait(full(s), ((t + i) / C::SLOTS) & 1, kErrTileWait))) break;
       const uint32_t kb = sbase + s * C::SLOT, vb = kb + C::HALF;
-      const int j0 = (w.tile + i) * BN + kr;  // this warp's first key
+      const int j0 = (x.tile0 + i) * BN + kr;  // this warp's first key
       if (j0 < end) {
         // ---- scores: [16 keys][8 rows]: (key g: rows 2 t4, + 1; key g + 8: the same)
         float sc[2][NT][4];
@@ -447,7 +648,11 @@ attn_rows(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUten
       if (lane == 0) mbar_arrive(empty(s));
     }
 
-    // ---- join the eight warps: rows in shared memory, columns swizzled by 8 floats with the row (no bank conflicts)
+    t += x.cnt;
+    if (!ok) break;
+
+    // ---- for the joiners: rows in shared memory, columns swizzled by 8 floats with the row (no bank conflicts)
+    if (u > 0 && !wait(join_empty, (u - 1) & 1, kErrJoinWait)) break;
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -469,95 +674,8 @@ attn_rows(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUten
           }
         }
       }
-    consumers_meet();
-    constexpr int PER = BR * D / 256;  // columns of a thread: 8, 4 or 2
-    const int r = threadIdx.x / (256 / BR), col = (threadIdx.x % (256 / BR)) * PER, row = row0 + r;
-    const bool there = row < R, whole = cnt == w.nt;
-    float M = -CUDART_INF_F, L = 0.f, acc[PER];
-#pragma unroll
-    for (int i = 0; i < PER; ++i) acc[i] = 0.f;
-#pragma unroll
-    for (int v = 0; v < kConsumers; ++v) M = fmaxf(M, ml[v * BR + r].x);
-    const float ref = M == -CUDART_INF_F ? 0.f : M;
-#pragma unroll
-    for (int v = 0; v < kConsumers; ++v) {
-      const float2 y = ml[v * BR + r];
-      const float wt = ex2(y.x - ref);
-      L = fmaf(wt, y.y, L);
-      const float* src = merge + (v * BR + r) * D + (col ^ (((r >> 1) & 3) * 8));
-#pragma unroll
-      for (int i = 0; i < PER; i += 2) {
-        const float2 f = *reinterpret_cast<const float2*>(src + i);
-        acc[i] = fmaf(wt, f.x, acc[i]);
-        acc[i + 1] = fmaf(wt, f.y, acc[i + 1]);
-      }
-    }
-    bool done = whole;
-    if (!whole) {
-      const long long w0 = w.cur - w.tile;
-      const int c0 = w.owner(w0), c1 = w.owner(w0 + w.nt - 1);
-      const long long slot = w.place(blockIdx.x, (int)blockIdx.x == c0);
-      if (there) {
-        float* dst = p.part + (slot * BR + r) * D + col;
-#pragma unroll
-        for (int i = 0; i < PER; i += 2) *reinterpret_cast<float2*>(dst + i) = make_float2(acc[i], acc[i + 1]);
-        if (col == 0) p.ml[slot * BR + r] = make_float2(M, L);
-      }
-      consumers_meet();
-      if (warp == 0) {
-        if (lane == 0 && ok) flag_set(p.flags + slot, p.call);
-        __syncwarp();
-        const bool all = flags_all(p.flags, 1, c0, c1, p.call);
-        if (all) flags_clear(p.flags, 1, c0, c1);
-        if (lane == 0) ml[0].x = all ? 1.f : 0.f;
-      }
-      consumers_meet();
-      done = ml[0].x != 0.f;
-      if (done) {
-        const int parts = c1 - c0 + 1;
-        consumers_meet();  // all have read ml[0]
-        float2* pml = reinterpret_cast<float2*>(merge);  // [part][BR]
-        for (int i = threadIdx.x; i < parts * BR; i += 256)
-          pml[i] = __ldcg(p.ml + (2LL * (c0 + i / BR) + (i < BR)) * BR + i % BR);
-        consumers_meet();
-        M = -CUDART_INF_F;
-        for (int c = 0; c < parts; ++c) M = fmaxf(M, pml[c * BR + r].x);
-        const float ref = M == -CUDART_INF_F ? 0.f : M;
-        L = 0.f;
-#pragma unroll
-        for (int i = 0; i < PER; ++i) acc[i] = 0.f;
-        if (there) {
-#pragma unroll 4
-          for (int c = 0; c < parts; ++c) {
-            const float2 y = pml[c * BR + r];
-            const float wt = ex2(y.x - ref);
-            L = fmaf(wt, y.y, L);
-            const float* src = p.part + ((2LL * (c0 + c) + (c == 0)) * BR + r) * D + col;
-#pragma unroll
-            for (int i = 0; i < PER; i += 2) {
-              const float2 f = __ldcg(reinterpret_cast<const float2*>(src + i));
-              acc[i] = fmaf(wt, f.x, acc[i]);
-              acc[i + 1] = fmaf(wt, f.y, acc[i + 1]);
-            }
-          }
-        }
-      }
-    }
-    if (done && there) {
-      const float inv = M == -CUDART_INF_F ? 0.f : 1.f / L;
-      uint32_t* dst = reinterpret_cast<uint32_t*>(
-          p.o + ((long long)(x.tok0 + row / group) * p.s.heads * group + w.h * group + row % group) * D + col);
-#pragma unroll
-      for (int i = 0; i < PER / 2; ++i) dst[i] = pack2<BF16>(acc[2 * i] * inv, acc[2 * i + 1] * inv);
-    }
-    consumers_meet();
-    w.advance(p.s, p.blocks);
-  }
-  if (blockIdx.x == 0) {
-    // zeroes the rows of packed tokens that belong to no sequence
-    const int first = min(max(p.s.cu_new[p.s.batch], 0), p.s.total);
-    const long long row = (long long)p.s.heads * group * D;
-    for (long long i = first * row + threadIdx.x; i < p.s.total * row; i += 256) p.o[i] = 0;
+    __syncwarp();
+    if (lane == 0) mbar_arrive(join_full);
   }
 }
 
