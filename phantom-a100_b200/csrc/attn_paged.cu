@@ -17,7 +17,7 @@
 //     that several CTAs share (fp32 rows, reference maximum, sum) are joined in the order of the CTAs by the one that
 //     finishes last: the result depends on the lengths and the GPU's SM count alone.
 //   * Two producer warps read the page table and keep a ring of tiles in flight by TMA (a box per page, swizzled, so that
-//     pages of 16 tokens land as one conflict-free tile); 128 KB in flight for each SM.
+//     pages of 16 tokens land as one conflict-free tile), two tiles to each pair of consumer warps.
 //   * Eight consumer warps work without meeting: two to a tile, 32 keys each, every warp with its own running maximum,
 //     sum and output. At the end of a unit they leave these in shared memory and go on to the next, whose queries a
 //     producer has brought there; four further warps join and write them. (With the consumers doing this themselves a
@@ -42,31 +42,35 @@ namespace phantom {
 namespace rows {
 
 // A unit has 8 NT query rows (NT = 1, 2).
-constexpr int BN = 64;        // keys of a tile
-constexpr int kConsumers = 8; // warps; pairs of them take the tiles in turn
 constexpr int kJoiners = 4;
-constexpr int K_WARP = kConsumers + kJoiners, V_WARP = K_WARP + 1;  // producers; two idle warps complete their warpgroup
-constexpr int kThreads = 32 * 16;
-// Registers: 512 threads launch with 128 each; 2 * 168 + 104 + 72 = 4 * 128 (setmaxnreg, by warpgroup).
-constexpr int kRegsConsumer = 168, kRegsJoiner = 104, kRegsProducer = 72;
 constexpr int kUnitRing = 4;
 constexpr int kErrCopyWait = 1, kErrTileWait = 4, kErrJoinWait = 8;
+
+// Warps: eight consumers, in pairs that take the tiles in turn; the joiners; four producers. Registers (setmaxnreg, by
+// warpgroup): 512 threads launch with 128 each; 2 * 168 + 104 + 72 = 4 * 128.
+constexpr int kConsumers = 8, PRODUCER = kConsumers + kJoiners, kThreads = 32 * (PRODUCER + 4);
+constexpr int kRegsConsumer = 168, kRegsJoiner = 104, kRegsProducer = 72;
 
 template <int D, bool INT8, int NT>
 struct Cfg {
   static constexpr int BR = 8 * NT;
   static constexpr int ROW = INT8 ? D : 128;              // bytes of a swizzled row (16-bit: 64 columns)
   static constexpr int BLOCKS = INT8 ? 1 : D / 64;        // such blocks across d
-  static constexpr int HALF = BN * D * (INT8 ? 1 : 2);    // keys (or values) of a tile
-  static constexpr int SLOT = 2 * HALF;
-  // A multiple of the four pairs: a slot's tiles then all go to one pair, which sees every phase of its barriers. (With a
-  // slot passed between pairs, a pair could wait for a phase whose predecessor was still open, and parity would let it by.)
-  static constexpr int SLOTS = INT8 ? (D == 128 ? 8 : 16) : (D == 128 ? 4 : 8);
-  static_assert(SLOTS % 4 == 0, "each ring slot belongs to one pair of warps");
-  static constexpr int OFF_MERGE = SLOTS * SLOT;          // [kConsumers][BR][D] fp32
-  static constexpr int OFF_ML = OFF_MERGE + kConsumers * BR * D * 4;
+  static constexpr bool WIDE = !INT8 && D == 128 && NT == 1;
+  static constexpr int SLOT = (WIDE ? 32 : 16) * 1024, HALF = SLOT / 2;  // a tile: its keys, its values
+  static constexpr int BN = HALF / (D * (INT8 ? 1 : 2));  // keys of a tile: 32, 64 or 128
+  static constexpr int MT = BN <= 64 || NT == 1 ? BN / 32 : 2;  // 16 MT keys at a time go through a warp
+  static constexpr int SUB = BN / (32 * MT);              // times
+  // Two slots to a pair, so that a pair's next tile is on its way while it works on one. A slot's tiles all go to one pair,
+  // which so sees every phase of its barriers. (With a slot passed between pairs, a pair could wait for a phase whose
+  // predecessor was still open, and parity would let it by.)
+  static constexpr int PAIRS = WIDE ? 3 : 4, WARPS = 2 * PAIRS, SLOTS = 2 * PAIRS;
+  // producers of a tile: keys, values, and an 8-bit cache's scales of each
+  static constexpr int PRODUCERS = INT8 ? 4 : 2;
+  static constexpr int OFF_MERGE = SLOTS * SLOT;          // [WARPS][BR][D] fp32
+  static constexpr int OFF_ML = OFF_MERGE + WARPS * BR * D * 4;
   static constexpr int Q_ROW = 2 * D + 16;                // padded: lanes of 8 rows and 4 words read without conflicts
-  static constexpr int OFF_Q = OFF_ML + kConsumers * BR * 8;
+  static constexpr int OFF_Q = OFF_ML + WARPS * BR * 8;
   static constexpr int OFF_SCALE = OFF_Q + kUnitRing * BR * Q_ROW;
   static constexpr int OFF_UNIT = OFF_SCALE + (INT8 ? SLOTS * 2 * BN * 4 : 0);
   static constexpr int OFF_BAR = OFF_UNIT + kUnitRing * 48;
@@ -77,8 +81,8 @@ struct Cfg {
 
 
 // ------------------------------------------------------------------------------------------------ units and tiles
-// Units of 8 NT rows; tiles of 64 keys.
-template <int NT>
+// Units of 8 NT rows; tiles of BN keys.
+template <int NT, int BN>
 struct RowBlocks {
   int group, causal, heads;
   static constexpr int kTile = BN, BR = 8 * NT;
@@ -91,7 +95,7 @@ struct RowBlocks {
   __device__ long long head_tiles(const Seq& x) const { return sum_tiles(*this, x); }
 };
 
-template <int NT>
+template <int NT, int BN>
 struct Params {
   PagedSeqs s;
   const uint16_t* q;
@@ -99,7 +103,7 @@ struct Params {
   uint16_t* o;
   const float *ks, *vs;
   Strides3 kss, vss;
-  RowBlocks<NT> blocks;
+  RowBlocks<NT, BN> blocks;
   float scale_log2;  // of the scores' size
   uint32_t flip;     // sign bits to flip in the queries (a negative scale)
   float* part;       // parts of shared units, [place][8 NT] rows of D sums of values
@@ -152,9 +156,10 @@ struct Unit {
 
 template <int D, bool BF16, bool INT8, int NT>
 __global__ void __launch_bounds__(kThreads, 1)
-attn_rows(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV, const Params<NT> p) {
+attn_rows(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV, const Params<NT, Cfg<D, INT8, NT>::BN> p) {
   using C = Cfg<D, INT8, NT>;
-  constexpr int BR = C::BR;
+  using Blocks = RowBlocks<NT, C::BN>;
+  constexpr int BR = C::BR, BN = C::BN, MT = C::MT;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   const uint32_t sbase = smem_u32(smem), bars = sbase + C::OFF_BAR;
@@ -172,14 +177,14 @@ attn_rows(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUten
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < C::SLOTS; ++s) {
-      mbar_init(full(s), 2);   // the producers
+      mbar_init(full(s), C::PRODUCERS);
       mbar_init(empty(s), 2);  // the consuming pair
     }
     for (int u = 0; u < kUnitRing; ++u) {
       mbar_init(q_full(u), 1);
-      mbar_init(q_empty(u), kConsumers + kJoiners);
+      mbar_init(q_empty(u), C::WARPS + kJoiners);
     }
-    mbar_init(join_full, kConsumers);
+    mbar_init(join_full, C::WARPS);
     mbar_init(join_empty, kJoiners);
     *abort_flag = 0;
     fence_mbar_init();
@@ -205,26 +210,35 @@ attn_rows(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUten
     return x;
   };
 
-  if (warp >= K_WARP) {
+  if (warp >= PRODUCER) {
     setmaxnreg_dec<kRegsProducer>();
-    if (warp > V_WARP) return;
-    // Producers, one of the keys (and of the units' records and queries) and one of the values: a tile's boxes, one to a
-    // page, and an 8-bit cache's scales. Each walks the CTA's share by itself. One elected lane of warp-uniform code issues
-    // the copies; the issue is what limits pages of 16 tokens, hence two warps.
-    const bool vals = warp == V_WARP;
+    const int role = warp - PRODUCER;
+    if (role >= C::PRODUCERS) return;
+    // Producers: of the keys (and of the units' records and queries), of the values, and of an 8-bit cache's scales of
+    // each, a copy to a page. Each walks the CTA's share by itself. One elected lane of warp-uniform code issues the
+    // copies: that issue is what limits pages of 16 tokens, hence a warp for each kind. Page ids are held a lane each, 32
+    // pages ahead of their use.
+    const bool vals = role & 1;
     const CUtensorMap* map = vals ? &tmV : &tmK;
-    if (elect_one()) tma_prefetch_desc(map);
+    if (role < 2 && elect_one()) tma_prefetch_desc(map);
     __syncwarp();
-    Walk<RowBlocks<NT>> w;
+    Walk<Blocks> w;
     w.start(p.s, p.blocks, blockIdx.x, gridDim.x);
     int t = 0, nu = 0;
     bool ok = true;
-    const int page = 1 << p.s.page_log2, box = min(page, BN);
+    const int page_log2 = p.s.page_log2, page = 1 << page_log2, box = min(page, BN);
     const Strides3 st = vals ? p.vss : p.kss;
     const float* scale = vals ? p.vs : p.ks;
+    const uint32_t bytes = role < 2 ? box * D * (INT8 ? 1 : 2) : box * 4;  // of a copy
+    const uint32_t dst0 = role < 2 ? sbase + role * C::HALF : sbase + C::OFF_SCALE + vals * BN * 4;
+    const uint32_t slot_bytes = role < 2 ? C::SLOT : 2 * BN * 4;
     while (w.cur < w.end) {
       const int end = p.blocks.key_end(w.x, w.blk), cnt = w.count();
-      if (!vals) {
+      const int pages = (end + page - 1) >> page_log2;  // that the unit sees
+      int base = (w.tile * BN) >> page_log2;
+      auto ids_from = [&](int i) { return i + lane < pages ? page_of(p.s, w.b, i + lane) : 0; };
+      int ids = ids_from(base), next = ids_from(base + 32);
+      if (role == 0) {
         if (nu >= kUnitRing && !(ok = wait(q_empty(nu), (nu / kUnitRing - 1) & 1, kErrCopyWait))) break;
         const int row0 = w.blk * BR, rows = min(BR, w.x.n * group - row0);
         const long long w0 = w.cur - w.tile;
@@ -245,24 +259,35 @@ attn_rows(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUten
         __syncwarp();
         ++nu;
       }
+      const float* head_scale = scale + w.h * st.head;
       for (int i = 0; i < cnt; ++i, ++t) {
         const int s = t % C::SLOTS, round = t / C::SLOTS;
-        const int j0 = (w.tile + i) * BN;
+        const int j0 = (w.tile + i) * BN, place = j0 & (page - 1);
         const int boxes = max(0, (min(j0 + BN, end) - j0 + box - 1) / box);  // pages of the tile that hold keys
-        int id = 0;
-        if (lane < boxes) id = page_of(p.s, w.b, (j0 >> p.s.page_log2) + lane);
         if (round > 0 && !(ok = wait(empty(s), (round - 1) & 1, kErrCopyWait))) break;
-        const int place = j0 & (page - 1);
-        const uint32_t dst = sbase + s * C::SLOT + (vals ? C::HALF : 0);
-        if (elect_one()) mbar_arrive_expect_tx(full(s), boxes * box * (D * (INT8 ? 1 : 2) + (INT8 ? 4 : 0)));
-        for (int pg = 0; pg < boxes; ++pg) {
-          const int from = __shfl_sync(0xffffffffu, id, pg);
+        const uint32_t dst = dst0 + s * slot_bytes;
+        if (elect_one()) mbar_arrive_expect_tx(full(s), boxes * bytes);
+        for (int pg = 0; pg < boxes; pg += 4) {
+          // up to four pages at once (a tile's are 1, 2, or a multiple of 4, and begin at a multiple of that in the 32)
+          const int at = (j0 >> page_log2) + pg;
+          if (at - base >= 32) {
+            base += 32;
+            ids = next;
+            next = ids_from(base + 32);
+          }
+          int from[4];
+#pragma unroll
+          for (int k = 0; k < 4; ++k) from[k] = __shfl_sync(0xffffffffu, ids, at - base + k);
           if (elect_one()) {
-            // an id that is out of range reads as zeros (the map's bounds)
-            tma_load_5d(dst + pg * box * C::BLOCKS * C::ROW, map, full(s), 0, place, 0, w.h, from);
-            if constexpr (INT8)
-              bulk_load(sbase + C::OFF_SCALE + (s * 2 + vals) * BN * 4 + pg * box * 4,
-                        scale + max(from, 0) * st.page + w.h * st.head + place, box * 4, full(s));
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              if (pg + k >= boxes) break;
+              const uint32_t to = dst + (pg + k) * bytes;
+              if (role < 2)  // an id that is out of range reads as zeros (the map's bounds)
+                tma_load_5d(to, map, full(s), 0, place, 0, w.h, from[k]);
+              else
+                bulk_load(to, head_scale + max(from[k], 0) * st.page + place, bytes, full(s));
+            }
           }
         }
         __syncwarp();
@@ -270,7 +295,7 @@ attn_rows(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUten
       if (!ok) break;
       w.advance(p.s, p.blocks);
     }
-    if (!vals) {
+    if (role == 0) {
       if (ok && nu >= kUnitRing) ok = wait(q_empty(nu), (nu / kUnitRing - 1) & 1, kErrCopyWait);
       if (ok) {
         if (elect_one()) {
@@ -308,11 +333,11 @@ attn_rows(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUten
 #pragma unroll
       for (int i = 0; i < PER; ++i) acc[i] = 0.f;
 #pragma unroll
-      for (int v = 0; v < kConsumers; ++v) M = fmaxf(M, ml[v * BR + r].x);
+      for (int v = 0; v < C::WARPS; ++v) M = fmaxf(M, ml[v * BR + r].x);
       {
         const float ref = M == -CUDART_INF_F ? 0.f : M;
 #pragma unroll 2
-        for (int v = 0; v < kConsumers; ++v) {
+        for (int v = 0; v < C::WARPS; ++v) {
           const float2 y = ml[v * BR + r];
           if (y.x == -CUDART_INF_F && y.y == 0.f) continue;  // no key seen, and maybe nothing written
           const float wt = ex2(y.x - ref);
@@ -333,7 +358,7 @@ attn_rows(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUten
         __syncwarp();
         if (lane == 0) mbar_arrive(join_empty);
       } else {
-        const long long slot = Walk<RowBlocks<NT>>::place(blockIdx.x, (int)blockIdx.x == x.c0);
+        const long long slot = Walk<Blocks>::place(blockIdx.x, (int)blockIdx.x == x.c0);
         if (there) {
           float* dst = p.part + (slot * BR + r) * D + col;
 #pragma unroll
@@ -403,16 +428,21 @@ attn_rows(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUten
   }
 
   setmaxnreg_inc<kRegsConsumer>();
+  if (warp >= C::WARPS) return;
   const int g = lane >> 2, t4 = lane & 3;
-  const int pair = warp >> 1, kr = (warp & 1) * 32;  // this warp's keys of its pair's tiles
-  // Where this lane's rows for ldmatrix lie in a tile: 16 keys from kr + 16 mt, matrices (keys 0-7, 8-15) x (first, second
+  const int pair = warp >> 1;
+  constexpr int KEYS = 16 * MT;  // that go through this warp at a time
+  const int kr = (warp & 1) * (BN / 2);  // its first key of its pair's tiles
+  // Where this lane's rows for ldmatrix lie in a tile: 16 keys from kr + KEYS sub + 16 mt, matrices (keys 0-7, 8-15) x (first, second
   // 16-byte chunk of a pair); V^T of 16-bit values has the two the other way around. Boxes of min(page, 64) tokens, each
   // [64-column block][token][ROW bytes]; a chunk lies at its number ^ the row's swizzle, so stepping over pairs of chunks
   // is an XOR with 32 times the pair's number.
-  const int box_log2 = min(p.s.page_log2, 6), blk_stride = C::ROW << box_log2;
-  uint32_t at_k[2], at_v[2];
+  const int box_log2 = min(p.s.page_log2, BN == 32 ? 5 : BN == 64 ? 6 : 7), blk_stride = C::ROW << box_log2;
+  constexpr int AT = C::BLOCKS == 1 ? 1 : MT;  // one column block: 16 rows further on is a constant away
+  static_assert(C::SUB == 1 || C::BLOCKS == 1);
+  uint32_t at_k[AT], at_v[AT];
 #pragma unroll
-  for (int mt = 0; mt < 2; ++mt) {
+  for (int mt = 0; mt < AT; ++mt) {
     auto place_of = [&](int key, int chunk) {
       const int row = C::BLOCKS == 1 ? key : (((key >> box_log2) * C::BLOCKS) << box_log2) + (key & ((1 << box_log2) - 1));
       const int sw = C::ROW == 128 ? key & 7 : (key >> 1) & 3;
@@ -422,7 +452,7 @@ attn_rows(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUten
     at_k[mt] = place_of(key + ((lane >> 3) & 1) * 8, lane >> 4);
     at_v[mt] = INT8 ? at_k[mt] : place_of(key + (lane >> 4) * 8, (lane >> 3) & 1);
   }
-  int t = 0;
+  int t = 0, first = pair;  // tiles before this unit; the first of it that is this pair's
   for (int u = 0;; ++u) {
     const Unit x = next_unit(u);
     if (x.id < 0) break;
@@ -465,23 +495,25 @@ attn_rows(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUten
     }
 
     bool ok = true;
-    for (int i = (pair - t) & 3; i < x.cnt; i += 4) {  // every fourth tile
+    for (int i = first; i < x.cnt; i += C::PAIRS) {  // tiles of the whole share go to the pairs in turn
       const int s = (t + i) % C::SLOTS;
       if (!(ok = wait(full(s), ((t + i) / C::SLOTS) & 1, kErrTileWait))) break;
-      const uint32_t kb = sbase + s * C::SLOT, vb = kb + C::HALF;
-      const int j0 = (x.tile0 + i) * BN + kr;  // this warp's first key
-      if (j0 < end) {
+#pragma unroll 1
+      for (int sub_i = 0; sub_i < C::SUB; ++sub_i) {
+        const uint32_t kb = sbase + s * C::SLOT + sub_i * KEYS * C::ROW, vb = kb + C::HALF;
+        const int j0 = (x.tile0 + i) * BN + kr + sub_i * KEYS;  // the first key
+        if (j0 >= end) break;
         // ---- scores: [16 keys][8 rows]: (key g: rows 2 t4, + 1; key g + 8: the same)
-        float sc[2][NT][4];
+        float sc[MT][NT][4];
 #pragma unroll
-        for (int mt = 0; mt < 2; ++mt) {
+        for (int mt = 0; mt < MT; ++mt) {
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt) sc[mt][nt][0] = sc[mt][nt][1] = sc[mt][nt][2] = sc[mt][nt][3] = 0.f;
           if constexpr (INT8) {
 #pragma unroll
             for (int k = 0; k < D / 32; ++k) {
               uint32_t r[4], a[2][4];
-              ldsm4(kb + (at_k[mt] ^ (k << 5)), r);
+              ldsm4(kb + mt * 16 * C::ROW + (at_k[0] ^ (k << 5)), r);
 #pragma unroll
               for (int e = 0; e < 4; ++e) {  // r: (keys 0-7, 8-15) of chunk 2 k, then of 2 k + 1
                 if constexpr (BF16) {
@@ -503,18 +535,18 @@ attn_rows(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUten
 #pragma unroll
             for (int k = 0; k < D / 16; ++k) {
               uint32_t r[4];
-              ldsm4(kb + (k >> 2) * blk_stride + (at_k[mt] ^ ((k & 3) << 5)), r);
+              ldsm4(kb + (C::BLOCKS == 1 ? mt * 16 * C::ROW : (k >> 2) * blk_stride) + (at_k[C::BLOCKS == 1 ? 0 : mt] ^ ((k & 3) << 5)), r);
 #pragma unroll
               for (int nt = 0; nt < NT; ++nt) mma16816<BF16>(sc[mt][nt], r, qb[nt][k][0], qb[nt][k][1]);
             }
           }
         }
         // ---- 8-bit: to the log2 domain, with the values' scales; masks
-        float inv_vs[2][2];
+        float inv_vs[MT][2];
         if constexpr (INT8) {
-          const float* scl = reinterpret_cast<const float*>(smem + C::OFF_SCALE + s * 2 * BN * 4) + kr + g;
+          const float* scl = reinterpret_cast<const float*>(smem + C::OFF_SCALE + s * 2 * BN * 4) + kr + sub_i * KEYS + g;
 #pragma unroll
-          for (int mt = 0; mt < 2; ++mt)
+          for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
               const float a = scl[mt * 16 + e * 8] * p.scale_log2, v = scl[BN + mt * 16 + e * 8], lv = __log2f(v);
@@ -527,9 +559,9 @@ attn_rows(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUten
               }
             }
         }
-        if (j0 + 32 > lim_least) {
+        if (j0 + KEYS > lim_least) {
 #pragma unroll
-          for (int mt = 0; mt < 2; ++mt)
+          for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -544,7 +576,9 @@ attn_rows(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUten
         for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
-            float y = fmaxf(fmaxf(sc[0][nt][e], sc[0][nt][2 + e]), fmaxf(sc[1][nt][e], sc[1][nt][2 + e]));
+            float y = fmaxf(sc[0][nt][e], sc[0][nt][2 + e]);
+#pragma unroll
+            for (int mt = 1; mt < MT; ++mt) y = fmaxf(y, fmaxf(sc[mt][nt][e], sc[mt][nt][2 + e]));
             y = fmaxf(y, __shfl_xor_sync(0xffffffffu, y, 4));
             y = fmaxf(y, __shfl_xor_sync(0xffffffffu, y, 8));
             y = fmaxf(y, __shfl_xor_sync(0xffffffffu, y, 16));
@@ -568,9 +602,9 @@ attn_rows(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUten
             }
         }
         // ---- probabilities, turned into B operands (16 keys by 8 rows)
-        uint32_t hi[2][NT][2], lo[2][NT][2];
+        uint32_t hi[MT][NT][2], lo[MT][NT][2];
 #pragma unroll
-        for (int mt = 0; mt < 2; ++mt)
+        for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -596,9 +630,9 @@ attn_rows(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUten
               }
             }
         // ---- values; those of keys past the end are zeroed (what lies in the page there may be anything)
-        const bool tail = j0 + 32 > end;
+        const bool tail = j0 + KEYS > end;
 #pragma unroll
-        for (int mt = 0; mt < 2; ++mt) {
+        for (int mt = 0; mt < MT; ++mt) {
           uint32_t keep[2] = {0xffffffffu, 0xffffffffu};
           if (tail) {
 #pragma unroll
@@ -611,7 +645,7 @@ attn_rows(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUten
 #pragma unroll
             for (int c = 0; c < D / 32; ++c) {
               uint32_t r[4], a[2][4];
-              ldsm4_t(vb + (at_v[mt] ^ (c << 5)), r);
+              ldsm4_t(vb + mt * 16 * C::ROW + (at_v[0] ^ (c << 5)), r);
 #pragma unroll
               for (int e = 0; e < 4; ++e) {  // r: (keys 0-7, 8-15) of columns 32 c ... + 15, then ... + 31; even and odd columns
                 const uint32_t u = (tail ? r[e] & keep[e & 1] : r[e]) ^ 0x80808080u;
@@ -628,7 +662,7 @@ attn_rows(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUten
 #pragma unroll
             for (int c = 0; c < D / 16; ++c) {
               uint32_t r[4];
-              ldsm4_t(vb + (c >> 2) * blk_stride + (at_v[mt] ^ ((c & 3) << 5)), r);
+              ldsm4_t(vb + (C::BLOCKS == 1 ? mt * 16 * C::ROW : (c >> 2) * blk_stride) + (at_v[C::BLOCKS == 1 ? 0 : mt] ^ ((c & 3) << 5)), r);
               if (tail) {
                 r[0] &= keep[0];
                 r[1] &= keep[0];
@@ -649,6 +683,8 @@ attn_rows(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUten
     }
 
     t += x.cnt;
+    first = (first - x.cnt) % C::PAIRS;
+    if (first < 0) first += C::PAIRS;
     if (!ok) break;
 
     // ---- for the joiners: rows in shared memory, columns swizzled by 8 floats with the row (no bank conflicts)
@@ -694,7 +730,7 @@ cudaError_t launch(const PagedAttnArgs& a, int dev) {
     attr.store(true, std::memory_order_release);
   }
   CUtensorMap mk, mv;
-  const int page = 1 << a.s.page_log2, box = std::min(page, BN), elem = INT8 ? 1 : 2, cols = INT8 ? D : 64;
+  const int page = 1 << a.s.page_log2, box = std::min(page, C::BN), elem = INT8 ? 1 : 2, cols = INT8 ? D : 64;
   if (!make_paged_map(&mk, a.kc, a.s.num_pages, a.s.heads, page, D, a.kcs, elem, BF16, cols, box, C::BLOCKS, 1) ||
       !make_paged_map(&mv, a.vc, a.s.num_pages, a.s.heads, page, D, a.vcs, elem, BF16, cols, box, C::BLOCKS, 1))
     return cudaErrorInvalidValue;
@@ -702,8 +738,9 @@ cudaError_t launch(const PagedAttnArgs& a, int dev) {
   void* block = nullptr;
   if ((e = scratch_alloc(dev, part_bytes + ml_bytes + places * 8, a.stream, &block)) != cudaSuccess) return e;
   char* base = static_cast<char*>(block);
-  Params<NT> p{a.s, static_cast<const uint16_t*>(a.q), a.q_token, a.q_head, static_cast<uint16_t*>(a.o), a.ks, a.vs, a.kss, a.vss,
-               RowBlocks<NT>{a.group, a.causal ? 1 : 0, a.s.heads},
+  constexpr int BN = C::BN;
+  Params<NT, BN> p{a.s, static_cast<const uint16_t*>(a.q), a.q_token, a.q_head, static_cast<uint16_t*>(a.o), a.ks, a.vs, a.kss, a.vss,
+               RowBlocks<NT, BN>{a.group, a.causal ? 1 : 0, a.s.heads},
                (INT8 ? a.scale : fabsf(a.scale)) * 1.4426950408889634f, !INT8 && a.scale < 0.f ? 0x80008000u : 0u,
                reinterpret_cast<float*>(base), reinterpret_cast<float2*>(base + part_bytes),
                reinterpret_cast<unsigned long long*>(base + part_bytes + ml_bytes), next_call()};
