@@ -549,7 +549,8 @@ attn_rows(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUten
           for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
-              const float a = scl[mt * 16 + e * 8] * p.scale_log2, v = scl[BN + mt * 16 + e * 8], lv = __log2f(v);
+              const float a = scl[mt * 16 + e * 8] * p.scale_log2, v = least_scale(scl[BN + mt * 16 + e * 8]),
+                          lv = __log2f(v);
               // past the end a scale may be anything; p' is 0 there
               inv_vs[mt][e] = j0 + mt * 16 + e * 8 + g < end ? __fdividef(1.f, v) : 0.f;
 #pragma unroll

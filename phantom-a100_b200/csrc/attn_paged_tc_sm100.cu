@@ -10,7 +10,12 @@
 //   * Rows of the last tile past the keys that the unit sees may hold anything (the page's stale rest, or what an earlier
 //     tile left): their scores are masked by selection, and their values are zeroed, since 0 * NaN is NaN in a product.
 //
-// The probabilities are rounded to the cache's 16-bit type, as tcgen05.mma wants P and V of one type: half an ulp of each,
+//   * An 8-bit cache goes through a warpgroup that reads its pages, turns the bytes into 16-bit numbers (the whole numbers
+//     themselves, exact: keys in the queries' type, values in fp16) and writes them where TMA would have put them. The
+//     scales take no part in the products: the softmax multiplies a key's scale into the score and puts the value's into
+//     the exponent, as in attn_paged.cu.
+//
+// The probabilities are rounded to the 16-bit type of V (fp16 for an 8-bit cache), as tcgen05.mma wants P and V of one type: half an ulp of each,
 // which adds to the output an error of the size of its own rounding (sqrt(2) times in all).
 #include <cuda.h>
 #include <math_constants.h>
@@ -28,15 +33,17 @@ namespace chunk {
 constexpr int BM = 128;  // rows of a query tile = TMEM lanes
 constexpr int BN = 128;  // keys of a tile
 constexpr int MMA_WARP = 8, TMA_WARP = 9, PV_WARP = 10, V_WARP = 11;
-constexpr int kThreads = 384;
-// Register split, as in attn_tc_sm100.cu: 384 threads launch with 168 each; 128 * (168 - 72) = 2 * 128 * (216 - 168).
-constexpr int kRegsProducer = 72, kRegsSoftmax = 216;
+constexpr int CONV_WARP = 12;  // and the three after it: 8-bit caches
+// Register split (setmaxnreg, by warpgroup). 16-bit: 384 threads launch with 168 each, 2 * 216 + 72 = 3 * 168. 8-bit: 512
+// threads with 128 each, 2 * 184 + 72 + 72 = 4 * 128.
+constexpr int kRegsProducer = 72;
 constexpr float kRescaleThreshold = 8.0f;  // log2 units: rescale O only when the maximum grows by more than 2^8
 constexpr int kErrTmaWait = 1, kErrMmaWait = 2, kErrSoftmaxWait = 4, kErrEpilogueWait = 8;
 constexpr int kUnitRing = 4;
 
-template <int D>
+template <int D, bool INT8>
 struct Cfg {
+  static constexpr int THREADS = INT8 ? 512 : 384, REGS_SOFTMAX = INT8 ? 184 : 216;
   static constexpr bool SHARED_S = D == 128;       // one S region for both query tiles (d = 128), or one each
   static constexpr int KBLK = D / 64;              // 64-column (128-byte) swizzle blocks across d
   static constexpr int SUB = BN * 128;             // one such block of a tile of 128 rows
@@ -46,8 +53,10 @@ struct Cfg {
   static constexpr int OFF_KV = 2 * TILE;
   static constexpr int OFF_OST = OFF_KV + STAGES * TILE;  // output staging: per softmax warp 32 rows of 64 bytes
   static constexpr int OST_WARP = 32 * 64;
-  static constexpr int OFF_BAR = OFF_OST + 8 * OST_WARP;
-  static constexpr int NUM_BARS = 2 * STAGES + 7 * 2 + 3;
+  static constexpr int SCALES = INT8 ? 4 : 0;      // tiles' scales in flight: the keys', log2 of the values', 1 / these
+  static constexpr int OFF_SCALE = OFF_OST + 8 * OST_WARP;
+  static constexpr int OFF_BAR = OFF_SCALE + SCALES * 3 * BN * 4;
+  static constexpr int NUM_BARS = 2 * STAGES + 7 * 2 + 3 + (INT8 ? 2 * SCALES + kUnitRing : 0);
   static constexpr int OFF_MISC = (OFF_BAR + NUM_BARS * 8 + 15) / 16 * 16;  // TMEM base, abort flag, unit ring
   static constexpr int SMEM = OFF_MISC + 16 + 48 * kUnitRing + 1024;
   static_assert(SMEM <= 227 * 1024, "shared memory plan exceeds 227 KB");
@@ -97,6 +106,9 @@ struct Params {
   uint16_t* o;
   float scale_log2;        // of the scores' size; their sign is in the instruction (negate)
   int negate;
+  const int8_t *kc, *vc;   // 8-bit cache, read by plain loads
+  const float *ks, *vs;
+  Strides3 kcs, vcs, kss, vss;
   float4* part;            // partial results: [CTA][2][query tile][D / 4][row], fp32
   float2* ml;              // their (reference maximum, sum): [CTA][2][query tile][row]
 };
@@ -121,18 +133,21 @@ __device__ __forceinline__ float row_max(const float (&s)[N]) {
 }
 
 // p = exp2(s * scale - sub) of 64 scores as packed 16-bit pairs; returns the sum of the unrounded values. Every fourth pair
-// by the FMA pipe's polynomial, as in attn_tc_sm100.cu, with an exact zero where bf16 could hold its 2^-125.
-template <bool BF16, int OFF>
-__device__ __forceinline__ float softmax64(const float (&s)[BN], float scale_log2, float sub, uint32_t (&p)[32]) {
+// by the FMA pipe's polynomial, as in attn_tc_sm100.cu, with an exact zero where its 2^-125 would count: bf16 holds it, and
+// an 8-bit cache's sum multiplies it with 1 / vs (`inv`, of the 64 keys).
+template <bool BF16, bool INT8, int OFF>
+__device__ __forceinline__ float softmax64(const float (&s)[BN], float scale_log2, float sub, const float* inv, uint32_t (&p)[32]) {
   const float2 sc = make_float2(scale_log2, scale_log2), nm = make_float2(-sub, -sub);
   float2 acc[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+  float4 iv;
 #pragma unroll
   for (int c = 0; c < 32; ++c) {
-    float2 x = fma2(make_float2(s[OFF + 2 * c], s[OFF + 2 * c + 1]), sc, nm);
+    float2 x = make_float2(s[OFF + 2 * c], s[OFF + 2 * c + 1]);
+    x = INT8 ? add2(x, nm) : fma2(x, sc, nm);
     if ((0x09 >> (c & 7)) & 1) {
       const float2 arg = x;
       x = exp2_fma2(x);
-      if constexpr (BF16) {
+      if constexpr (BF16 || INT8) {
         x.x = arg.x < -125.f ? 0.f : x.x;
         x.y = arg.y < -125.f ? 0.f : x.y;
       }
@@ -140,18 +155,23 @@ __device__ __forceinline__ float softmax64(const float (&s)[BN], float scale_log
       x.x = ex2(x.x);
       x.y = ex2(x.y);
     }
-    acc[c & 1] = add2(acc[c & 1], x);
-    p[c] = pack2<BF16>(x.x, x.y);
+    if constexpr (INT8) {
+      if (c % 2 == 0) iv = *reinterpret_cast<const float4*>(inv + 2 * c);
+      acc[c & 1] = fma2(x, c % 2 == 0 ? make_float2(iv.x, iv.y) : make_float2(iv.z, iv.w), acc[c & 1]);
+    } else {
+      acc[c & 1] = add2(acc[c & 1], x);
+    }
+    p[c] = pack2<BF16 && !INT8>(x.x, x.y);
   }
   const float2 t = add2(acc[0], acc[1]);
   return t.x + t.y;
 }
 
-template <int D, bool BF16>
-__global__ void __launch_bounds__(kThreads, 1)
+template <int D, bool BF16, bool INT8>
+__global__ void __launch_bounds__(Cfg<D, INT8>::THREADS, 1)
 attn_chunk(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
            const __grid_constant__ CUtensorMap tmV, const Params p) {
-  using C = Cfg<D>;
+  using C = Cfg<D, INT8>;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   const uint32_t sbase = smem_u32(smem);
@@ -169,6 +189,11 @@ attn_chunk(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUte
   auto o_done = [&](int g) { return bar0 + 8u * (B0 + 10 + g); };
   auto o_free = [&](int g) { return bar0 + 8u * (B0 + 12 + g); };
   const uint32_t q_free = bar0 + 8u * (B0 + 14), drain_bar = bar0 + 8u * (B0 + 15), drain_pv_bar = bar0 + 8u * (B0 + 16);
+  // 8-bit: the scales of tile j of the share are there, are done with; unit u's record is published
+  auto sc_full = [&](int j) { return bar0 + 8u * (B0 + 17 + j % 4); };
+  auto sc_empty = [&](int j) { return bar0 + 8u * (B0 + 21 + j % 4); };
+  auto rec_full = [&](int u) { return bar0 + 8u * (B0 + 25 + u % kUnitRing); };
+  static_assert(kUnitRing == 4);
   uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(smem + C::OFF_MISC);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + C::OFF_MISC + 4);
   int4* ring = reinterpret_cast<int4*>(smem + C::OFF_MISC + 16);  // [kUnitRing][3]
@@ -177,18 +202,24 @@ attn_chunk(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUte
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < C::STAGES; ++s) {
-      mbar_init(kv_full(s), 1);
+      mbar_init(kv_full(s), INT8 ? 4 : 1);  // the converting warps, or TMA's issuer
       mbar_init(kv_empty(s), 1);
     }
     for (int g = 0; g < 2; ++g) {
       mbar_init(q_full(g), 1);
-      mbar_init(unit_read(g), 10);  // eight softmax warps, the two MMA warps
+      mbar_init(unit_read(g), INT8 ? 14 : 10);  // eight softmax warps, the two MMA warps, the converting warps
       mbar_init(s_full(g), 1);
       mbar_init(s_free(g), 128);
       mbar_init(p_ready(g), 128);
       mbar_init(o_done(g), 1);
       mbar_init(o_free(g), 128);
     }
+    if constexpr (INT8)
+      for (int j = 0; j < 4; ++j) {
+        mbar_init(sc_full(j), 4);
+        mbar_init(sc_empty(j), 8);
+        mbar_init(rec_full(j), 1);
+      }
     mbar_init(q_free, 1);
     mbar_init(drain_bar, 1);
     mbar_init(drain_pv_bar, 1);
@@ -238,6 +269,7 @@ attn_chunk(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUte
 
   if (warp == TMA_WARP || warp == V_WARP) {
     setmaxnreg_dec<kRegsProducer>();
+    if (!INT8 || warp == TMA_WARP) {
     // Producers: V_WARP copies the values, TMA_WARP the keys, and the units' records and queries. Each walks the CTA's
     // share by itself. One elected lane of warp-uniform code issues the copies; their issue is what limits pages of 16
     // tokens, hence two warps and, for the values, boxes of all columns (the tensor core takes V 16 keys at a time from
@@ -245,7 +277,7 @@ attn_chunk(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUte
     const bool vals = warp == V_WARP;
     if (elect_one()) {
       if (!vals) tma_prefetch_desc(&tmQ);
-      tma_prefetch_desc(vals ? &tmV : &tmK);
+      if (!INT8) tma_prefetch_desc(vals ? &tmV : &tmK);
     }
     __syncwarp();
     Walk<TokenBlocks> w;
@@ -281,9 +313,8 @@ attn_chunk(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUte
       const int cnt = w.count(), end = p.blocks.key_end(w.x, w.blk);
       int i = 0;
       if (!vals) {
-        copy_tile(w.tile * BN, end);  // before the wait for the last unit's queries to be done with
+        if (!INT8) copy_tile(w.tile * BN, end);  // before the waits for the last units to be done with
         i = 1;
-        if (ok && nu > 0) ok = wait(q_free, (nu - 1) & 1, kErrTmaWait);
         if (ok && nu > 1) ok = wait(unit_read(nu), ((nu >> 1) - 1) & 1, kErrTmaWait);
         if (!ok) break;
         Unit x;
@@ -299,6 +330,11 @@ attn_chunk(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUte
         x.slot = cnt == w.nt ? -1 : 2 * (int)blockIdx.x + (begin > w.cur - w.tile ? 0 : 1);
         if (elect_one()) {
           publish(nu, x);
+          if (INT8) mbar_arrive(rec_full(nu));
+        }
+        __syncwarp();
+        if (nu > 0 && !(ok = wait(q_free, (nu - 1) & 1, kErrTmaWait))) break;
+        if (elect_one()) {
           const int tiles = x.has_b ? 2 : 1;
           mbar_arrive_expect_tx(q_full(nu), tiles * C::KBLK * p.tile_tokens * p.group * 128);
           for (int g = 0; g < tiles; ++g)
@@ -310,18 +346,18 @@ attn_chunk(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUte
         ++nu;
         ++nq;
       }
-      for (; ok && i < cnt; ++i) copy_tile((w.tile + i) * BN, end);
+      for (; !INT8 && ok && i < cnt; ++i) copy_tile((w.tile + i) * BN, end);
       w.advance(p.s, p.blocks);
     }
     if (!vals && ok) {
       // the end of the units
-      if (nu > 0) ok = wait(q_free, (nu - 1) & 1, kErrTmaWait);
-      if (ok && nu > 1) ok = wait(unit_read(nu), ((nu >> 1) - 1) & 1, kErrTmaWait);
+      if (nu > 1) ok = wait(unit_read(nu), ((nu >> 1) - 1) & 1, kErrTmaWait);
       if (ok) {
         Unit x = {};
         x.id = -1;
         if (elect_one()) {
           publish(nu, x);
+          if (INT8) mbar_arrive(rec_full(nu));
           mbar_arrive(q_full(nu));
         }
         __syncwarp();
@@ -331,7 +367,119 @@ attn_chunk(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUte
     if (!ok) *abort_flag = 1;
     // every issued copy lands before this CTA's shared memory can be released
     for (int a = max(0, nq - 2); a < nq; ++a) mbar_wait_drain(q_full(a), (a >> 1) & 1);
-    for (int i = max((int)vals, t - C::STAGES); i < t; i += 2) mbar_wait_drain(kv_full(i % C::STAGES), (i / C::STAGES) & 1);
+    for (int i = max((int)vals, t - C::STAGES); !INT8 && i < t; i += 2) mbar_wait_drain(kv_full(i % C::STAGES), (i / C::STAGES) & 1);
+    }
+  } else if (INT8 && warp >= CONV_WARP) {
+    setmaxnreg_dec<72>();
+    // 8-bit pages to 16-bit tiles: keys of tile j, its values, keys of tile j + 1, ...; thread = 16-byte chunk of every
+    // 16 rows (16 rows lie in one page). The next item's bytes are on their way into the registers that the current one
+    // leaves. Rows past the unit's end become zeros, with scales of no effect.
+    constexpr int CHUNKS = D / 16, STEP = 128 / CHUNKS, N = BN / STEP;  // rows at a time; times
+    const int tid = threadIdx.x - 32 * CONV_WARP, chunk = tid % CHUNKS, row_in = tid / CHUNKS;
+    const int page_mask = (1 << p.s.page_log2) - 1;
+    int nu = 0, i = 0;
+    bool ok = true;
+    // the place being read: a tile of a unit, and the ids of its 16-row pieces (lanes 0-7)
+    Unit x;
+    x.id = -1;
+    auto take_unit = [&](int u) {
+      if (!(ok = wait(rec_full(u), (u / kUnitRing) & 1, kErrTmaWait))) return -1;
+      x = record(u);
+      __syncwarp();
+      if (x.id >= 0 && lane == 0) mbar_arrive(unit_read(u));
+      return x.id;
+    };
+    int ids = -1, j0 = 0;
+    auto take_ids = [&]() {
+      j0 = (x.tile0 + i) * BN;
+      ids = lane < 8 && j0 + lane * 16 < x.end ? page_of(p.s, x.b, (j0 + lane * 16) >> p.s.page_log2) : -1;
+    };
+    uint4 raw[N];
+    auto load = [&](int n, bool vals) {
+      const int row = n * STEP + row_in;
+      const int id = __shfl_sync(0xffffffffu, ids, row >> 4);
+      const Strides3& st = vals ? p.vcs : p.kcs;
+      raw[n] = make_uint4(0, 0, 0, 0);
+      if (id >= 0 && j0 + row < x.end)
+        raw[n] = *reinterpret_cast<const uint4*>((vals ? p.vc : p.kc) + id * st.page + x.h * st.head +
+                                                 ((j0 + row) & page_mask) * st.token + chunk * 16);
+    };
+    float ks = 0.f, vs = 1.f;
+    bool past = false;
+    auto load_scales = [&]() {
+      const int id = __shfl_sync(0xffffffffu, ids, tid >> 4);
+      const bool there = id >= 0 && j0 + tid < x.end;
+      const int place = (j0 + tid) & page_mask;
+      ks = there ? p.ks[id * p.kss.page + x.h * p.kss.head + place] : 0.f;
+      vs = there ? p.vs[id * p.vss.page + x.h * p.vss.head + place] : 1.f;
+      past = j0 + tid >= x.end;
+    };
+    if (take_unit(0) >= 0) {
+      take_ids();
+#pragma unroll
+      for (int n = 0; n < N; ++n) load(n, false);
+      load_scales();
+    }
+    for (int t = 0, j = 0; ok && x.id >= 0; ++j) {
+      // -- the tile's scales
+      if (j >= 4 && !(ok = wait(sc_empty(j), (j / 4 - 1) & 1, kErrTmaWait))) break;
+      float* scl = reinterpret_cast<float*>(smem + C::OFF_SCALE) + (j & 3) * 3 * BN + tid;
+      scl[0] = ks * p.scale_log2;
+      vs = least_scale(vs);
+      scl[BN] = past ? 0.f : __log2f(vs);
+      scl[2 * BN] = past ? 0.f : __fdividef(1.f, vs);
+      __syncwarp();
+      if (lane == 0) mbar_arrive(sc_full(j));
+      // -- keys, then values
+      for (int vals = 0; vals < 2; ++vals, ++t) {
+        const int s = t % C::STAGES, round = t / C::STAGES;
+        if (round > 0 && !(ok = wait(kv_empty(s), (round - 1) & 1, kErrTmaWait))) break;
+        const uint32_t dst = sbase + C::OFF_KV + s * C::TILE + (chunk >> 2) * C::SUB;
+        if (vals) {  // what comes next is the next tile
+          ++i;
+          if (i == x.cnt) {
+            i = 0;
+            ++nu;
+            take_unit(nu);
+          }
+          if (x.id >= 0) take_ids();
+        }
+        const bool more = !vals || x.id >= 0;
+#pragma unroll
+        for (int n = 0; n < N; ++n) {
+          const int row = n * STEP + row_in;
+          const uint32_t in[4] = {raw[n].x, raw[n].y, raw[n].z, raw[n].w};
+          uint32_t w[8];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            if (BF16 && !vals) {
+              w[2 * e] = bytes_bf16<0x4140>(in[e]);
+              w[2 * e + 1] = bytes_bf16<0x4342>(in[e]);
+            } else {
+              const uint32_t u = in[e] ^ 0x80808080u;
+              w[2 * e] = bytes_f16<0x4140>(u);
+              w[2 * e + 1] = bytes_f16<0x4342>(u);
+            }
+          }
+          if (more) load(n, !vals);
+          // (chunks of the two column blocks write their halves in opposite order: no bank conflicts)
+          const uint32_t at = dst + row * 128;
+          const int c0 = (chunk & 3) * 2, flip = (chunk >> 2) & 1;
+          const uint32_t lo = at + ((c0 ^ (row & 7)) << 4), hi = at + (((c0 + 1) ^ (row & 7)) << 4);
+          if (flip) {
+            st_shared_v4(hi, w[4], w[5], w[6], w[7]);
+            st_shared_v4(lo, w[0], w[1], w[2], w[3]);
+          } else {
+            st_shared_v4(lo, w[0], w[1], w[2], w[3]);
+            st_shared_v4(hi, w[4], w[5], w[6], w[7]);
+          }
+        }
+        if (vals && x.id >= 0) load_scales();
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(kv_full(s));
+      }
+    }
   } else if (warp == MMA_WARP || warp == PV_WARP) {
     setmaxnreg_dec<kRegsProducer>();
     const uint64_t dq = smem_desc_sw128(sbase + C::OFF_Q, 16, 1024);
@@ -384,9 +532,9 @@ attn_chunk(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUte
       mbar_wait_drain(drain_bar, 0);
     } else {
       // O_g += P_g V: P from TMEM, V as an MN-major operand.
-      constexpr uint32_t idesc = idesc_f16(BF16, BM, D, true);
+      constexpr uint32_t idesc = idesc_f16(BF16 && !INT8, BM, D, true);
       // V lies as boxes of `box` keys, [64-column block][key][128 bytes]
-      const int box_log2 = min(p.s.page_log2, 7), box = 1 << box_log2;
+      const int box_log2 = INT8 ? 7 : min(p.s.page_log2, 7), box = 1 << box_log2;
       const uint64_t dv = smem_desc_sw128(sbase + C::OFF_KV, box * 128, 1024);
       auto place_of = [&](int key, int blk) {
         return ((((key >> box_log2) * C::KBLK + blk) << box_log2) + (key & (box - 1))) * 128;
@@ -408,7 +556,7 @@ attn_chunk(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUte
           const int tv = tb + 2 * q + 1, sv = tv % C::STAGES;
           if (!(ok = kv_wait(tv))) break;
           const int j0 = (x.tile0 + q) * BN;
-          if (j0 + BN > x.end) {  // zero the values of keys past the unit's end
+          if (!INT8 && j0 + BN > x.end) {  // zero the values of keys past the unit's end
             for (int i = max(0, x.end - j0) * 8 + lane; i < BN * 8; i += 32)
               for (int c = 0; c < C::KBLK; ++c)
                 st_shared_v4(sbase + C::OFF_KV + sv * C::TILE + place_of(i >> 3, c) + (i & 7) * 16, 0, 0, 0, 0);
@@ -438,7 +586,7 @@ attn_chunk(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUte
     }
   } else {
     // Softmax warpgroups: warps 0-3 query tile A, 4-7 tile B; thread = query row = TMEM lane (see attn_tc_sm100.cu).
-    setmaxnreg_inc<kRegsSoftmax>();
+    setmaxnreg_inc<C::REGS_SOFTMAX>();
     const int g = warp >> 2, r_local = threadIdx.x & 127;
     const uint32_t lane_off = (uint32_t)((warp & 3) * 32) << 16;
     const uint32_t t_s = tmem + lane_off + (g ? C::T_S1 : C::T_S0);
@@ -446,11 +594,13 @@ attn_chunk(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUte
     const uint32_t t_o = tmem + lane_off + (g ? C::T_O1 : C::T_O0);
     uint8_t* stage = smem + C::OFF_OST + warp * C::OST_WARP;
     const int row_tok = r_local / p.group;  // this row's token within the query tile
-    int sc = 0, oc = 0;
+    int sc = 0, oc = 0, tiles = 0;
     bool ok = true;
     for (int nu = 0;; ++nu) {
       Unit x = next_unit(nu, ok);
       if (x.id < 0) break;
+      const int tb = tiles;  // the share's tiles before this unit
+      tiles += x.cnt;
       if (g == 1 && !x.has_b) continue;
       const int tile_tok = x.tok + g * p.tile_tokens;
       const int see = x.len - x.n + tile_tok + 1;  // causal: keys that the tile's first row sees
@@ -474,12 +624,24 @@ attn_chunk(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUte
         tc_fence_before();
         mbar_arrive(s_free(C::SHARED_S ? 0 : g));
         const int j0 = jb + j * BN;
+        const float* scl = nullptr;
+        if constexpr (INT8) {
+          if (!(ok = wait(sc_full(tb + j), ((tb + j) >> 2) & 1, kErrSoftmaxWait))) break;
+          scl = reinterpret_cast<const float*>(smem + C::OFF_SCALE) + ((tb + j) & 3) * 3 * BN;
+#pragma unroll
+          for (int c = 0; c < BN; c += 4) {
+            const float4 a = *reinterpret_cast<const float4*>(scl + c), b = *reinterpret_cast<const float4*>(scl + BN + c);
+            const float2 y = fma2(make_float2(s[c], s[c + 1]), make_float2(a.x, a.y), make_float2(b.x, b.y));
+            const float2 z = fma2(make_float2(s[c + 2], s[c + 3]), make_float2(a.z, a.w), make_float2(b.z, b.w));
+            s[c] = y.x, s[c + 1] = y.y, s[c + 2] = z.x, s[c + 3] = z.y;
+          }
+        }
         if (j0 + BN > lim_least) {
           const int left = lim - j0;
 #pragma unroll
           for (int c = 0; c < BN; ++c) s[c] = c < left ? s[c] : -CUDART_INF_F;
         }
-        const float m_new = row_max<BN>(s) * p.scale_log2;
+        const float m_new = INT8 ? row_max<BN>(s) : row_max<BN>(s) * p.scale_log2;
         float alpha = 1.f;
         bool need = false;
         if (j == 0) {
@@ -511,15 +673,20 @@ attn_chunk(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUte
         }
         const float sub = m_used == -CUDART_INF_F ? 0.f : m_used;
         uint32_t pk[32];
-        float psum = softmax64<BF16, 0>(s, p.scale_log2, sub, pk);
+        float psum = softmax64<BF16, INT8, 0>(s, p.scale_log2, sub, scl + 2 * BN, pk);
         tmem_st32(t_p, pk);
         bool next_test = false;
         if constexpr (!C::SHARED_S) next_test = j + 1 < cnt && mbar_test(s_full(g), sc & 1);
-        psum += softmax64<BF16, 64>(s, p.scale_log2, sub, pk);
+        psum += softmax64<BF16, INT8, 64>(s, p.scale_log2, sub, scl + 2 * BN + 64, pk);
         tmem_st32(t_p + 32, pk);
         tmem_wait_st();
         tc_fence_before();
         mbar_arrive(p_ready(g));
+        if constexpr (INT8) {
+          __syncwarp();
+          if (lane == 0) mbar_arrive(sc_empty(tb + j));
+          if (lane == 0 && !x.has_b) mbar_arrive(sc_empty(tb + j));  // in the absent tile's place
+        }
         if constexpr (!C::SHARED_S) s_ready = __all_sync(0xffffffffu, next_test);
         l = l * alpha + psum;
       }
@@ -640,33 +807,35 @@ __global__ void __launch_bounds__(BM) merge_chunk(const Params p, int grid) {
   dst[1] = make_uint4(out[4], out[5], out[6], out[7]);
 }
 
-std::atomic<bool> g_attr[2][2][64];
+std::atomic<bool> g_attr[2][2][2][64];
 
-template <int D, bool BF16>
+template <int D, bool BF16, bool INT8>
 cudaError_t launch(const PagedAttnArgs& a, int dev) {
-  using C = Cfg<D>;
+  using C = Cfg<D, INT8>;
+  auto kern = attn_chunk<D, BF16, INT8>;
   int ctas = 0;
   cudaError_t e = sm_count(dev, &ctas);
   if (e != cudaSuccess) return e;
-  std::atomic<bool>& attr = g_attr[D / 128][BF16][dev];
+  std::atomic<bool>& attr = g_attr[D / 128][BF16][INT8][dev];
   if (!attr.load(std::memory_order_acquire)) {
-    if ((e = cudaFuncSetAttribute(attn_chunk<D, BF16>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM)) != cudaSuccess)
+    if ((e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM)) != cudaSuccess)
       return e;
     attr.store(true, std::memory_order_release);
   }
   const int page = 1 << a.s.page_log2, box = std::min(page, BN), tile_tokens = BM / a.group;
-  CUtensorMap mq, mk, mv;
+  CUtensorMap mq, mk = {}, mv = {};
   // queries as (packed token, key head, query head of it, d), boxes of one key head's rows of a tile
   const Strides3 qs{a.q_token, a.q_head * a.group, a.q_head};
-  if (!make_paged_map(&mk, a.kc, a.s.num_pages, a.s.heads, page, D, a.kcs, 2, BF16, 64, box, 1, 1) ||
-      !make_paged_map(&mv, a.vc, a.s.num_pages, a.s.heads, page, D, a.vcs, 2, BF16, 64, box, C::KBLK, 1) ||
+  if ((!INT8 && !make_paged_map(&mk, a.kc, a.s.num_pages, a.s.heads, page, D, a.kcs, 2, BF16, 64, box, 1, 1)) ||
+      (!INT8 && !make_paged_map(&mv, a.vc, a.s.num_pages, a.s.heads, page, D, a.vcs, 2, BF16, 64, box, C::KBLK, 1)) ||
       !make_paged_map(&mq, a.q, a.s.total, a.s.heads, a.group, D, qs, 2, BF16, 64, a.group, 1, tile_tokens))
     return cudaErrorInvalidValue;
   const size_t ml_bytes = (size_t)ctas * 4 * BM * sizeof(float2);
   void* block = nullptr;
   if ((e = scratch_alloc(dev, ml_bytes + (size_t)ctas * 4 * BM * D * sizeof(float), a.stream, &block)) != cudaSuccess) return e;
   Params p{a.s, TokenBlocks{2 * tile_tokens, a.causal ? 1 : 0, a.s.heads}, a.group, tile_tokens, static_cast<uint16_t*>(a.o),
-           fabsf(a.scale) * 1.4426950408889634f, a.scale < 0.f ? 1 : 0,
+           (INT8 ? a.scale : fabsf(a.scale)) * 1.4426950408889634f, !INT8 && a.scale < 0.f ? 1 : 0,
+           static_cast<const int8_t*>(a.kc), static_cast<const int8_t*>(a.vc), a.ks, a.vs, a.kcs, a.vcs, a.kss, a.vss,
            reinterpret_cast<float4*>(static_cast<char*>(block) + ml_bytes), static_cast<float2*>(block)};
   cudaLaunchConfig_t cfg = {};
   cudaLaunchAttribute pdl[1];
@@ -676,9 +845,9 @@ cudaError_t launch(const PagedAttnArgs& a, int dev) {
   cfg.numAttrs = 1;
   cfg.stream = a.stream;
   cfg.gridDim = dim3((unsigned)ctas);
-  cfg.blockDim = dim3(kThreads);
+  cfg.blockDim = dim3(C::THREADS);
   cfg.dynamicSmemBytes = C::SMEM;
-  e = cudaLaunchKernelEx(&cfg, attn_chunk<D, BF16>, mq, mk, mv, p);
+  e = cudaLaunchKernelEx(&cfg, kern, mq, mk, mv, p);
   if (e == cudaSuccess) {
     note_launch();
     cfg.gridDim = dim3((unsigned)ctas, 2, D / kMergeCols);
@@ -695,8 +864,11 @@ cudaError_t launch(const PagedAttnArgs& a, int dev) {
 
 cudaError_t launch_paged_attn_chunk(const PagedAttnArgs& a, int dev) {
   using namespace chunk;
-  if (a.d == 64) return a.bf16 ? launch<64, true>(a, dev) : launch<64, false>(a, dev);
-  return a.bf16 ? launch<128, true>(a, dev) : launch<128, false>(a, dev);
+  if (a.d == 64)
+    return a.int8 ? (a.bf16 ? launch<64, true, true>(a, dev) : launch<64, false, true>(a, dev))
+                  : (a.bf16 ? launch<64, true, false>(a, dev) : launch<64, false, false>(a, dev));
+  return a.int8 ? (a.bf16 ? launch<128, true, true>(a, dev) : launch<128, false, true>(a, dev))
+                : (a.bf16 ? launch<128, true, false>(a, dev) : launch<128, false, false>(a, dev));
 }
 
 }  // namespace phantom

@@ -465,7 +465,7 @@ int phantom_attn_paged(const phantom_paged_cache* cache, const void* q, long lon
   // Query rows of one key head in one sequence, as expected: up to one 16-row block the rows kernel reads the keys once
   // and is bound by that; above, its blocks would each read them, and the chunk kernel takes up to 256 rows at a time.
   const long long new_tokens = max_new > 0 ? max_new : (total_new + cache->batch - 1) / cache->batch;
-  const bool few = new_tokens * a.group <= 16 || a.int8;
+  const bool few = new_tokens * a.group <= 16;
   const cudaError_t e = few ? launch_paged_attn_rows(a, dev.id, (int)std::min(new_tokens * a.group, 1LL << 30)) : launch_paged_attn_chunk(a, dev.id);
   if (e != cudaSuccess) return cuda_fail(name, e);
   g_last_error.clear();

@@ -198,6 +198,9 @@ __device__ __forceinline__ void tma_load_5d(uint32_t dst, const void* tmap, uint
       "l"(reinterpret_cast<uint64_t>(tmap)), "r"(c0), "r"(c1), "r"(c2), "r"(c3), "r"(c4), "r"(bar)
       : "memory");
 }
+// A value's scale, at least what paged_append writes (log2 and the reciprocal stay in range); a NaN stays one.
+__device__ __forceinline__ float least_scale(float x) { return x < 0x1p-100f ? 0x1p-100f : x; }
+
 // Two signed bytes of w (chosen by sel: result bytes [lo, 4, hi, 4], byte 4 = 0x64) as exact fp16 pairs; w already has its
 // sign bits flipped, so a byte u = b + 128 gives the fp16 number 1024 + u.
 template <uint32_t SEL>

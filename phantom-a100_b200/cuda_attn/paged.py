@@ -22,12 +22,13 @@ from __future__ import annotations
 
 import torch
 
+from . import _ext  # defined above this module's import in the package
+
 
 def paged_append(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, page_table: torch.Tensor,
                  kv_lens: torch.Tensor, cu_new: torch.Tensor, k_scale: torch.Tensor | None = None,
                  v_scale: torch.Tensor | None = None) -> None:
     """Write the new tokens' keys and values (tokens, heads, d) into the cache, quantised if it is int8."""
-    from . import _ext
     _ext().paged_append(k, v, k_cache, v_cache, page_table, kv_lens, cu_new, k_scale, v_scale)
 
 
@@ -37,7 +38,6 @@ def paged_read(k_cache: torch.Tensor, v_cache: torch.Tensor, page_table: torch.T
     """The keys and values (total, heads, d) that the cache holds of the last cu_new[b + 1] - cu_new[b] tokens of each
     sequence; all of them where that is kv_lens[b]. `total` is cu_new[-1], known to the caller. `dtype`: the cache's, or
     float16 or bfloat16 of an int8 cache (bfloat16 by default)."""
-    from . import _ext
     if dtype is None:
         dtype = torch.bfloat16 if k_cache.dtype == torch.int8 else k_cache.dtype
     if dtype not in (torch.float16, torch.bfloat16):
@@ -54,7 +54,6 @@ def paged_attn(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, pa
     kv_lens[b] - n + i + 1 tokens if causal, else all kv_lens[b]; one that sees none gets zeros. `scale` of the scores: 1 /
     sqrt(d) by default. `max_new`: the largest number of new tokens of a sequence, a hint that picks the kernel and changes
     nothing else (default: the average)."""
-    from . import _ext
     if scale is not None and not 0.0 < abs(scale) < float("inf"):
         raise RuntimeError(f"paged_attn: scale must be finite and not zero (got {scale})")
     return _ext().paged_attn(q, k_cache, v_cache, page_table, kv_lens, cu_new, k_scale, v_scale, causal, max_new,
