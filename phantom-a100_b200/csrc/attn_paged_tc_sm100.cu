@@ -51,12 +51,14 @@ struct Cfg {
   static constexpr int STAGES = D == 128 ? 4 : 8;  // ring slots, keys and values in turn
   static constexpr int OFF_Q = 0;
   static constexpr int OFF_KV = 2 * TILE;
-  static constexpr int OFF_OST = OFF_KV + STAGES * TILE;  // output staging: per softmax warp 32 rows of 64 bytes
-  static constexpr int OST_WARP = 32 * 64;
+  static constexpr int OFF_OST = OFF_KV + STAGES * TILE;  // output staging: per softmax warp 32 rows of OST_COLS columns
+  static constexpr int OST_COLS = INT8 ? 16 : 32, OST_WARP = 32 * 2 * OST_COLS;
   static constexpr int SCALES = INT8 ? 4 : 0;      // tiles' scales in flight: the keys', log2 of the values', 1 / these
   static constexpr int OFF_SCALE = OFF_OST + 8 * OST_WARP;
-  static constexpr int OFF_BAR = OFF_SCALE + SCALES * 3 * BN * 4;
-  static constexpr int NUM_BARS = 2 * STAGES + 7 * 2 + 3 + (INT8 ? 2 * SCALES + kUnitRing : 0);
+  static constexpr int OFF_RAW = OFF_SCALE + SCALES * 3 * BN * 4;  // 8-bit: bytes of the item after the one being converted
+  static constexpr int OFF_IDS = OFF_RAW + (INT8 ? BN * D : 0);    // 16-bit: page ids, 64 to each of two producers
+  static constexpr int OFF_BAR = OFF_IDS + (INT8 ? 0 : 2 * 64 * 4);
+  static constexpr int NUM_BARS = 2 * STAGES + 7 * 2 + 3 + kUnitRing + 2 * SCALES;
   static constexpr int OFF_MISC = (OFF_BAR + NUM_BARS * 8 + 15) / 16 * 16;  // TMEM base, abort flag, unit ring
   static constexpr int SMEM = OFF_MISC + 16 + 48 * kUnitRing + 1024;
   static_assert(SMEM <= 227 * 1024, "shared memory plan exceeds 227 KB");
@@ -133,8 +135,9 @@ __device__ __forceinline__ float row_max(const float (&s)[N]) {
 }
 
 // p = exp2(s * scale - sub) of 64 scores as packed 16-bit pairs; returns the sum of the unrounded values. Every fourth pair
-// by the FMA pipe's polynomial, as in attn_tc_sm100.cu, with an exact zero where its 2^-125 would count: bf16 holds it, and
-// an 8-bit cache's sum multiplies it with 1 / vs (`inv`, of the 64 keys).
+// by the FMA pipe's polynomial, as in attn_tc_sm100.cu; its least value is 2^-125, which is nothing beside a row's largest
+// p (at least 2^-8) unless it meets a value of 1e30, but not in an 8-bit cache's sum, which multiplies it with 1 / vs (`inv`,
+// of the 64 keys): an exact zero there.
 template <bool BF16, bool INT8, int OFF>
 __device__ __forceinline__ float softmax64(const float (&s)[BN], float scale_log2, float sub, const float* inv, uint32_t (&p)[32]) {
   const float2 sc = make_float2(scale_log2, scale_log2), nm = make_float2(-sub, -sub);
@@ -147,7 +150,7 @@ __device__ __forceinline__ float softmax64(const float (&s)[BN], float scale_log
     if ((0x09 >> (c & 7)) & 1) {
       const float2 arg = x;
       x = exp2_fma2(x);
-      if constexpr (BF16 || INT8) {
+      if constexpr (INT8) {
         x.x = arg.x < -125.f ? 0.f : x.x;
         x.y = arg.y < -125.f ? 0.f : x.y;
       }
@@ -189,11 +192,11 @@ attn_chunk(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUte
   auto o_done = [&](int g) { return bar0 + 8u * (B0 + 10 + g); };
   auto o_free = [&](int g) { return bar0 + 8u * (B0 + 12 + g); };
   const uint32_t q_free = bar0 + 8u * (B0 + 14), drain_bar = bar0 + 8u * (B0 + 15), drain_pv_bar = bar0 + 8u * (B0 + 16);
-  // 8-bit: the scales of tile j of the share are there, are done with; unit u's record is published
-  auto sc_full = [&](int j) { return bar0 + 8u * (B0 + 17 + j % 4); };
-  auto sc_empty = [&](int j) { return bar0 + 8u * (B0 + 21 + j % 4); };
-  auto rec_full = [&](int u) { return bar0 + 8u * (B0 + 25 + u % kUnitRing); };
-  static_assert(kUnitRing == 4);
+  // unit u's record is published (for the roles that work ahead of its queries)
+  auto rec_full = [&](int u) { return bar0 + 8u * (B0 + 17 + u % kUnitRing); };
+  // 8-bit: the scales of tile j of the share are there, are done with
+  auto sc_full = [&](int j) { return bar0 + 8u * (B0 + 17 + kUnitRing + j % 4); };
+  auto sc_empty = [&](int j) { return bar0 + 8u * (B0 + 21 + kUnitRing + j % 4); };
   uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(smem + C::OFF_MISC);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + C::OFF_MISC + 4);
   int4* ring = reinterpret_cast<int4*>(smem + C::OFF_MISC + 16);  // [kUnitRing][3]
@@ -207,18 +210,18 @@ attn_chunk(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUte
     }
     for (int g = 0; g < 2; ++g) {
       mbar_init(q_full(g), 1);
-      mbar_init(unit_read(g), INT8 ? 14 : 10);  // eight softmax warps, the two MMA warps, the converting warps
+      mbar_init(unit_read(g), INT8 ? 14 : 11);  // eight softmax warps, two MMA warps, the warps that bring the values
       mbar_init(s_full(g), 1);
       mbar_init(s_free(g), 128);
       mbar_init(p_ready(g), 128);
       mbar_init(o_done(g), 1);
       mbar_init(o_free(g), 128);
     }
+    for (int u = 0; u < kUnitRing; ++u) mbar_init(rec_full(u), 1);
     if constexpr (INT8)
       for (int j = 0; j < 4; ++j) {
         mbar_init(sc_full(j), 4);
         mbar_init(sc_empty(j), 8);
-        mbar_init(rec_full(j), 1);
       }
     mbar_init(q_free, 1);
     mbar_init(drain_bar, 1);
@@ -267,73 +270,126 @@ attn_chunk(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUte
     return x;
   };
 
+  // A role that works ahead: the record of unit u as soon as it is published (id -1 at the end).
+  auto take_unit = [&](int u, bool& ok) -> Unit {
+    Unit x;
+    x.id = -1;
+    if ((ok = wait(rec_full(u), (u / kUnitRing) & 1, kErrTmaWait))) {
+      x = record(u);
+      __syncwarp();
+      if (x.id >= 0 && lane == 0) mbar_arrive(unit_read(u));
+    }
+    return x;
+  };
+
   if (warp == TMA_WARP || warp == V_WARP) {
     setmaxnreg_dec<kRegsProducer>();
-    if (!INT8 || warp == TMA_WARP) {
-    // Producers: V_WARP copies the values, TMA_WARP the keys, and the units' records and queries. Each walks the CTA's
-    // share by itself. One elected lane of warp-uniform code issues the copies; their issue is what limits pages of 16
-    // tokens, hence two warps and, for the values, boxes of all columns (the tensor core takes V 16 keys at a time from
-    // anywhere, but K's 128 keys at one stride).
+    // TMA_WARP walks the CTA's share: each unit's record and queries, and (16-bit) its keys; V_WARP follows the records
+    // with the values. Page ids wait in shared memory. The copies' issue is what limits pages of 16 tokens, hence the
+    // two warps and, for the values, boxes of all columns (the tensor core takes V 16 keys at a time from anywhere, but K's
+    // 128 keys at one stride).
+    const int page_log2 = p.s.page_log2, page = 1 << page_log2, box = min(page, BN);
     const bool vals = warp == V_WARP;
-    if (elect_one()) {
-      if (!vals) tma_prefetch_desc(&tmQ);
-      if (!INT8) tma_prefetch_desc(vals ? &tmV : &tmK);
-    }
-    __syncwarp();
-    Walk<TokenBlocks> w;
-    w.start(p.s, p.blocks, blockIdx.x, gridDim.x);
-    const long long begin = w.cur;
-    const int page = 1 << p.s.page_log2, box = min(page, BN);
-    int t = vals, nu = 0, nq = 0;  // copies (keys even, values odd), units, phases of q_full begun
+    int t = vals;  // copies: keys even, values odd
     bool ok = true;
+    int* ids = reinterpret_cast<int*>(smem + C::OFF_IDS) + vals * 64;  // page i's id at i % 64
+    int ahead = 0, pages = 0, seq = 0, head = 0;                       // ids are there for pages below `ahead`
+    auto ids_more = [&]() {
+      ids[(ahead + lane) & 63] = ahead + lane < pages ? page_of(p.s, seq, ahead + lane) : 0;
+      ahead += 32;
+    };
+    auto begin_unit = [&](int b, int h, int tile0, int end) {
+      seq = b;
+      head = h;
+      pages = (end + page - 1) >> page_log2;
+      ahead = (tile0 * BN) >> page_log2 & ~31;
+      ids_more();
+      ids_more();
+      __syncwarp();
+    };
     auto copy_tile = [&](int j0, int end) {
       const int s = t % C::STAGES, round = t / C::STAGES;
       const int boxes = max(0, (min(j0 + BN, end) - j0 + box - 1) / box);  // pages of the tile that hold keys
-      int id = 0;
-      if (lane < boxes) id = page_of(p.s, w.b, (j0 >> p.s.page_log2) + lane);
+      const int first = j0 >> page_log2;
       if (round > 0 && !(ok = wait(kv_empty(s), (round - 1) & 1, kErrTmaWait))) return;
-      const uint32_t dst = sbase + C::OFF_KV + s * C::TILE;
-      if (elect_one()) mbar_arrive_expect_tx(kv_full(s), boxes * box * D * 2);
-      for (int pg = 0; pg < boxes; ++pg) {
-        const int from = __shfl_sync(0xffffffffu, id, pg);
-        if (elect_one()) {  // an id that is out of range reads as zeros
+      if (elect_one()) {
+        mbar_arrive_expect_tx(kv_full(s), boxes * box * D * 2);
+        uint32_t dst = sbase + C::OFF_KV + s * C::TILE;
+        const int place = j0 & (page - 1);
+        // (left as a loop: the code of all roles shares the instruction cache)
+#pragma unroll 1
+        for (int pg = 0; pg < boxes; ++pg) {
+          const int from = ids[(first + pg) & 63];  // one that is out of range reads as zeros
           if (vals) {
-            tma_load_5d(dst + pg * box * D * 2, &tmV, kv_full(s), 0, j0 & (page - 1), 0, w.h, from);
+            tma_load_5d(dst, &tmV, kv_full(s), 0, place, 0, head, from);
+            dst += box * D * 2;
           } else {
-#pragma unroll
-            for (int c = 0; c < C::KBLK; ++c)
-              tma_load_5d(dst + c * C::SUB + pg * box * 128, &tmK, kv_full(s), 0, j0 & (page - 1), c, w.h, from);
+            tma_load_5d(dst, &tmK, kv_full(s), 0, place, 0, head, from);
+            if constexpr (C::KBLK == 2) tma_load_5d(dst + C::SUB, &tmK, kv_full(s), 0, place, 1, head, from);
+            dst += box * 128;
           }
         }
       }
       __syncwarp();
+      // (a tile has at most 8 pages; those below ahead - 32, which the next ones take the place of, are done with)
+      if (first >= ahead - 32 && ahead < pages) ids_more();
+      __syncwarp();
       t += 2;
     };
-    while (ok && w.cur < w.end) {
-      const int cnt = w.count(), end = p.blocks.key_end(w.x, w.blk);
-      int i = 0;
-      if (!vals) {
-        if (!INT8) copy_tile(w.tile * BN, end);  // before the waits for the last units to be done with
-        i = 1;
-        if (ok && nu > 1) ok = wait(unit_read(nu), ((nu >> 1) - 1) & 1, kErrTmaWait);
-        if (!ok) break;
-        Unit x;
-        x.id = nu;
-        x.b = w.b;
-        x.h = w.h;
-        x.cnt = cnt;
-        x.tile0 = w.tile;
-        x.end = end;
-        x.tok = w.blk * p.blocks.per;
-        x.len = w.x.len, x.n = w.x.n, x.tok0 = w.x.tok0;
-        x.has_b = x.tok + p.tile_tokens < x.n;
-        x.slot = cnt == w.nt ? -1 : 2 * (int)blockIdx.x + (begin > w.cur - w.tile ? 0 : 1);
+    int nq = 0;  // phases of q_full begun
+    if (vals) {
+      if (!INT8) {
+        if (elect_one()) tma_prefetch_desc(&tmV);
+        __syncwarp();
+        for (int nu = 0;; ++nu) {
+          const Unit x = take_unit(nu, ok);
+          if (x.id < 0) break;
+          begin_unit(x.b, x.h, x.tile0, x.end);
+          for (int i = 0; ok && i < x.cnt; ++i) copy_tile((x.tile0 + i) * BN, x.end);
+          if (!ok) break;
+        }
+      }
+    } else {
+      if (elect_one()) {
+        tma_prefetch_desc(&tmQ);
+        if (!INT8) tma_prefetch_desc(&tmK);
+      }
+      __syncwarp();
+      Walk<TokenBlocks> w;
+      w.start(p.s, p.blocks, blockIdx.x, gridDim.x);
+      const long long begin = w.cur;
+      int nu = 0;
+      for (;; ++nu) {
+        if (nu > 1 && !(ok = wait(unit_read(nu), ((nu >> 1) - 1) & 1, kErrTmaWait))) break;
+        Unit x = {};
+        x.id = w.cur < w.end ? nu : -1;
+        if (x.id >= 0) {
+          x.b = w.b;
+          x.h = w.h;
+          x.cnt = w.count();
+          x.tile0 = w.tile;
+          x.end = p.blocks.key_end(w.x, w.blk);
+          x.tok = w.blk * p.blocks.per;
+          x.len = w.x.len, x.n = w.x.n, x.tok0 = w.x.tok0;
+          x.has_b = x.tok + p.tile_tokens < x.n;
+          x.slot = x.cnt == w.nt ? -1 : w.place(blockIdx.x, begin <= w.cur - w.tile);
+        }
         if (elect_one()) {
           publish(nu, x);
-          if (INT8) mbar_arrive(rec_full(nu));
+          mbar_arrive(rec_full(nu));
+          if (x.id < 0) mbar_arrive(q_full(nu));
         }
         __syncwarp();
-        if (nu > 0 && !(ok = wait(q_free, (nu - 1) & 1, kErrTmaWait))) break;
+        if (x.id < 0) {
+          ++nq;
+          break;
+        }
+        if (!INT8) {
+          begin_unit(x.b, x.h, x.tile0, x.end);
+          copy_tile(x.tile0 * BN, x.end);  // before the wait for the last unit's queries to be done with
+        }
+        if (ok && nu > 0) ok = wait(q_free, (nu - 1) & 1, kErrTmaWait);
+        if (!ok) break;
         if (elect_one()) {
           const int tiles = x.has_b ? 2 : 1;
           mbar_arrive_expect_tx(q_full(nu), tiles * C::KBLK * p.tile_tokens * p.group * 128);
@@ -343,143 +399,141 @@ attn_chunk(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUte
                           x.tok0 + x.tok + g * p.tile_tokens);
         }
         __syncwarp();
-        ++nu;
         ++nq;
-      }
-      for (; !INT8 && ok && i < cnt; ++i) copy_tile((w.tile + i) * BN, end);
-      w.advance(p.s, p.blocks);
-    }
-    if (!vals && ok) {
-      // the end of the units
-      if (nu > 1) ok = wait(unit_read(nu), ((nu >> 1) - 1) & 1, kErrTmaWait);
-      if (ok) {
-        Unit x = {};
-        x.id = -1;
-        if (elect_one()) {
-          publish(nu, x);
-          if (INT8) mbar_arrive(rec_full(nu));
-          mbar_arrive(q_full(nu));
-        }
-        __syncwarp();
-        ++nq;
+        for (int i = 1; !INT8 && ok && i < x.cnt; ++i) copy_tile((x.tile0 + i) * BN, x.end);
+        if (!ok) break;
+        w.advance(p.s, p.blocks);
       }
     }
     if (!ok) *abort_flag = 1;
     // every issued copy lands before this CTA's shared memory can be released
     for (int a = max(0, nq - 2); a < nq; ++a) mbar_wait_drain(q_full(a), (a >> 1) & 1);
     for (int i = max((int)vals, t - C::STAGES); !INT8 && i < t; i += 2) mbar_wait_drain(kv_full(i % C::STAGES), (i / C::STAGES) & 1);
-    }
   } else if (INT8 && warp >= CONV_WARP) {
     setmaxnreg_dec<72>();
-    // 8-bit pages to 16-bit tiles: keys of tile j, its values, keys of tile j + 1, ...; thread = 16-byte chunk of every
-    // 16 rows (16 rows lie in one page). The next item's bytes are on their way into the registers that the current one
-    // leaves. Rows past the unit's end become zeros, with scales of no effect.
-    constexpr int CHUNKS = D / 16, STEP = 128 / CHUNKS, N = BN / STEP;  // rows at a time; times
-    const int tid = threadIdx.x - 32 * CONV_WARP, chunk = tid % CHUNKS, row_in = tid / CHUNKS;
-    const int page_mask = (1 << p.s.page_log2) - 1;
-    int nu = 0, i = 0;
+    // 8-bit pages to 16-bit tiles: keys of tile j, its values, keys of tile j + 1, ... A thread has one 16-byte chunk of a
+    // row in every pass over 16 (d = 64: 32) rows; the next item's bytes are on their way into the place that the
+    // current one's leave. Eight lanes that store together have four chunks of a column block in two rows: swizzled, these
+    // meet no bank twice. Rows past the unit's end turn into whatever the page holds, numbers all (their weights are 0).
+    constexpr int STEP = D == 128 ? 16 : 32, N = BN / STEP;  // rows at a time; times
+    const int tid = threadIdx.x - 32 * CONV_WARP;
+    const int chunk = D == 128 ? (lane & 3) + 4 * ((lane >> 3) & 1) : lane & 3;
+    const int row_in = D == 128 ? ((lane >> 2) & 1) + 2 * (lane >> 4) + 4 * (warp & 3) : (lane >> 2) + 8 * (warp & 3);
+    const int page_log2 = p.s.page_log2, page_mask = (1 << page_log2) - 1;
+    // where this thread's chunk goes in pass 0, its halves by the row's swizzle (16 rows further on is 2 KB further)
+    const uint32_t at = (chunk >> 2) * C::SUB + row_in * 128, c0 = (chunk & 3) * 2, sw = row_in & 7;
+    const uint32_t at_lo = at + ((c0 ^ sw) << 4), at_hi = at + (((c0 + 1) ^ sw) << 4);
+    int nu = 0, i = 0, j0 = 0;
     bool ok = true;
-    // the place being read: a tile of a unit, and the ids of its 16-row pieces (lanes 0-7)
-    Unit x;
-    x.id = -1;
-    auto take_unit = [&](int u) {
-      if (!(ok = wait(rec_full(u), (u / kUnitRing) & 1, kErrTmaWait))) return -1;
-      x = record(u);
-      __syncwarp();
-      if (x.id >= 0 && lane == 0) mbar_arrive(unit_read(u));
-      return x.id;
-    };
-    int ids = -1, j0 = 0;
-    auto take_ids = [&]() {
+    Unit x = take_unit(0, ok);
+    // Byte offsets of the tile's 16-row pieces (a page has whole ones), a lane each; -1: no keys there that the unit sees.
+    long long k_off = -1, v_off = -1;
+    int id = -1;
+    const int8_t *k_base = nullptr, *v_base = nullptr;
+    auto begin_tile = [&]() {
       j0 = (x.tile0 + i) * BN;
-      ids = lane < 8 && j0 + lane * 16 < x.end ? page_of(p.s, x.b, (j0 + lane * 16) >> p.s.page_log2) : -1;
+      const int j = j0 + (lane & 7) * 16;
+      id = j < x.end ? page_of(p.s, x.b, j >> page_log2) : -1;
+      k_off = id < 0 ? -1 : id * p.kcs.page + (j & page_mask) * p.kcs.token;
+      v_off = id < 0 ? -1 : id * p.vcs.page + (j & page_mask) * p.vcs.token;
+      k_base = p.kc + x.h * p.kcs.head + (row_in & 15) * p.kcs.token + chunk * 16;
+      v_base = p.vc + x.h * p.vcs.head + (row_in & 15) * p.vcs.token + chunk * 16;
     };
-    uint4 raw[N];
-    auto load = [&](int n, bool vals) {
-      const int row = n * STEP + row_in;
-      const int id = __shfl_sync(0xffffffffu, ids, row >> 4);
-      const Strides3& st = vals ? p.vcs : p.kcs;
-      raw[n] = make_uint4(0, 0, 0, 0);
-      if (id >= 0 && j0 + row < x.end)
-        raw[n] = *reinterpret_cast<const uint4*>((vals ? p.vc : p.kc) + id * st.page + x.h * st.head +
-                                                 ((j0 + row) & page_mask) * st.token + chunk * 16);
+    // Pass n's 16 bytes of this thread lie in its own place of shared memory, filled one item ahead by its own asynchronous
+    // copies (a copy group to a pass, empty where there is nothing to copy), so the roles meet nowhere but at the ring.
+    const uint32_t raw = sbase + C::OFF_RAW + tid * 16;
+    auto load = [&](int n, const int8_t* base, long long off) {
+      const long long o = __shfl_sync(0xffffffffu, off, (n * STEP + row_in) >> 4);
+      if (o >= 0)
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(raw + n * 2048), "l"(base + o) : "memory");
+      asm volatile("cp.async.commit_group;" ::: "memory");
+    };
+    auto take = [&](int n, uint32_t (&in)[4]) {  // the oldest of the N groups in flight
+      asm volatile("cp.async.wait_group %0;" ::"n"(N - 1) : "memory");
+      asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(in[0]), "=r"(in[1]), "=r"(in[2]), "=r"(in[3]) : "r"(raw + n * 2048) : "memory");
     };
     float ks = 0.f, vs = 1.f;
     bool past = false;
     auto load_scales = [&]() {
-      const int id = __shfl_sync(0xffffffffu, ids, tid >> 4);
-      const bool there = id >= 0 && j0 + tid < x.end;
+      const int from = __shfl_sync(0xffffffffu, id, (tid >> 4) & 7);
       const int place = (j0 + tid) & page_mask;
-      ks = there ? p.ks[id * p.kss.page + x.h * p.kss.head + place] : 0.f;
-      vs = there ? p.vs[id * p.vss.page + x.h * p.vss.head + place] : 1.f;
-      past = j0 + tid >= x.end;
+      past = from < 0 || j0 + tid >= x.end;
+      ks = past ? 0.f : p.ks[from * p.kss.page + x.h * p.kss.head + place];
+      vs = past ? 1.f : p.vs[from * p.vss.page + x.h * p.vss.head + place];
     };
-    if (take_unit(0) >= 0) {
-      take_ids();
-#pragma unroll
-      for (int n = 0; n < N; ++n) load(n, false);
+    if (x.id >= 0) {
+      begin_tile();
+      for (int n = 0; n < N; ++n) load(n, k_base, k_off);
       load_scales();
     }
     for (int t = 0, j = 0; ok && x.id >= 0; ++j) {
       // -- the tile's scales
       if (j >= 4 && !(ok = wait(sc_empty(j), (j / 4 - 1) & 1, kErrTmaWait))) break;
       float* scl = reinterpret_cast<float*>(smem + C::OFF_SCALE) + (j & 3) * 3 * BN + tid;
-      scl[0] = ks * p.scale_log2;
       vs = least_scale(vs);
+      scl[0] = ks * p.scale_log2;
       scl[BN] = past ? 0.f : __log2f(vs);
       scl[2 * BN] = past ? 0.f : __fdividef(1.f, vs);
       __syncwarp();
       if (lane == 0) mbar_arrive(sc_full(j));
-      // -- keys, then values
-      for (int vals = 0; vals < 2; ++vals, ++t) {
-        const int s = t % C::STAGES, round = t / C::STAGES;
-        if (round > 0 && !(ok = wait(kv_empty(s), (round - 1) & 1, kErrTmaWait))) break;
-        const uint32_t dst = sbase + C::OFF_KV + s * C::TILE + (chunk >> 2) * C::SUB;
-        if (vals) {  // what comes next is the next tile
-          ++i;
-          if (i == x.cnt) {
-            i = 0;
-            ++nu;
-            take_unit(nu);
-          }
-          if (x.id >= 0) take_ids();
-        }
-        const bool more = !vals || x.id >= 0;
+      // -- keys; the values' bytes take their place
+      int s = t % C::STAGES;
+      if (t >= C::STAGES && !(ok = wait(kv_empty(s), (t / C::STAGES - 1) & 1, kErrTmaWait))) break;
+      uint32_t dst = sbase + C::OFF_KV + s * C::TILE;
+#pragma unroll 1
+      for (int n = 0; n < N; ++n) {  // (left as loops: the code of all roles shares the instruction cache)
+        uint32_t in[4], w[8];
+        take(n, in);
+        load(n, v_base, v_off);
 #pragma unroll
-        for (int n = 0; n < N; ++n) {
-          const int row = n * STEP + row_in;
-          const uint32_t in[4] = {raw[n].x, raw[n].y, raw[n].z, raw[n].w};
-          uint32_t w[8];
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            if (BF16 && !vals) {
-              w[2 * e] = bytes_bf16<0x4140>(in[e]);
-              w[2 * e + 1] = bytes_bf16<0x4342>(in[e]);
-            } else {
-              const uint32_t u = in[e] ^ 0x80808080u;
-              w[2 * e] = bytes_f16<0x4140>(u);
-              w[2 * e + 1] = bytes_f16<0x4342>(u);
-            }
-          }
-          if (more) load(n, !vals);
-          // (chunks of the two column blocks write their halves in opposite order: no bank conflicts)
-          const uint32_t at = dst + row * 128;
-          const int c0 = (chunk & 3) * 2, flip = (chunk >> 2) & 1;
-          const uint32_t lo = at + ((c0 ^ (row & 7)) << 4), hi = at + (((c0 + 1) ^ (row & 7)) << 4);
-          if (flip) {
-            st_shared_v4(hi, w[4], w[5], w[6], w[7]);
-            st_shared_v4(lo, w[0], w[1], w[2], w[3]);
+        for (int e = 0; e < 4; ++e) {
+          if constexpr (BF16) {
+            w[2 * e] = bytes_bf16<0x4140>(in[e]);
+            w[2 * e + 1] = bytes_bf16<0x4342>(in[e]);
           } else {
-            st_shared_v4(lo, w[0], w[1], w[2], w[3]);
-            st_shared_v4(hi, w[4], w[5], w[6], w[7]);
+            in[e] ^= 0x80808080u;
+            w[2 * e] = bytes_f16<0x4140>(in[e]);
+            w[2 * e + 1] = bytes_f16<0x4342>(in[e]);
           }
         }
-        if (vals && x.id >= 0) load_scales();
-        fence_proxy_async_smem();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(kv_full(s));
+        st_shared_v4(dst + at_lo + n * STEP * 128, w[0], w[1], w[2], w[3]);
+        st_shared_v4(dst + at_hi + n * STEP * 128, w[4], w[5], w[6], w[7]);
       }
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(kv_full(s));
+      ++t;
+      // -- the next tile; values; its keys' bytes take their place
+      if (++i == x.cnt) {
+        i = 0;
+        x = take_unit(++nu, ok);
+      }
+      k_off = -1;
+      if (x.id >= 0) begin_tile();
+      s = t % C::STAGES;
+      if (!ok || (t >= C::STAGES && !(ok = wait(kv_empty(s), (t / C::STAGES - 1) & 1, kErrTmaWait)))) break;
+      dst = sbase + C::OFF_KV + s * C::TILE;
+#pragma unroll 1
+      for (int n = 0; n < N; ++n) {
+        uint32_t in[4], w[8];
+        take(n, in);
+        load(n, k_base, k_off);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          in[e] ^= 0x80808080u;
+          w[2 * e] = bytes_f16<0x4140>(in[e]);
+          w[2 * e + 1] = bytes_f16<0x4342>(in[e]);
+        }
+        st_shared_v4(dst + at_lo + n * STEP * 128, w[0], w[1], w[2], w[3]);
+        st_shared_v4(dst + at_hi + n * STEP * 128, w[4], w[5], w[6], w[7]);
+      }
+      if (x.id >= 0) load_scales();
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(kv_full(s));
+      ++t;
     }
+    asm volatile("cp.async.wait_all;" ::: "memory");
   } else if (warp == MMA_WARP || warp == PV_WARP) {
     setmaxnreg_dec<kRegsProducer>();
     const uint64_t dq = smem_desc_sw128(sbase + C::OFF_Q, 16, 1024);
@@ -539,12 +593,15 @@ attn_chunk(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUte
       auto place_of = [&](int key, int blk) {
         return ((((key >> box_log2) * C::KBLK + blk) << box_log2) + (key & (box - 1))) * 128;
       };
+      uint32_t v_off[BN / 16];
+#pragma unroll
+      for (int kk = 0; kk < BN / 16; ++kk) v_off[kk] = place_of(kk * 16, 0) >> 4;
       auto issue = [&](int g, int stage, bool acc) {
         const uint32_t b_off = (uint32_t)(stage * C::TILE) >> 4;
         const uint32_t d_t = tmem + (g ? C::T_O1 : C::T_O0), p_t = tmem + (g ? C::T_P1 : C::T_P0);
 #pragma unroll
         for (int kk = 0; kk < BN / 16; ++kk)
-          mma_ts(d_t, p_t + kk * 8, dv + (b_off + (place_of(kk * 16, 0) >> 4)), idesc, (acc || kk > 0) ? 1u : 0u);
+          mma_ts(d_t, p_t + kk * 8, dv + (b_off + v_off[kk]), idesc, (acc || kk > 0) ? 1u : 0u);
       };
       int tb = 0, nu = 0;
       int pc[2] = {0, 0}, uc[2] = {0, 0};
@@ -657,7 +714,7 @@ attn_chunk(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUte
           tc_fence_after();
           if (__any_sync(0xffffffffu, need)) {
             const float2 a2 = make_float2(alpha, alpha);
-#pragma unroll
+#pragma unroll 1
             for (int c = 0; c < D / 32; ++c) {
               uint32_t rr[32];
               tmem_ld32_wait(t_o + c * 32, rr);
@@ -696,38 +753,48 @@ attn_chunk(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUte
       tc_fence_after();
       x = record(nu);  // read again: fewer registers live across the tile loop
       if (x.slot < 0) {
-        // O / l, 32 columns at a time through shared memory (16-byte chunk k of row r at k ^ (r / 2 % 4): conflict-free)
-        // so that four lanes write 64 consecutive bytes of a row
+        // O / l, some columns at a time through shared memory (16-byte chunks swizzled by the row: conflict-free) so that a
+        // few lanes write consecutive bytes of a row
+        constexpr int COLS = C::OST_COLS, NCH = COLS / 8;  // chunks of a row
         const float inv_l = m_used == -CUDART_INF_F ? 0.f : 1.f / l;
         const int rows = min(p.tile_tokens, x.n - (x.tok + g * p.tile_tokens)) * p.group;
         const long long at = (long long)(x.tok0 + x.tok + g * p.tile_tokens) * p.s.heads;
+        auto place_of = [](int r, int k) { return r * 2 * COLS + ((k ^ (NCH == 4 ? (r >> 1) & 3 : (r >> 2) & 1)) << 4); };
+#pragma unroll 1
+        for (int cb = 0; cb < D / COLS; ++cb) {
+          uint32_t w[COLS / 2];
+          if constexpr (COLS == 32) {
+            uint32_t rr[32];
+            tmem_ld32_wait(t_o + cb * 32, rr);
 #pragma unroll
-        for (int cb = 0; cb < D / 32; ++cb) {
-          uint32_t rr[32], w[16];
-          tmem_ld32_wait(t_o + cb * 32, rr);
+            for (int i = 0; i < 16; ++i)
+              w[i] = pack2<BF16>(__uint_as_float(rr[2 * i]) * inv_l, __uint_as_float(rr[2 * i + 1]) * inv_l);
+          } else {
+            uint32_t rr[16];
+            tmem_ld16_wait(t_o + cb * 16, rr);
 #pragma unroll
-          for (int i = 0; i < 16; ++i)
-            w[i] = pack2<BF16>(__uint_as_float(rr[2 * i]) * inv_l, __uint_as_float(rr[2 * i + 1]) * inv_l);
+            for (int i = 0; i < 8; ++i)
+              w[i] = pack2<BF16>(__uint_as_float(rr[2 * i]) * inv_l, __uint_as_float(rr[2 * i + 1]) * inv_l);
+          }
           __syncwarp();
 #pragma unroll
-          for (int k = 0; k < 4; ++k)
-            *reinterpret_cast<uint4*>(stage + lane * 64 + ((k ^ ((lane >> 1) & 3)) << 4)) =
-                make_uint4(w[4 * k], w[4 * k + 1], w[4 * k + 2], w[4 * k + 3]);
+          for (int k = 0; k < NCH; ++k)
+            *reinterpret_cast<uint4*>(stage + place_of(lane, k)) = make_uint4(w[4 * k], w[4 * k + 1], w[4 * k + 2], w[4 * k + 3]);
           __syncwarp();
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const int r = i * 8 + (lane >> 2), k = lane & 3, row = (warp & 3) * 32 + r;
+          for (int i = 0; i < NCH; ++i) {
+            const int r = (i * 32 + lane) / NCH, k = lane % NCH, row = (warp & 3) * 32 + r;
             if (row < rows) {
-              const uint4 v = *reinterpret_cast<const uint4*>(stage + r * 64 + ((k ^ ((r >> 1) & 3)) << 4));
+              const uint4 v = *reinterpret_cast<const uint4*>(stage + place_of(r, k));
               const int tok = row / p.group;
               *reinterpret_cast<uint4*>(p.o + ((at + (long long)tok * p.s.heads + x.h) * p.group + (row - tok * p.group)) * D +
-                                        cb * 32 + k * 8) = v;
+                                        cb * COLS + k * 8) = v;
             }
           }
         }
       } else {
         float4* po = p.part + ((long long)x.slot * 2 + g) * (D / 4) * BM + r_local;
-#pragma unroll
+#pragma unroll 1
         for (int c = 0; c < D / 32; ++c) {
           uint32_t rr[32];
           tmem_ld32_wait(t_o + c * 32, rr);
