@@ -136,39 +136,49 @@ __device__ __forceinline__ float row_max(const float (&s)[N]) {
 
 // p = exp2(s * scale - sub) of 64 scores as packed 16-bit pairs; returns the sum of the unrounded values. Every fourth pair
 // by the FMA pipe's polynomial, as in attn_tc_sm100.cu; its least value is 2^-125, which is nothing beside a row's largest
-// p (at least 2^-8) unless it meets a value of 1e30, but not in an 8-bit cache's sum, which multiplies it with 1 / vs (`inv`,
-// of the 64 keys): an exact zero there.
-template <bool BF16, bool INT8, int OFF>
-__device__ __forceinline__ float softmax64(const float (&s)[BN], float scale_log2, float sub, const float* inv, uint32_t (&p)[32]) {
+// p (at least 2^-8) unless it meets a value of 1e30.
+template <bool BF16, int OFF>
+__device__ __forceinline__ float softmax64(const float (&s)[BN], float scale_log2, float sub, uint32_t (&p)[32]) {
   const float2 sc = make_float2(scale_log2, scale_log2), nm = make_float2(-sub, -sub);
   float2 acc[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
-  float4 iv;
 #pragma unroll
   for (int c = 0; c < 32; ++c) {
-    float2 x = make_float2(s[OFF + 2 * c], s[OFF + 2 * c + 1]);
-    x = INT8 ? add2(x, nm) : fma2(x, sc, nm);
+    float2 x = fma2(make_float2(s[OFF + 2 * c], s[OFF + 2 * c + 1]), sc, nm);
     if ((0x09 >> (c & 7)) & 1) {
-      const float2 arg = x;
       x = exp2_fma2(x);
-      if constexpr (INT8) {
-        x.x = arg.x < -125.f ? 0.f : x.x;
-        x.y = arg.y < -125.f ? 0.f : x.y;
-      }
     } else {
       x.x = ex2(x.x);
       x.y = ex2(x.y);
     }
-    if constexpr (INT8) {
-      if (c % 2 == 0) iv = *reinterpret_cast<const float4*>(inv + 2 * c);
-      acc[c & 1] = fma2(x, c % 2 == 0 ? make_float2(iv.x, iv.y) : make_float2(iv.z, iv.w), acc[c & 1]);
-    } else {
-      acc[c & 1] = add2(acc[c & 1], x);
-    }
-    p[c] = pack2<BF16 && !INT8>(x.x, x.y);
+    acc[c & 1] = add2(acc[c & 1], x);
+    p[c] = pack2<BF16>(x.x, x.y);
   }
   const float2 t = add2(acc[0], acc[1]);
   return t.x + t.y;
 }
+
+// The softmax of an 8-bit cache's tile. Every column has three numbers of its own (the key's scale, log2 of the value's,
+// its reciprocal); with a thread to a row, each thread reads all 3 x 128 of them from shared memory, and that, 3000 cycles
+// of its bandwidth for two query tiles, was what bound the kernel. So a thread takes 32 columns of four rows: lane 4 g + t
+// has columns 8 i + 2 t, + 1 of rows g, g + 8, g + 16, g + 24 of its warp's 32.
+struct Rows4 {
+  float m[4];   // reference maximum
+  float2 l[4];  // this lane's share of the sum
+  __device__ __forceinline__ void start() {
+#pragma unroll
+    for (int k = 0; k < 4; ++k) m[k] = -CUDART_INF_F, l[k] = make_float2(0.f, 0.f);
+  }
+  // Of the row that is this lane's number.
+  __device__ __forceinline__ static float of_lane(const float (&x)[4], int lane) {
+    float y = 0.f;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const float z = __shfl_sync(0xffffffffu, x[k], (lane & 7) * 4);
+      y = (lane >> 3) == k ? z : y;
+    }
+    return y;
+  }
+};
 
 template <int D, bool BF16, bool INT8>
 __global__ void __launch_bounds__(Cfg<D, INT8>::THREADS, 1)
@@ -469,11 +479,11 @@ attn_chunk(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUte
     for (int t = 0, j = 0; ok && x.id >= 0; ++j) {
       // -- the tile's scales
       if (j >= 4 && !(ok = wait(sc_empty(j), (j / 4 - 1) & 1, kErrTmaWait))) break;
-      float* scl = reinterpret_cast<float*>(smem + C::OFF_SCALE) + (j & 3) * 3 * BN + tid;
+      float* scl = reinterpret_cast<float*>(smem + C::OFF_SCALE) + (j & 3) * 3 * BN;
       vs = least_scale(vs);
-      scl[0] = ks * p.scale_log2;
-      scl[BN] = past ? 0.f : __log2f(vs);
-      scl[2 * BN] = past ? 0.f : __fdividef(1.f, vs);
+      scl[(tid & ~1) * 2 + (tid & 1)] = ks * p.scale_log2;  // of a pair of keys: two of these, then two of those
+      scl[(tid & ~1) * 2 + (tid & 1) + 2] = past ? 0.f : __log2f(vs);
+      scl[2 * BN + tid] = past ? 0.f : __fdividef(1.f, vs);
       __syncwarp();
       if (lane == 0) mbar_arrive(sc_full(j));
       // -- keys; the values' bytes take their place
@@ -651,6 +661,22 @@ attn_chunk(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUte
     const uint32_t t_o = tmem + lane_off + (g ? C::T_O1 : C::T_O0);
     uint8_t* stage = smem + C::OFF_OST + warp * C::OST_WARP;
     const int row_tok = r_local / p.group;  // this row's token within the query tile
+    // multiplies this lane's row of O
+    auto rescale_o = [&](float alpha) {
+      const float2 a2 = make_float2(alpha, alpha);
+#pragma unroll 1
+      for (int c = 0; c < D / 32; ++c) {
+        uint32_t rr[32];
+        tmem_ld32_wait(t_o + c * 32, rr);
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          const float2 y = mul2(make_float2(__uint_as_float(rr[2 * i]), __uint_as_float(rr[2 * i + 1])), a2);
+          rr[2 * i] = __float_as_uint(y.x);
+          rr[2 * i + 1] = __float_as_uint(y.y);
+        }
+        tmem_st32(t_o + c * 32, rr);
+      }
+    };
     int sc = 0, oc = 0, tiles = 0;
     bool ok = true;
     for (int nu = 0;; ++nu) {
@@ -666,39 +692,110 @@ attn_chunk(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUte
       const int lim_least = causal ? min(x.len, see) : x.len;
       const int cnt = x.cnt, jb = x.tile0 * BN;
       float m_used = -CUDART_INF_F, l = 0.f;
+      Rows4 r4;
+      if constexpr (INT8) r4.start();
       bool s_ready = false;
       for (int j = 0; j < cnt; ++j) {
         if (!s_ready && !(ok = wait(s_full(g), sc & 1, kErrSoftmaxWait))) break;
         ++sc;
         tc_fence_after();
+        const int j0 = jb + j * BN;
         float s[BN];
         {
           uint32_t r[BN];
-          tmem_ld128_wait(t_s, r);
+          if constexpr (INT8) tmem_ld_rows4_wait(t_s, r);
+          else tmem_ld128_wait(t_s, r);
 #pragma unroll
           for (int i = 0; i < BN; ++i) s[i] = __uint_as_float(r[i]);
         }
         tc_fence_before();
         mbar_arrive(s_free(C::SHARED_S ? 0 : g));
-        const int j0 = jb + j * BN;
-        const float* scl = nullptr;
         if constexpr (INT8) {
+          // (s_full of this tile: the scales are there, since they were written before the keys)
+          const float* scl = reinterpret_cast<const float*>(smem + C::OFF_SCALE) + ((tb + j) & 3) * 3 * BN + 4 * (lane & 3);
           if (!(ok = wait(sc_full(tb + j), ((tb + j) >> 2) & 1, kErrSoftmaxWait))) break;
-          scl = reinterpret_cast<const float*>(smem + C::OFF_SCALE) + ((tb + j) & 3) * 3 * BN;
 #pragma unroll
-          for (int c = 0; c < BN; c += 4) {
-            const float4 a = *reinterpret_cast<const float4*>(scl + c), b = *reinterpret_cast<const float4*>(scl + BN + c);
-            const float2 y = fma2(make_float2(s[c], s[c + 1]), make_float2(a.x, a.y), make_float2(b.x, b.y));
-            const float2 z = fma2(make_float2(s[c + 2], s[c + 3]), make_float2(a.z, a.w), make_float2(b.z, b.w));
-            s[c] = y.x, s[c + 1] = y.y, s[c + 2] = z.x, s[c + 3] = z.y;
+          for (int i = 0; i < 16; ++i) {
+            const float4 a = *reinterpret_cast<const float4*>(scl + 16 * i);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              const int e = 64 * (k >> 1) + 4 * i + 2 * (k & 1);
+              const float2 y = fma2(make_float2(s[e], s[e + 1]), make_float2(a.x, a.y), make_float2(a.z, a.w));
+              s[e] = y.x, s[e + 1] = y.y;
+            }
           }
+          if (j0 + BN > lim_least) {
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              const int row = (warp & 3) * 32 + 8 * k + (lane >> 2);
+              const int left = (causal ? min(x.len, see + row / p.group) : x.len) - j0 - 2 * (lane & 3);
+#pragma unroll
+              for (int i = 0; i < 16; ++i) {
+                const int e = 64 * (k >> 1) + 4 * i + 2 * (k & 1);
+                s[e] = 8 * i < left ? s[e] : -CUDART_INF_F;
+                s[e + 1] = 8 * i + 1 < left ? s[e + 1] : -CUDART_INF_F;
+              }
+            }
+          }
+          float alpha[4], sub[4];
+          bool need = false;
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            const int o = 64 * (k >> 1) + 2 * (k & 1);
+            float y = fmaxf(s[o], s[o + 1]);
+#pragma unroll
+            for (int i = 1; i < 16; ++i) y = max3(y, s[o + 4 * i], s[o + 4 * i + 1]);
+            y = fmaxf(y, __shfl_xor_sync(0xffffffffu, y, 1));
+            y = fmaxf(y, __shfl_xor_sync(0xffffffffu, y, 2));
+            alpha[k] = 1.f;
+            if (j == 0) {
+              r4.m[k] = y;
+            } else if (y > r4.m[k] + kRescaleThreshold) {
+              need = true;
+              alpha[k] = ex2(r4.m[k] - y);
+              r4.m[k] = y;
+              r4.l[k] = mul2(r4.l[k], make_float2(alpha[k], alpha[k]));
+            }
+            sub[k] = r4.m[k] == -CUDART_INF_F ? 0.f : r4.m[k];
+          }
+          if (j > 0) {
+            if (!(ok = wait(o_done(g), oc & 1, kErrSoftmaxWait))) break;
+            ++oc;
+            tc_fence_after();
+            if (__any_sync(0xffffffffu, need)) rescale_o(Rows4::of_lane(alpha, lane));
+          }
+          uint32_t pk[2][32];
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            const float2 inv = *reinterpret_cast<const float2*>(scl - 2 * (lane & 3) + 2 * BN + 8 * i);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              // (all by ex2: the polynomial's least value, 2^-125, would count in a sum that multiplies it with 1 / vs)
+              const int e = 64 * (k >> 1) + 4 * i + 2 * (k & 1);
+              const float2 x = make_float2(ex2(s[e] - sub[k]), ex2(s[e + 1] - sub[k]));
+              r4.l[k] = fma2(x, inv, r4.l[k]);
+              pk[k >> 1][2 * i + (k & 1)] = pack2<false>(x.x, x.y);
+            }
+          }
+          tmem_st_16x128b_x16(t_p, pk[0]);
+          tmem_st_16x128b_x16(t_p + (16u << 16), pk[1]);
+          bool next_test = false;
+          if constexpr (!C::SHARED_S) next_test = j + 1 < cnt && mbar_test(s_full(g), sc & 1);
+          tmem_wait_st();
+          tc_fence_before();
+          mbar_arrive(p_ready(g));
+          __syncwarp();
+          if (lane == 0) mbar_arrive(sc_empty(tb + j));
+          if (lane == 0 && !x.has_b) mbar_arrive(sc_empty(tb + j));  // in the absent tile's place
+          if constexpr (!C::SHARED_S) s_ready = __all_sync(0xffffffffu, next_test);
+          continue;
         }
         if (j0 + BN > lim_least) {
           const int left = lim - j0;
 #pragma unroll
           for (int c = 0; c < BN; ++c) s[c] = c < left ? s[c] : -CUDART_INF_F;
         }
-        const float m_new = INT8 ? row_max<BN>(s) : row_max<BN>(s) * p.scale_log2;
+        const float m_new = row_max<BN>(s) * p.scale_log2;
         float alpha = 1.f;
         bool need = false;
         if (j == 0) {
@@ -712,38 +809,19 @@ attn_chunk(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUte
           if (!(ok = wait(o_done(g), oc & 1, kErrSoftmaxWait))) break;
           ++oc;
           tc_fence_after();
-          if (__any_sync(0xffffffffu, need)) {
-            const float2 a2 = make_float2(alpha, alpha);
-#pragma unroll 1
-            for (int c = 0; c < D / 32; ++c) {
-              uint32_t rr[32];
-              tmem_ld32_wait(t_o + c * 32, rr);
-#pragma unroll
-              for (int i = 0; i < 16; ++i) {
-                const float2 y = mul2(make_float2(__uint_as_float(rr[2 * i]), __uint_as_float(rr[2 * i + 1])), a2);
-                rr[2 * i] = __float_as_uint(y.x);
-                rr[2 * i + 1] = __float_as_uint(y.y);
-              }
-              tmem_st32(t_o + c * 32, rr);
-            }
-          }
+          if (__any_sync(0xffffffffu, need)) rescale_o(alpha);
         }
         const float sub = m_used == -CUDART_INF_F ? 0.f : m_used;
         uint32_t pk[32];
-        float psum = softmax64<BF16, INT8, 0>(s, p.scale_log2, sub, scl + 2 * BN, pk);
+        float psum = softmax64<BF16, 0>(s, p.scale_log2, sub, pk);
         tmem_st32(t_p, pk);
         bool next_test = false;
         if constexpr (!C::SHARED_S) next_test = j + 1 < cnt && mbar_test(s_full(g), sc & 1);
-        psum += softmax64<BF16, INT8, 64>(s, p.scale_log2, sub, scl + 2 * BN + 64, pk);
+        psum += softmax64<BF16, 64>(s, p.scale_log2, sub, pk);
         tmem_st32(t_p + 32, pk);
         tmem_wait_st();
         tc_fence_before();
         mbar_arrive(p_ready(g));
-        if constexpr (INT8) {
-          __syncwarp();
-          if (lane == 0) mbar_arrive(sc_empty(tb + j));
-          if (lane == 0 && !x.has_b) mbar_arrive(sc_empty(tb + j));  // in the absent tile's place
-        }
         if constexpr (!C::SHARED_S) s_ready = __all_sync(0xffffffffu, next_test);
         l = l * alpha + psum;
       }
@@ -751,6 +829,17 @@ attn_chunk(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUte
       if (!(ok = wait(o_done(g), oc & 1, kErrEpilogueWait))) break;
       ++oc;
       tc_fence_after();
+      if constexpr (INT8) {
+        float sum[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          sum[k] = r4.l[k].x + r4.l[k].y;
+          sum[k] += __shfl_xor_sync(0xffffffffu, sum[k], 1);
+          sum[k] += __shfl_xor_sync(0xffffffffu, sum[k], 2);
+        }
+        m_used = Rows4::of_lane(r4.m, lane);
+        l = Rows4::of_lane(sum, lane);
+      }
       x = record(nu);  // read again: fewer registers live across the tile loop
       if (x.slot < 0) {
         // O / l, some columns at a time through shared memory (16-byte chunks swizzled by the row: conflict-free) so that a

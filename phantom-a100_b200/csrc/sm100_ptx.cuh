@@ -229,6 +229,17 @@ __device__ __forceinline__ void tmem_ld128_wait(uint32_t taddr, uint32_t (&r)[12
       : "r"(taddr), "r"(taddr + 32), "r"(taddr + 64), "r"(taddr + 96)
       : "memory");
 }
+// 32 lanes x 128 columns as two 16x256b.x16 loads and one wait: thread 4 g + t holds, in r[64 h + 4 i ...], lane 16 h + g,
+// columns 8 i + 2 t and + 1, then lane 16 h + g + 8, the same columns.
+__device__ __forceinline__ void tmem_ld_rows4_wait(uint32_t taddr, uint32_t (&r)[128]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.16x256b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32,%33,%34,%35,%36,%37,%38,%39,%40,%41,%42,%43,%44,%45,%46,%47,%48,%49,%50,%51,%52,%53,%54,%55,%56,%57,%58,%59,%60,%61,%62,%63}, [%128];\n\t"
+      "tcgen05.ld.sync.aligned.16x256b.x16.b32 {%64,%65,%66,%67,%68,%69,%70,%71,%72,%73,%74,%75,%76,%77,%78,%79,%80,%81,%82,%83,%84,%85,%86,%87,%88,%89,%90,%91,%92,%93,%94,%95,%96,%97,%98,%99,%100,%101,%102,%103,%104,%105,%106,%107,%108,%109,%110,%111,%112,%113,%114,%115,%116,%117,%118,%119,%120,%121,%122,%123,%124,%125,%126,%127}, [%129];\n\t"
+      "tcgen05.wait::ld.sync.aligned;"
+      : PHANTOM_R8(0), PHANTOM_R8(8), PHANTOM_R8(16), PHANTOM_R8(24), PHANTOM_R8(32), PHANTOM_R8(40), PHANTOM_R8(48), PHANTOM_R8(56), PHANTOM_R8(64), PHANTOM_R8(72), PHANTOM_R8(80), PHANTOM_R8(88), PHANTOM_R8(96), PHANTOM_R8(104), PHANTOM_R8(112), PHANTOM_R8(120)
+      : "r"(taddr), "r"(taddr + (16u << 16))
+      : "memory");
+}
 #undef PHANTOM_R8
 
 #define PHANTOM_S8(i) "r"(r[i]), "r"(r[i + 1]), "r"(r[i + 2]), "r"(r[i + 3]), \
@@ -249,6 +260,13 @@ __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16
       "{%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(taddr),
       PHANTOM_S8(0), PHANTOM_S8(8)
       : "memory");
+}
+// 16 lanes x 64 columns as 16x128b.x16: thread 4 g + t gives lane g, column 4 i + t in r[2 i], lane g + 8 in r[2 i + 1] (no
+// wait).
+__device__ __forceinline__ void tmem_st_16x128b_x16(uint32_t taddr, const uint32_t (&r)[32]) {
+  asm volatile("tcgen05.st.sync.aligned.16x128b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};" ::"r"(taddr),
+               PHANTOM_S8(0), PHANTOM_S8(8), PHANTOM_S8(16), PHANTOM_S8(24)
+               : "memory");
 }
 #undef PHANTOM_S8
 
