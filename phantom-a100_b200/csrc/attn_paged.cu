@@ -72,7 +72,8 @@ struct Cfg {
   static constexpr int Q_ROW = 2 * D + 16;                // padded: lanes of 8 rows and 4 words read without conflicts
   static constexpr int OFF_Q = OFF_ML + WARPS * BR * 8;
   static constexpr int OFF_SCALE = OFF_Q + kUnitRing * BR * Q_ROW;
-  static constexpr int OFF_UNIT = OFF_SCALE + (INT8 ? SLOTS * 2 * BN * 4 : 0);
+  static constexpr int OFF_IDS = OFF_SCALE + (INT8 ? SLOTS * 2 * BN * 4 : 0);  // page ids, 64 to each producer
+  static constexpr int OFF_UNIT = OFF_IDS + PRODUCERS * 64 * 4;
   static constexpr int OFF_BAR = OFF_UNIT + kUnitRing * 48;
   static constexpr int OFF_FLAG = OFF_BAR + (2 * SLOTS + 2 * kUnitRing + 2) * 8;
   static constexpr int SMEM = OFF_FLAG + 16 + 1024;       // + slack to align the base
@@ -215,9 +216,8 @@ attn_rows(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUten
     const int role = warp - PRODUCER;
     if (role >= C::PRODUCERS) return;
     // Producers: of the keys (and of the units' records and queries), of the values, and of an 8-bit cache's scales of
-    // each, a copy to a page. Each walks the CTA's share by itself. One elected lane of warp-uniform code issues the
-    // copies: that issue is what limits pages of 16 tokens, hence a warp for each kind. Page ids are held a lane each, 32
-    // pages ahead of their use.
+    // each, a copy to a page. Each walks the CTA's share by itself. One elected lane issues the copies, whose issue is what
+    // limits pages of 16 tokens, hence a warp for each kind. Page ids wait in shared memory, 32 pages and more ahead.
     const bool vals = role & 1;
     const CUtensorMap* map = vals ? &tmV : &tmK;
     if (role < 2 && elect_one()) tma_prefetch_desc(map);
@@ -232,22 +232,27 @@ attn_rows(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUten
     const uint32_t bytes = role < 2 ? box * D * (INT8 ? 1 : 2) : box * 4;  // of a copy
     const uint32_t dst0 = role < 2 ? sbase + role * C::HALF : sbase + C::OFF_SCALE + vals * BN * 4;
     const uint32_t slot_bytes = role < 2 ? C::SLOT : 2 * BN * 4;
+    int* ids = reinterpret_cast<int*>(smem + C::OFF_IDS) + role * 64;  // page i's id at i % 64
     while (w.cur < w.end) {
       const int end = p.blocks.key_end(w.x, w.blk), cnt = w.count();
-      const int pages = (end + page - 1) >> page_log2;  // that the unit sees
-      int base = (w.tile * BN) >> page_log2;
-      auto ids_from = [&](int i) { return i + lane < pages ? page_of(p.s, w.b, i + lane) : 0; };
-      int ids = ids_from(base), next = ids_from(base + 32);
+      const int pages = (end + page - 1) >> page_log2;    // that the unit sees
+      int ahead = ((w.tile * BN) >> page_log2) & ~31;     // ids are there for pages below
+      auto ids_more = [&]() {
+        ids[(ahead + lane) & 63] = ahead + lane < pages ? page_of(p.s, w.b, ahead + lane) : 0;
+        ahead += 32;
+      };
+      ids_more();
+      ids_more();
+      __syncwarp();
       if (role == 0) {
         if (nu >= kUnitRing && !(ok = wait(q_empty(nu), (nu / kUnitRing - 1) & 1, kErrCopyWait))) break;
         const int row0 = w.blk * BR, rows = min(BR, w.x.n * group - row0);
-        const long long w0 = w.cur - w.tile;
-        const int c0 = w.owner(w0), c1 = w.owner(w0 + w.nt - 1);
+        const int2 own = w.owners(blockIdx.x);
         if (elect_one()) {
           int4* r = ring + 3 * (nu % kUnitRing);
           r[0] = make_int4(cnt, w.tile, end, nu);
           r[1] = make_int4(w.x.len, w.x.n, row0, w.x.tok0);
-          r[2] = make_int4(w.h, c0, c1, 0);
+          r[2] = make_int4(w.h, own.x, own.y, 0);
           mbar_arrive_expect_tx(q_full(nu), rows * D * 2);
         }
         __syncwarp();
@@ -262,34 +267,24 @@ attn_rows(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUten
       const float* head_scale = scale + w.h * st.head;
       for (int i = 0; i < cnt; ++i, ++t) {
         const int s = t % C::SLOTS, round = t / C::SLOTS;
-        const int j0 = (w.tile + i) * BN, place = j0 & (page - 1);
+        const int j0 = (w.tile + i) * BN, place = j0 & (page - 1), first = j0 >> page_log2;
         const int boxes = max(0, (min(j0 + BN, end) - j0 + box - 1) / box);  // pages of the tile that hold keys
         if (round > 0 && !(ok = wait(empty(s), (round - 1) & 1, kErrCopyWait))) break;
-        const uint32_t dst = dst0 + s * slot_bytes;
-        if (elect_one()) mbar_arrive_expect_tx(full(s), boxes * bytes);
-        for (int pg = 0; pg < boxes; pg += 4) {
-          // up to four pages at once (a tile's are 1, 2, or a multiple of 4, and begin at a multiple of that in the 32)
-          const int at = (j0 >> page_log2) + pg;
-          if (at - base >= 32) {
-            base += 32;
-            ids = next;
-            next = ids_from(base + 32);
-          }
-          int from[4];
-#pragma unroll
-          for (int k = 0; k < 4; ++k) from[k] = __shfl_sync(0xffffffffu, ids, at - base + k);
-          if (elect_one()) {
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-              if (pg + k >= boxes) break;
-              const uint32_t to = dst + (pg + k) * bytes;
-              if (role < 2)  // an id that is out of range reads as zeros (the map's bounds)
-                tma_load_5d(to, map, full(s), 0, place, 0, w.h, from[k]);
-              else
-                bulk_load(to, head_scale + max(from[k], 0) * st.page + place, bytes, full(s));
-            }
+        if (elect_one()) {
+          mbar_arrive_expect_tx(full(s), boxes * bytes);
+          uint32_t dst = dst0 + s * slot_bytes;
+#pragma unroll 1
+          for (int pg = 0; pg < boxes; ++pg, dst += bytes) {
+            const int from = ids[(first + pg) & 63];
+            if (role < 2)  // an id that is out of range reads as zeros (the map's bounds)
+              tma_load_5d(dst, map, full(s), 0, place, 0, w.h, from);
+            else
+              bulk_load(dst, head_scale + max(from, 0) * st.page + place, bytes, full(s));
           }
         }
+        __syncwarp();
+        // (a tile has at most 8 pages; those below ahead - 32, which the next ones take the place of, are done with)
+        if (first >= ahead - 32 && ahead < pages) ids_more();
         __syncwarp();
       }
       if (!ok) break;
@@ -377,32 +372,71 @@ attn_rows(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUten
         joiners_meet();
         done = *joined != 0;
         if (done) {
-          const int parts = x.c1 - x.c0 + 1;
-          float2* pml = reinterpret_cast<float2*>(merge);  // [part][BR]
-          for (int i = tid; i < parts * BR; i += 128) pml[i] = __ldcg(p.ml + (2LL * (x.c0 + i / BR) + (i < BR)) * BR + i % BR);
+          // Warp v takes every fourth part, all rows of it at once (32 lanes to a row), and the four sums meet in shared memory.
+          const int parts = x.c1 - x.c0 + 1, rows = min(BR, x.n * group - x.row0);
+          const int v = warp - kConsumers;
+          constexpr int W = D / 32;  // columns of a lane
+          float* sums = merge;       // [warp][BR][D]
+          auto part_ml = [&](int c, int row) { return __ldcg(p.ml + (2LL * (x.c0 + c) + (c == 0)) * BR + row); };
+          for (int r0 = 0; r0 < rows; r0 += 4) {
+            float m4[4], l4[4], a4[4][W];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              m4[k] = -CUDART_INF_F;
+              for (int c = lane; c < parts; c += 32) m4[k] = fmaxf(m4[k], part_ml(c, min(r0 + k, rows - 1)).x);
+              l4[k] = 0.f;
+#pragma unroll
+              for (int e = 0; e < W; ++e) a4[k][e] = 0.f;
+            }
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+#pragma unroll
+              for (int o = 16; o > 0; o >>= 1) m4[k] = fmaxf(m4[k], __shfl_xor_sync(0xffffffffu, m4[k], o));
+              m4[k] = m4[k] == -CUDART_INF_F ? 0.f : m4[k];
+            }
+#pragma unroll 2
+            for (int c = v; c < parts; c += kJoiners) {
+              const float* src = p.part + ((2LL * (x.c0 + c) + (c == 0)) * BR + r0) * D + lane * W;
+#pragma unroll
+              for (int k = 0; k < 4; ++k) {
+                if (r0 + k >= rows) continue;
+                const float2 y = part_ml(c, r0 + k);
+                const float wt = ex2(y.x - m4[k]);
+                l4[k] = fmaf(wt, y.y, l4[k]);
+                float f[W];
+                if constexpr (W == 4) *reinterpret_cast<float4*>(f) = __ldcg(reinterpret_cast<const float4*>(src + k * D));
+                else *reinterpret_cast<float2*>(f) = __ldcg(reinterpret_cast<const float2*>(src + k * D));
+#pragma unroll
+                for (int e = 0; e < W; ++e) a4[k][e] = fmaf(wt, f[e], a4[k][e]);
+              }
+            }
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              if (r0 + k >= rows) continue;
+#pragma unroll
+              for (int e = 0; e < W; ++e) sums[(v * BR + r0 + k) * D + lane * W + e] = a4[k][e];
+              if (lane == 0) ml[v * BR + r0 + k] = make_float2(m4[k], l4[k]);
+            }
+          }
           joiners_meet();
-          M = -CUDART_INF_F;
-          for (int c = 0; c < parts; ++c) M = fmaxf(M, pml[c * BR + r].x);
-          const float ref = M == -CUDART_INF_F ? 0.f : M;
+          M = 0.f;  // (of a row without keys all sums are 0)
           L = 0.f;
 #pragma unroll
           for (int i = 0; i < PER; ++i) acc[i] = 0.f;
           if (there) {
-#pragma unroll 4
-            for (int c = 0; c < parts; ++c) {
-              const float2 y = pml[c * BR + r];
-              const float wt = ex2(y.x - ref);
-              L = fmaf(wt, y.y, L);
-              const float* src = p.part + ((2LL * (x.c0 + c) + (c == 0)) * BR + r) * D + col;
+#pragma unroll 1
+            for (int u4 = 0; u4 < kJoiners; ++u4) {
+              L += ml[u4 * BR + r].y;
 #pragma unroll
               for (int i = 0; i < PER; i += 4) {
-                const float4 f = __ldcg(reinterpret_cast<const float4*>(src + i));
-                acc[i] = fmaf(wt, f.x, acc[i]);
-                acc[i + 1] = fmaf(wt, f.y, acc[i + 1]);
-                acc[i + 2] = fmaf(wt, f.z, acc[i + 2]);
-                acc[i + 3] = fmaf(wt, f.w, acc[i + 3]);
+                const float4 f = *reinterpret_cast<const float4*>(sums + (u4 * BR + r) * D + col + i);
+                acc[i] += f.x;
+                acc[i + 1] += f.y;
+                acc[i + 2] += f.z;
+                acc[i + 3] += f.w;
               }
             }
+            if (L == 0.f) M = -CUDART_INF_F;
           }
           joiners_meet();
         }

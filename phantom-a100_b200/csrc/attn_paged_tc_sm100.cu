@@ -927,7 +927,7 @@ __global__ void __launch_bounds__(BM) merge_chunk(const Params p, int grid) {
   Walk<TokenBlocks> w;
   w.start(p.s, p.blocks, c0 + 1, grid);
   const long long w0 = w.cur - w.tile;
-  if (w.cur >= w.end || w.tile == 0 || w.first(c0) > w0) return;
+  if (w.by_unit || w.cur >= w.end || w.tile == 0 || w.first(c0) > w0) return;
   const int tok = w.blk * p.blocks.per + g * p.tile_tokens;
   if (r >= min(p.tile_tokens, w.x.n - tok) * p.group) return;
   auto slot = [&](int c) { return ((2LL * c + (c > c0 ? 0 : 1)) * 2 + g) * BM + r; };

@@ -293,6 +293,7 @@ int paged_copy(const char* name, const phantom_paged_cache* c, const void* k, co
   a.d = c->head_dim;
   a.bf16 = dtype == PHANTOM_ATTN_BF16;
   a.int8 = c->dtype == PHANTOM_ATTN_I8;
+  a.wide = (reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v)) % 32 == 0;
   a.stream = static_cast<cudaStream_t>(stream);
   const cudaError_t e = launch(a);
   if (e != cudaSuccess) return cuda_fail(name, e);

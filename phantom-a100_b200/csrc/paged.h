@@ -32,6 +32,7 @@ struct PagedCopyArgs {
   Strides3 kcs, vcs, kss, vss;
   int d;
   bool bf16, int8;
+  bool wide;                // k and v are 32-byte aligned
   cudaStream_t stream;
 };
 

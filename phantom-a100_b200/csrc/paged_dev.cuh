@@ -62,11 +62,14 @@ __device__ __forceinline__ long long sum_tiles(const Blocks& k, const Seq& x) {
   return w;
 }
 
+constexpr int kJoinTiles = 5;
+
 // A whole warp walks one CTA's share; every value is uniform over the warp.
 template <typename Blocks>
 struct Walk {
   long long share, cur, end;
   int more, ctas;           // CTA c has share + (c < more) tiles; CTAs that have any
+  bool by_unit;             // or CTA c has the unit c
   Seq x;
   int b, h, blk, tile, nt;  // the unit, its tile at `cur`, its tiles
 
@@ -83,55 +86,87 @@ struct Walk {
   __device__ void start(const PagedSeqs& s, const Blocks& k, int cta, int grid) {
     const int lane = threadIdx.x & 31;
     auto seq_tiles = [&](int i) { return i < s.batch ? k.head_tiles(seq_of(s, i)) * s.heads : 0LL; };
-    // (up to 32 sequences: one scan gives the total and the place)
-    long long w = scan(seq_tiles(lane), lane);
-    long long total = __shfl_sync(0xffffffffu, w, 31);
-    for (int i0 = 32; i0 < s.batch; i0 += 32) total += __shfl_sync(0xffffffffu, scan(seq_tiles(i0 + lane), lane), 31);
+    // Whole units, one to a CTA, where that takes no more than kJoinTiles tiles longer than even shares: joining a shared
+    // unit costs about as much (measured: 4 us, a tile of 32 KB 0.75 us). First and last blocks bound a head's units.
+    long long units = 0, w = 0, total = 0;
+    int most = 0;
+    for (int i0 = 0; i0 < s.batch; i0 += 32) {
+      long long y = 0;
+      if (i0 + lane < s.batch) {
+        const Seq q = seq_of(s, i0 + lane);
+        y = k.head_tiles(q) * s.heads;
+        const int c = k.count(q);
+        units += (long long)c * s.heads;
+        if (c > 0) most = max(most, tiles_of(k, q, c - 1));
+      }
+      const long long z = scan(y, lane);
+      if (i0 == 0) w = z;  // (up to 32 sequences: one scan gives the total and the place)
+      total += __shfl_sync(0xffffffffu, z, 31);
+    }
+    for (int m = 16; m > 0; m >>= 1) {
+      units += __shfl_xor_sync(0xffffffffu, units, m);
+      most = max(most, __shfl_xor_sync(0xffffffffu, most, m));
+    }
     ctas = (int)min((long long)grid, total);  // each has a tile then
     share = ctas > 0 ? quotient(total, ctas) : 0;
     more = (int)(total - share * ctas);
-    cur = cta < ctas ? first(cta) : 0;
-    end = cta < ctas ? first(cta + 1) : 0;
-    if (cur >= end) return;
+    by_unit = units <= grid && most <= share + kJoinTiles;
+    if (by_unit) ctas = (int)units;
+    cur = end = 0;
+    if (cta >= ctas) return;
+    // the place of the CTA's first tile, or of its unit, among all
+    const long long at = by_unit ? cta : first(cta);
+    auto seq_part = [&](int i) {
+      return by_unit ? (i < s.batch ? (long long)k.count(seq_of(s, i)) * s.heads : 0LL) : seq_tiles(i);
+    };
     long long before = 0;
     for (int i0 = 0;; i0 += 32) {
-      if (i0 > 0) w = scan(seq_tiles(i0 + lane), lane);
-      const unsigned past = __ballot_sync(0xffffffffu, before + w > cur);
+      if (i0 > 0 || by_unit) w = scan(seq_part(i0 + lane), lane);
+      const unsigned past = __ballot_sync(0xffffffffu, before + w > at);
       if (past) {
-        const int at = __ffs(past) - 1;
-        const long long up_to = __shfl_sync(0xffffffffu, w, max(at - 1, 0));
-        b = i0 + at;
-        before += at > 0 ? up_to : 0;
+        const int l = __ffs(past) - 1;
+        const long long up_to = __shfl_sync(0xffffffffu, w, max(l - 1, 0));
+        b = i0 + l;
+        before += l > 0 ? up_to : 0;
         break;
       }
       before += __shfl_sync(0xffffffffu, w, 31);
     }
     x = seq_of(s, b);
-    const long long head = k.head_tiles(x);
-    long long r = cur - before;
+    const int count = k.count(x);
+    const long long head = by_unit ? count : k.head_tiles(x);
+    long long r = at - before;
     h = (int)quotient(r, head);
     r -= h * head;
     blk = 0;
-    const int count = k.count(x);
-    for (int i0 = 0; count > 1; i0 += 32) {
+    if (by_unit) {
+      blk = (int)r;
+      r = 0;
+    }
+    for (int i0 = 0; !by_unit && count > 1; i0 += 32) {
       const int y = i0 + lane < count ? tiles_of(k, x, i0 + lane) : 0;
       w = scan(y, lane);
       const unsigned past = __ballot_sync(0xffffffffu, w > r);
       if (past) {
-        const int at = __ffs(past) - 1;
-        const long long up_to = __shfl_sync(0xffffffffu, w, max(at - 1, 0));
-        blk = i0 + at;
-        r -= at > 0 ? up_to : 0;
+        const int l = __ffs(past) - 1;
+        const long long up_to = __shfl_sync(0xffffffffu, w, max(l - 1, 0));
+        blk = i0 + l;
+        r -= l > 0 ? up_to : 0;
         break;
       }
       r -= __shfl_sync(0xffffffffu, w, 31);
     }
     nt = tiles_of(k, x, blk);
     tile = (int)r;
+    cur = by_unit ? 0 : at;
+    end = by_unit ? nt : first(cta + 1);
   }
-  // The first tile of a CTA's share.
+  // The first tile of a CTA's share (even shares).
   __device__ long long first(int cta) const { return cta * share + min(cta, more); }
-  // The CTA that has a tile.
+  // The first and the last CTA that have tiles of the unit, the caller being CTA `cta`.
+  __device__ int2 owners(int cta) const {
+    return by_unit ? make_int2(cta, cta) : make_int2(owner(cur - tile), owner(cur - tile + nt - 1));
+  }
   __device__ int owner(long long at) const {
     const long long big = more * (share + 1);
     return (int)(at < big ? quotient(at, share + 1) : more + quotient(at - big, share));
@@ -157,13 +192,12 @@ struct Walk {
 };
 
 // The parts of a shared unit are joined by the CTA that finds all of them written. Each part has a 64-bit flag that holds
-// the call's number (unique in the process) once the part is in memory. A CTA writes its part, then its flag, then reads
-// all the unit's flags: in the order that fence.sc gives the flags' writes, the CTA of the last one finds them all. (Two
+// the call's number (unique in the process) once the part is in memory. A CTA writes its part, then its flag (release), then,
+// past a fence.sc, reads all the unit's flags: in the order that the fences have, the CTA of the last one finds them all. (Two
 // may; they write the same result.) It then clears them, so that a call replayed from a graph, whose number is the same
 // each time, finds none set. Flags need no initialisation: what a pool's memory held before does not equal the number.
 __device__ __forceinline__ void flag_set(unsigned long long* flag, unsigned long long call) {
-  asm volatile("fence.sc.gpu;" ::: "memory");
-  asm volatile("st.relaxed.gpu.global.u64 [%0], %1;" ::"l"(flag), "l"(call) : "memory");
+  asm volatile("st.release.gpu.global.u64 [%0], %1;" ::"l"(flag), "l"(call) : "memory");
   asm volatile("fence.sc.gpu;" ::: "memory");
 }
 __device__ __forceinline__ unsigned long long flag_get(const unsigned long long* flag) {
@@ -176,7 +210,7 @@ __device__ __forceinline__ bool flags_all(const unsigned long long* flags, int p
   bool all = true;
   for (int c = c0 + (int)(threadIdx.x & 31); c <= c1; c += 32) all &= flag_get(flags + (2LL * c + (c == c0)) * per) == call;
   all = __all_sync(0xffffffffu, all);
-  asm volatile("fence.sc.gpu;" ::: "memory");
+  asm volatile("fence.acq_rel.gpu;" ::: "memory");
   return all;
 }
 __device__ __forceinline__ void flags_clear(unsigned long long* flags, int per, int c0, int c1) {
