@@ -86,7 +86,7 @@ struct Cfg {
 template <int NT, int BN>
 struct RowBlocks {
   int group, causal, heads;
-  static constexpr int kTile = BN, BR = 8 * NT;
+  static constexpr int kTile = BN, kUnit = 2, BR = 8 * NT;
   __device__ int count(const Seq& x) const { return (x.n * group + BR - 1) / BR; }
   __device__ int key_end(const Seq& x, int rb) const {
     if (!causal) return x.len;
@@ -233,8 +233,8 @@ attn_rows(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUten
     const uint32_t dst0 = role < 2 ? sbase + role * C::HALF : sbase + C::OFF_SCALE + vals * BN * 4;
     const uint32_t slot_bytes = role < 2 ? C::SLOT : 2 * BN * 4;
     int* ids = reinterpret_cast<int*>(smem + C::OFF_IDS) + role * 64;  // page i's id at i % 64
-    while (w.cur < w.end) {
-      const int end = p.blocks.key_end(w.x, w.blk), cnt = w.count();
+    while (w.cnt > 0) {
+      const int end = p.blocks.key_end(w.x, w.blk), cnt = w.cnt;
       const int pages = (end + page - 1) >> page_log2;    // that the unit sees
       int ahead = ((w.tile * BN) >> page_log2) & ~31;     // ids are there for pages below
       auto ids_more = [&]() {

@@ -72,7 +72,7 @@ struct Cfg {
 // Units of `per` new tokens; tiles of 128 keys.
 struct TokenBlocks {
   int per, causal, heads;
-  static constexpr int kTile = BN;
+  static constexpr int kTile = BN, kUnit = 4;
   __device__ int count(const Seq& x) const { return (x.n + per - 1) / per; }
   __device__ int key_end(const Seq& x, int blk) const {
     return causal ? min(max(x.len - x.n + min(x.n, (blk + 1) * per), 0), x.len) : x.len;
@@ -367,22 +367,21 @@ attn_chunk(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUte
       __syncwarp();
       Walk<TokenBlocks> w;
       w.start(p.s, p.blocks, blockIdx.x, gridDim.x);
-      const long long begin = w.cur;
       int nu = 0;
       for (;; ++nu) {
         if (nu > 1 && !(ok = wait(unit_read(nu), ((nu >> 1) - 1) & 1, kErrTmaWait))) break;
         Unit x = {};
-        x.id = w.cur < w.end ? nu : -1;
+        x.id = w.cnt > 0 ? nu : -1;
         if (x.id >= 0) {
           x.b = w.b;
           x.h = w.h;
-          x.cnt = w.count();
+          x.cnt = w.cnt;
           x.tile0 = w.tile;
           x.end = p.blocks.key_end(w.x, w.blk);
           x.tok = w.blk * p.blocks.per;
           x.len = w.x.len, x.n = w.x.n, x.tok0 = w.x.tok0;
           x.has_b = x.tok + p.tile_tokens < x.n;
-          x.slot = x.cnt == w.nt ? -1 : w.place(blockIdx.x, begin <= w.cur - w.tile);
+          x.slot = x.cnt == w.nt ? -1 : w.place(blockIdx.x, w.tile == 0);
         }
         if (elect_one()) {
           publish(nu, x);
@@ -907,38 +906,40 @@ attn_chunk(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUte
   }
 }
 
-// Joins the parts of the units that several CTAs of attn_chunk shared. Block (c, query tile, 16 columns): the unit that CTA
-// c continues, if c is the first to continue it; thread = query row; the parts in the order of the CTAs. Block (0, 0, 0)
-// also zeroes the rows of packed tokens that belong to no sequence.
-constexpr int kMergeCols = 16;
+// Joins the parts of the units that several CTAs of attn_chunk shared. Block (c, query tile): the unit that CTA c continues,
+// if c is the first to continue it; thread = query row and 32 columns; the parts in the order of the CTAs. Block (0, 0) also
+// zeroes the rows of packed tokens that belong to no sequence.
+constexpr int kMergeCols = 32;
 template <int D, bool BF16>
-__global__ void __launch_bounds__(BM) merge_chunk(const Params p, int grid) {
+__global__ void __launch_bounds__(BM * D / kMergeCols) merge_chunk(const Params p, int grid) {
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  const int g = blockIdx.y, col = blockIdx.z * kMergeCols, r = threadIdx.x, c0 = blockIdx.x - 1;
+  const int g = blockIdx.y, c0 = blockIdx.x - 1;
   if (c0 < 0) {
-    if (g == 0 && col == 0) {
+    if (g == 0) {
       const int first = min(max(p.s.cu_new[p.s.batch], 0), p.s.total);
       const long long row = (long long)p.s.heads * p.group * D;
-      for (long long i = first * row + r; i < p.s.total * row; i += BM) p.o[i] = 0;
+      for (long long i = first * row + threadIdx.x; i < p.s.total * row; i += blockDim.x) p.o[i] = 0;
     }
     return;
   }
   Walk<TokenBlocks> w;
   w.start(p.s, p.blocks, c0 + 1, grid);
-  const long long w0 = w.cur - w.tile;
-  if (w.by_unit || w.cur >= w.end || w.tile == 0 || w.first(c0) > w0) return;
+  if (w.by_unit || w.cnt <= 0 || w.tile == 0) return;
+  const int2 own = w.owners(c0 + 1);
+  if (own.x != c0) return;
+  const int r = threadIdx.x % BM, col = threadIdx.x / BM * kMergeCols;
   const int tok = w.blk * p.blocks.per + g * p.tile_tokens;
   if (r >= min(p.tile_tokens, w.x.n - tok) * p.group) return;
-  auto slot = [&](int c) { return ((2LL * c + (c > c0 ? 0 : 1)) * 2 + g) * BM + r; };
+  auto slot = [&](int c) { return ((long long)w.place(c, c == c0) * 2 + g) * BM + r; };
   float M = -CUDART_INF_F, L = 0.f, acc[kMergeCols];
 #pragma unroll
   for (int i = 0; i < kMergeCols; ++i) acc[i] = 0.f;
-  int c1 = c0;
-  for (; c1 < w.ctas && w.first(c1) < w0 + w.nt; ++c1) M = fmaxf(M, p.ml[slot(c1)].x);
+#pragma unroll 4
+  for (int c = c0; c <= own.y; ++c) M = fmaxf(M, p.ml[slot(c)].x);
   const float ref = M == -CUDART_INF_F ? 0.f : M;
 #pragma unroll 2
-  for (int c = c0; c < c1; ++c) {
+  for (int c = c0; c <= own.y; ++c) {
     const float2 y = p.ml[slot(c)];
     const float wt = ex2(y.x - ref);
     L = fmaf(wt, y.y, L);
@@ -953,14 +954,13 @@ __global__ void __launch_bounds__(BM) merge_chunk(const Params p, int grid) {
     }
   }
   const float inv = M == -CUDART_INF_F ? 0.f : 1.f / L;
-  uint32_t out[kMergeCols / 2];
-#pragma unroll
-  for (int i = 0; i < kMergeCols / 2; ++i) out[i] = pack2<BF16>(acc[2 * i] * inv, acc[2 * i + 1] * inv);
   const int t = r / p.group;
   uint4* dst = reinterpret_cast<uint4*>(
       p.o + (((long long)(w.x.tok0 + tok + t) * p.s.heads + w.h) * p.group + (r - t * p.group)) * D + col);
-  dst[0] = make_uint4(out[0], out[1], out[2], out[3]);
-  dst[1] = make_uint4(out[4], out[5], out[6], out[7]);
+#pragma unroll
+  for (int i = 0; i < kMergeCols / 8; ++i)
+    dst[i] = make_uint4(pack2<BF16>(acc[8 * i] * inv, acc[8 * i + 1] * inv), pack2<BF16>(acc[8 * i + 2] * inv, acc[8 * i + 3] * inv),
+                        pack2<BF16>(acc[8 * i + 4] * inv, acc[8 * i + 5] * inv), pack2<BF16>(acc[8 * i + 6] * inv, acc[8 * i + 7] * inv));
 }
 
 std::atomic<bool> g_attr[2][2][2][64];
@@ -1006,8 +1006,8 @@ cudaError_t launch(const PagedAttnArgs& a, int dev) {
   e = cudaLaunchKernelEx(&cfg, kern, mq, mk, mv, p);
   if (e == cudaSuccess) {
     note_launch();
-    cfg.gridDim = dim3((unsigned)ctas, 2, D / kMergeCols);
-    cfg.blockDim = dim3(BM);
+    cfg.gridDim = dim3((unsigned)ctas, 2);
+    cfg.blockDim = dim3(BM * D / kMergeCols);
     cfg.dynamicSmemBytes = 0;
     if ((e = cudaLaunchKernelEx(&cfg, merge_chunk<D, BF16>, p, ctas)) == cudaSuccess) note_launch();
   }

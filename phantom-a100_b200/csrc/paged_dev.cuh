@@ -48,12 +48,19 @@ __device__ __forceinline__ int seq_index(const PagedSeqs& s, int tok) {
 // An attention call's work: units (sequence, key head, block of query rows) in a row, each of as many tiles of keys as its
 // rows see. CTA c of G takes the tiles [c W / G, (c + 1) W / G) of all W, so a unit may be shared by several CTAs.
 // `Blocks` says how the rows are cut: kTile keys to a tile; count(x) blocks; the keys key_end(x, blk) that a block sees;
-// head_tiles(x) tiles in all of one head.
+// head_tiles(x) tiles in all of one head. A unit costs something besides its tiles (its queries, its output, the start of
+// its pipeline), as much as kUnit tiles; these are counted before its first one when the shares are cut, and a share that
+// ends among them has nothing of the unit.
 
 // At least one tile, so that rows without any key are written too (as zeros).
 template <typename Blocks>
 __device__ __forceinline__ int tiles_of(const Blocks& k, const Seq& x, int blk) {
   return max(1, (k.key_end(x, blk) + Blocks::kTile - 1) / Blocks::kTile);
+}
+// Tiles of one head, the units' own costs counted.
+template <typename Blocks>
+__device__ __forceinline__ long long head_work(const Blocks& k, const Seq& x) {
+  return k.head_tiles(x) + (long long)k.count(x) * Blocks::kUnit;
 }
 template <typename Blocks>
 __device__ __forceinline__ long long sum_tiles(const Blocks& k, const Seq& x) {
@@ -64,14 +71,16 @@ __device__ __forceinline__ long long sum_tiles(const Blocks& k, const Seq& x) {
 
 constexpr int kJoinTiles = 5;
 
-// A whole warp walks one CTA's share; every value is uniform over the warp.
+// A whole warp walks one CTA's share; every value is uniform over the warp. Positions count tiles and units' own costs.
 template <typename Blocks>
 struct Walk {
-  long long share, cur, end;
-  int more, ctas;           // CTA c has share + (c < more) tiles; CTAs that have any
-  bool by_unit;             // or CTA c has the unit c
+  static constexpr int kUnit = Blocks::kUnit;
+  long long share, at, end;  // at: where the unit begins; end: where the share does
+  int more, ctas;            // CTA c has share + (c < more); CTAs that have any
+  bool by_unit;              // or CTA c has the unit c
   Seq x;
-  int b, h, blk, tile, nt;  // the unit, its tile at `cur`, its tiles
+  int b, h, blk, nt;         // the unit, its tiles
+  int tile, cnt;             // the first of them here, how many are; 0 at the end of the share
 
   __device__ static long long scan(long long w, int lane) {
     for (int m = 1; m < 32; m <<= 1) {
@@ -85,16 +94,16 @@ struct Walk {
   }
   __device__ void start(const PagedSeqs& s, const Blocks& k, int cta, int grid) {
     const int lane = threadIdx.x & 31;
-    auto seq_tiles = [&](int i) { return i < s.batch ? k.head_tiles(seq_of(s, i)) * s.heads : 0LL; };
+    auto seq_work = [&](int i) { return i < s.batch ? head_work(k, seq_of(s, i)) * s.heads : 0LL; };
     // Whole units, one to a CTA, where that takes no more than kJoinTiles tiles longer than even shares: joining a shared
-    // unit costs about as much (measured: 4 us, a tile of 32 KB 0.75 us). First and last blocks bound a head's units.
+    // unit costs about as much (measured: 4 us, a tile of 32 KB 0.75 us). A head's last block sees the most keys.
     long long units = 0, w = 0, total = 0;
     int most = 0;
     for (int i0 = 0; i0 < s.batch; i0 += 32) {
       long long y = 0;
       if (i0 + lane < s.batch) {
         const Seq q = seq_of(s, i0 + lane);
-        y = k.head_tiles(q) * s.heads;
+        y = head_work(k, q) * s.heads;
         const int c = k.count(q);
         units += (long long)c * s.heads;
         if (c > 0) most = max(most, tiles_of(k, q, c - 1));
@@ -107,22 +116,22 @@ struct Walk {
       units += __shfl_xor_sync(0xffffffffu, units, m);
       most = max(most, __shfl_xor_sync(0xffffffffu, most, m));
     }
-    ctas = (int)min((long long)grid, total);  // each has a tile then
+    ctas = (int)min((long long)grid, total);
     share = ctas > 0 ? quotient(total, ctas) : 0;
     more = (int)(total - share * ctas);
-    by_unit = units <= grid && most <= share + kJoinTiles;
+    by_unit = units <= grid && most + kUnit <= share + kJoinTiles;
     if (by_unit) ctas = (int)units;
-    cur = end = 0;
+    cnt = 0;
     if (cta >= ctas) return;
-    // the place of the CTA's first tile, or of its unit, among all
-    const long long at = by_unit ? cta : first(cta);
+    // the place of the share's beginning, or of the CTA's unit, among all
+    const long long pos = by_unit ? cta : first(cta);
     auto seq_part = [&](int i) {
-      return by_unit ? (i < s.batch ? (long long)k.count(seq_of(s, i)) * s.heads : 0LL) : seq_tiles(i);
+      return by_unit ? (i < s.batch ? (long long)k.count(seq_of(s, i)) * s.heads : 0LL) : seq_work(i);
     };
     long long before = 0;
     for (int i0 = 0;; i0 += 32) {
       if (i0 > 0 || by_unit) w = scan(seq_part(i0 + lane), lane);
-      const unsigned past = __ballot_sync(0xffffffffu, before + w > at);
+      const unsigned past = __ballot_sync(0xffffffffu, before + w > pos);
       if (past) {
         const int l = __ffs(past) - 1;
         const long long up_to = __shfl_sync(0xffffffffu, w, max(l - 1, 0));
@@ -134,8 +143,8 @@ struct Walk {
     }
     x = seq_of(s, b);
     const int count = k.count(x);
-    const long long head = by_unit ? count : k.head_tiles(x);
-    long long r = at - before;
+    const long long head = by_unit ? count : head_work(k, x);
+    long long r = pos - before;
     h = (int)quotient(r, head);
     r -= h * head;
     blk = 0;
@@ -144,7 +153,7 @@ struct Walk {
       r = 0;
     }
     for (int i0 = 0; !by_unit && count > 1; i0 += 32) {
-      const int y = i0 + lane < count ? tiles_of(k, x, i0 + lane) : 0;
+      const int y = i0 + lane < count ? tiles_of(k, x, i0 + lane) + kUnit : 0;
       w = scan(y, lane);
       const unsigned past = __ballot_sync(0xffffffffu, w > r);
       if (past) {
@@ -157,28 +166,27 @@ struct Walk {
       r -= __shfl_sync(0xffffffffu, w, 31);
     }
     nt = tiles_of(k, x, blk);
-    tile = (int)r;
-    cur = by_unit ? 0 : at;
-    end = by_unit ? nt : first(cta + 1);
+    at = by_unit ? 0 : pos - r;
+    end = by_unit ? nt + kUnit : first(cta + 1);
+    tile = max(0, (int)r - kUnit);
+    cnt = (int)min((long long)nt, end - at - kUnit) - tile;
   }
-  // The first tile of a CTA's share (even shares).
+  // Where a CTA's share begins (even shares).
   __device__ long long first(int cta) const { return cta * share + min(cta, more); }
   // The first and the last CTA that have tiles of the unit, the caller being CTA `cta`.
   __device__ int2 owners(int cta) const {
-    return by_unit ? make_int2(cta, cta) : make_int2(owner(cur - tile), owner(cur - tile + nt - 1));
+    return by_unit ? make_int2(cta, cta) : make_int2(owner(at + kUnit), owner(at + kUnit + nt - 1));
   }
-  __device__ int owner(long long at) const {
+  __device__ int owner(long long pos) const {
     const long long big = more * (share + 1);
-    return (int)(at < big ? quotient(at, share + 1) : more + quotient(at - big, share));
+    return (int)(pos < big ? quotient(pos, share + 1) : more + quotient(pos - big, share));
   }
-  // The tiles of the unit that this CTA has.
-  __device__ int count() const { return (int)min((long long)(nt - tile), end - cur); }
-  // A unit that several CTAs share: CTA c's part of it lies in the place 2 c + 1 if the unit begins in c's share, else 2 c.
+  // A unit that several CTAs share: CTA c's part of it lies in the place 2 c + 1 if its first tile is c's, else 2 c.
   __device__ static int place(int cta, bool begins) { return 2 * cta + (begins ? 1 : 0); }
   __device__ void advance(const PagedSeqs& s, const Blocks& k) {
-    cur += count();
-    if (cur >= end) return;
-    tile = 0;
+    at += nt + kUnit;
+    cnt = 0;
+    if (at >= end) return;
     if (++blk == k.count(x)) {
       blk = 0;
       if (++h == s.heads) {
@@ -188,6 +196,8 @@ struct Walk {
       }
     }
     nt = tiles_of(k, x, blk);
+    tile = 0;
+    cnt = (int)max(0LL, min((long long)nt, end - at - kUnit));
   }
 };
 
