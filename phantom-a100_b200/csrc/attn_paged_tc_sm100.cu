@@ -771,7 +771,8 @@ attn_chunk(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUte
             for (int k = 0; k < 4; ++k) {
               // (all by ex2: the polynomial's least value, 2^-125, would count in a sum that multiplies it with 1 / vs)
               const int e = 64 * (k >> 1) + 4 * i + 2 * (k & 1);
-              const float2 x = make_float2(ex2(s[e] - sub[k]), ex2(s[e + 1] - sub[k]));
+              float2 x = add2(make_float2(s[e], s[e + 1]), make_float2(-sub[k], -sub[k]));
+              x = make_float2(ex2(x.x), ex2(x.y));
               r4.l[k] = fma2(x, inv, r4.l[k]);
               pk[k >> 1][2 * i + (k & 1)] = pack2<false>(x.x, x.y);
             }

@@ -10,6 +10,8 @@
 
 #include "../../include/phantom_attn.h"
 
+extern "C" void phantom_attn_pointers_checked(int on);  // capi.cu, between the library and this extension
+
 namespace {
 
 using CFn = int (*)(const void*, const void*, const void*, void*, int, int, int, int, int, void*);
@@ -128,6 +130,12 @@ phantom_paged_cache paged_cache(const torch::Tensor& kc, const torch::Tensor& vc
   return c;
 }
 
+// While it lives, the library takes this thread's pointers as checked (they are, by the tensors' devices).
+struct PointersChecked {
+  PointersChecked() { phantom_attn_pointers_checked(1); }
+  ~PointersChecked() { phantom_attn_pointers_checked(0); }
+};
+
 // A packed (tokens, heads, d) tensor of new tokens.
 void check_packed(const torch::Tensor& t, const torch::Tensor& kc, const char* what) {
   TORCH_CHECK(t.is_cuda(), "inputs must be CUDA tensors");
@@ -150,6 +158,7 @@ void paged_append(const torch::Tensor& k, const torch::Tensor& v, const torch::T
   if (k.size(0) == 0) return;
   const c10::cuda::CUDAGuard guard(kc.device());
   const long long d = k.size(2), token = k.size(1) * d;
+  const PointersChecked checked;
   const int rc = phantom_attn_paged_append(&c, k.data_ptr(), v.data_ptr(), stride_of(k, 0, token), stride_of(k, 1, d),
                                            stride_of(v, 0, token), stride_of(v, 1, d), (int)k.size(0), dtype_code(k),
                                            at::cuda::getCurrentCUDAStream().stream());
@@ -165,6 +174,7 @@ std::tuple<torch::Tensor, torch::Tensor> paged_read(const torch::Tensor& kc, con
   const auto opts = kc.options().dtype(bf16 ? at::kBFloat16 : at::kHalf);
   auto k = torch::empty({total, kc.size(1), kc.size(3)}, opts), v = torch::empty_like(k);
   if (total == 0) return {k, v};
+  const PointersChecked checked;
   const int rc = phantom_attn_paged_read(&c, k.data_ptr(), v.data_ptr(), (int)total, bf16 ? PHANTOM_ATTN_BF16 : PHANTOM_ATTN_F16,
                                          at::cuda::getCurrentCUDAStream().stream());
   TORCH_CHECK(rc == PHANTOM_ATTN_OK, phantom_attn_last_error());
@@ -181,6 +191,7 @@ torch::Tensor paged_attn(const torch::Tensor& q, const torch::Tensor& kc, const 
   auto o = torch::empty(q.sizes(), q.options());
   if (q.numel() == 0) return o;
   const long long d = q.size(2);
+  const PointersChecked checked;
   const int rc = phantom_attn_paged(&c, q.data_ptr(), stride_of(q, 0, q.size(1) * d), stride_of(q, 1, d), o.data_ptr(),
                                     (int)q.size(0), (int)q.size(1), dtype_code(q), causal ? 1 : 0, (float)scale, (int)max_new,
                                     at::cuda::getCurrentCUDAStream().stream());

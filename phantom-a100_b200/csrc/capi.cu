@@ -205,9 +205,16 @@ int noalloc_setup(const char* name, int dev, unsigned char** scratch, int* cc, i
 }
 
 // ------------------------------------------------------------------ paged cache
+// Set by the torch binding around its calls (phantom_attn_pointers_checked): its tensors are known to be device memory of
+// the current device, and asking the driver about each of nine pointers took a third of a small call's time on the host.
+thread_local bool g_pointers_checked = false;
+
 // One device pointer of a paged call, 16-byte aligned unless it is an int array (4 bytes).
 int check_paged_ptr(const char* name, const char* what, const void* p, int dev, int align) {
   if (p == nullptr) return fail(PHANTOM_ATTN_ERR_INVALID, "%s: inputs must be CUDA tensors (%s is a null pointer)", name, what);
+  if (reinterpret_cast<uintptr_t>(p) % align != 0)
+    return fail(PHANTOM_ATTN_ERR_INVALID, "%s: %s must be %d-byte aligned", name, what, align);
+  if (g_pointers_checked) return PHANTOM_ATTN_OK;
   cudaPointerAttributes attr;
   if (cudaPointerGetAttributes(&attr, p) != cudaSuccess) {
     cudaGetLastError();
@@ -217,8 +224,6 @@ int check_paged_ptr(const char* name, const char* what, const void* p, int dev, 
     return fail(PHANTOM_ATTN_ERR_INVALID, "%s: inputs must be CUDA tensors (%s)", name, what);
   if (attr.type == cudaMemoryTypeDevice && attr.device != dev)
     return fail(PHANTOM_ATTN_ERR_INVALID, "%s: all tensors must be on the same device (%s; current device %d)", name, what, dev);
-  if (reinterpret_cast<uintptr_t>(p) % align != 0)
-    return fail(PHANTOM_ATTN_ERR_INVALID, "%s: %s must be %d-byte aligned", name, what, align);
   return PHANTOM_ATTN_OK;
 }
 
@@ -422,6 +427,8 @@ int phantom_attn_fused_tc_noalloc(const void* q, const void* k, const void* v, v
   g_last_error.clear();
   return PHANTOM_ATTN_OK;
 }
+
+void phantom_attn_pointers_checked(int on) { g_pointers_checked = on != 0; }
 
 int phantom_attn_paged_append(const phantom_paged_cache* cache, const void* k, const void* v, long long k_token,
                               long long k_head, long long v_token, long long v_head, int total_new, int dtype, void* stream) {
