@@ -450,6 +450,8 @@ int phantom_attn_paged(const phantom_paged_cache* cache, const void* q, long lon
   if (q_heads <= 0 || q_heads % cache->heads != 0 || q_heads / cache->heads > 128)
     return fail(PHANTOM_ATTN_ERR_INVALID, "%s: query heads must be 1 to 128 times the key heads (got %d and %d)", name, q_heads,
                 cache->heads);
+  if ((long long)total_new * (q_heads / cache->heads) > 0x7fffffffLL - 1024)
+    return fail(PHANTOM_ATTN_ERR_UNSUPPORTED, "%s: query rows of a key head exceed 2^31 (total_new = %d)", name, total_new);
   if (max_new < 0 || !(scale - scale == 0.f))
     return fail(PHANTOM_ATTN_ERR_INVALID, "%s: max_new must not be negative and scale must be finite", name);
   if (!stride_ok(q_token, 2) || !stride_ok(q_head, 2))

@@ -18,7 +18,7 @@ __device__ __forceinline__ Seq seq_of(const PagedSeqs& s, int b) {
   Seq x;
   x.tok0 = min(max(c0, 0), s.total);
   x.n = min(max(c1, x.tok0), s.total) - x.tok0;
-  x.len = (int)min((long long)max(len, 0), min(room, 0x7fffff00LL));
+  x.len = (int)min((long long)max(len, 0), min(room, 0x7ffff000LL));
   if (x.tok0 != c0 || x.tok0 + x.n != c1 || x.len != len) atomicOr(s.status, PHANTOM_ATTN_STATUS_PAGE);
   return x;
 }

@@ -399,3 +399,12 @@ def test_c_abi(capi):
     capi.launch_count(reset=True)
     assert capi.lib.phantom_attn_paged(None, None, 0, 0, None, 1, 1, C_BF16, 1, 0.0, 0, stream) != 0 and "null cache" in capi.last_error()
     assert capi.launch_count() == 0
+
+
+@pytest.mark.parametrize("int8,dtype", [(False, BF16), (True, BF16), (True, F16)])
+def test_serving_example(int8, dtype):
+    """Prompts in chunks and decoding over reused pages; every finished sequence against the dense fp32 kernel on the
+    tokens read back: they differ by the output's rounding, the probabilities', and, for int8, the read back tokens'."""
+    from cuda_attn import serve_paged
+    server, worst, steps = serve_paged.run(8, pages=150, chunk=200, int8=int8, dtype=dtype, d=64, heads=2)
+    assert worst <= (8e-3 if dtype == BF16 else 1e-3) and steps > 40 and len(server.pool.free) == 150
