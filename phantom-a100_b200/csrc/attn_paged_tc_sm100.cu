@@ -113,6 +113,7 @@ struct Params {
   Strides3 kcs, vcs, kss, vss;
   float4* part;            // partial results: [CTA][2][query tile][D / 4][row], fp32
   float2* ml;              // their (reference maximum, sum): [CTA][2][query tile][row]
+  int4* starts;            // for merge_chunk, [CTA][2]: the unit that the CTA is the first to continue, or 0 CTAs
 };
 
 // What the producer tells the other roles of a unit (48 bytes).
@@ -367,6 +368,15 @@ attn_chunk(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUte
       __syncwarp();
       Walk<TokenBlocks> w;
       w.start(p.s, p.blocks, blockIdx.x, gridDim.x);
+      {
+        const int2 own = w.cnt > 0 && w.tile > 0 ? w.owners(blockIdx.x) : make_int2(0, 0);
+        const bool first = own.y > own.x && own.x == (int)blockIdx.x - 1;
+        if (elect_one()) {
+          p.starts[2 * blockIdx.x] = make_int4(first ? own.y - own.x + 1 : 0, w.h, w.blk * p.blocks.per, 0);
+          p.starts[2 * blockIdx.x + 1] = make_int4(w.x.tok0, w.x.n, 0, 0);
+        }
+        __syncwarp();
+      }
       int nu = 0;
       for (;; ++nu) {
         if (nu > 1 && !(ok = wait(unit_read(nu), ((nu >> 1) - 1) & 1, kErrTmaWait))) break;
@@ -907,61 +917,73 @@ attn_chunk(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUte
   }
 }
 
-// Joins the parts of the units that several CTAs of attn_chunk shared. Block (c, query tile): the unit that CTA c continues,
-// if c is the first to continue it; thread = query row and 32 columns; the parts in the order of the CTAs. Block (0, 0) also
-// zeroes the rows of packed tokens that belong to no sequence.
-constexpr int kMergeCols = 32;
+// Joins the parts of the units that several CTAs of attn_chunk shared. Block (c, query tile, 32 columns): the unit that CTA c
+// is the first to continue; thread = query row and 8 columns; the parts in the order of the CTAs, four on their way at
+// once, in one pass with a running maximum. Block (0, 0, 0) also zeroes the rows of packed tokens that belong to no sequence.
+constexpr int kMergeCols = 8, kMergeThreads = 512;
 template <int D, bool BF16>
-__global__ void __launch_bounds__(BM * D / kMergeCols) merge_chunk(const Params p, int grid) {
+__global__ void __launch_bounds__(kMergeThreads) merge_chunk(const Params p) {
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const int g = blockIdx.y, c0 = blockIdx.x - 1;
   if (c0 < 0) {
-    if (g == 0) {
+    if (g == 0 && blockIdx.z == 0) {
       const int first = min(max(p.s.cu_new[p.s.batch], 0), p.s.total);
       const long long row = (long long)p.s.heads * p.group * D;
       for (long long i = first * row + threadIdx.x; i < p.s.total * row; i += blockDim.x) p.o[i] = 0;
     }
     return;
   }
-  Walk<TokenBlocks> w;
-  w.start(p.s, p.blocks, c0 + 1, grid);
-  if (w.by_unit || w.cnt <= 0 || w.tile == 0) return;
-  const int2 own = w.owners(c0 + 1);
-  if (own.x != c0) return;
-  const int r = threadIdx.x % BM, col = threadIdx.x / BM * kMergeCols;
-  const int tok = w.blk * p.blocks.per + g * p.tile_tokens;
-  if (r >= min(p.tile_tokens, w.x.n - tok) * p.group) return;
-  auto slot = [&](int c) { return ((long long)w.place(c, c == c0) * 2 + g) * BM + r; };
+  const int4 a = p.starts[2 * blockIdx.x], b = p.starts[2 * blockIdx.x + 1];
+  const int parts = a.x, h = a.y, tok = a.z + g * p.tile_tokens, tok0 = b.x, n = b.y;
+  const int r = threadIdx.x % BM, col = (blockIdx.z * (kMergeThreads / BM) + threadIdx.x / BM) * kMergeCols;
+  if (r >= min(p.tile_tokens, n - tok) * p.group) return;
   float M = -CUDART_INF_F, L = 0.f, acc[kMergeCols];
 #pragma unroll
   for (int i = 0; i < kMergeCols; ++i) acc[i] = 0.f;
-#pragma unroll 4
-  for (int c = c0; c <= own.y; ++c) M = fmaxf(M, p.ml[slot(c)].x);
-  const float ref = M == -CUDART_INF_F ? 0.f : M;
-#pragma unroll 2
-  for (int c = c0; c <= own.y; ++c) {
-    const float2 y = p.ml[slot(c)];
-    const float wt = ex2(y.x - ref);
-    L = fmaf(wt, y.y, L);
-    const float4* src = p.part + (slot(c) - r) * (D / 4) + (col / 4) * BM + r;
+  for (int c = 0; c < parts; c += 4) {
+    float2 y[4];
+    float4 v[4][kMergeCols / 4];
 #pragma unroll
-    for (int i = 0; i < kMergeCols / 4; ++i) {
-      const float4 v = src[i * BM];
-      acc[4 * i] = fmaf(wt, v.x, acc[4 * i]);
-      acc[4 * i + 1] = fmaf(wt, v.y, acc[4 * i + 1]);
-      acc[4 * i + 2] = fmaf(wt, v.z, acc[4 * i + 2]);
-      acc[4 * i + 3] = fmaf(wt, v.w, acc[4 * i + 3]);
+    for (int k = 0; k < 4; ++k) {
+      const long long slot = (long long)(2 * (c0 + c + k) + (c + k == 0)) * 2 + g;
+      if (c + k < parts) {
+        y[k] = p.ml[slot * BM + r];
+#pragma unroll
+        for (int i = 0; i < kMergeCols / 4; ++i) v[k][i] = p.part[slot * (D / 4) * BM + (col / 4 + i) * BM + r];
+      } else {
+        y[k] = make_float2(-CUDART_INF_F, 0.f);
+#pragma unroll
+        for (int i = 0; i < kMergeCols / 4; ++i) v[k][i] = make_float4(0.f, 0.f, 0.f, 0.f);
+      }
+    }
+    const float m = fmaxf(fmaxf(fmaxf(y[0].x, y[1].x), fmaxf(y[2].x, y[3].x)), M);
+    const float ref = m == -CUDART_INF_F ? 0.f : m, old = ex2(M - ref);
+    M = m;
+    L *= old;
+#pragma unroll
+    for (int i = 0; i < kMergeCols; ++i) acc[i] *= old;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const float wt = ex2(y[k].x - ref);
+      L = fmaf(wt, y[k].y, L);
+#pragma unroll
+      for (int i = 0; i < kMergeCols / 4; ++i) {
+        acc[4 * i] = fmaf(wt, v[k][i].x, acc[4 * i]);
+        acc[4 * i + 1] = fmaf(wt, v[k][i].y, acc[4 * i + 1]);
+        acc[4 * i + 2] = fmaf(wt, v[k][i].z, acc[4 * i + 2]);
+        acc[4 * i + 3] = fmaf(wt, v[k][i].w, acc[4 * i + 3]);
+      }
     }
   }
+  if (parts == 0) return;
   const float inv = M == -CUDART_INF_F ? 0.f : 1.f / L;
   const int t = r / p.group;
-  uint4* dst = reinterpret_cast<uint4*>(
-      p.o + (((long long)(w.x.tok0 + tok + t) * p.s.heads + w.h) * p.group + (r - t * p.group)) * D + col);
+  uint32_t w[kMergeCols / 2];
 #pragma unroll
-  for (int i = 0; i < kMergeCols / 8; ++i)
-    dst[i] = make_uint4(pack2<BF16>(acc[8 * i] * inv, acc[8 * i + 1] * inv), pack2<BF16>(acc[8 * i + 2] * inv, acc[8 * i + 3] * inv),
-                        pack2<BF16>(acc[8 * i + 4] * inv, acc[8 * i + 5] * inv), pack2<BF16>(acc[8 * i + 6] * inv, acc[8 * i + 7] * inv));
+  for (int i = 0; i < kMergeCols / 2; ++i) w[i] = pack2<BF16>(acc[2 * i] * inv, acc[2 * i + 1] * inv);
+  *reinterpret_cast<uint4*>(p.o + (((long long)(tok0 + tok + t) * p.s.heads + h) * p.group + (r - t * p.group)) * D + col) =
+      make_uint4(w[0], w[1], w[2], w[3]);
 }
 
 std::atomic<bool> g_attr[2][2][2][64];
@@ -989,11 +1011,13 @@ cudaError_t launch(const PagedAttnArgs& a, int dev) {
     return cudaErrorInvalidValue;
   const size_t ml_bytes = (size_t)ctas * 4 * BM * sizeof(float2);
   void* block = nullptr;
-  if ((e = scratch_alloc(dev, ml_bytes + (size_t)ctas * 4 * BM * D * sizeof(float), a.stream, &block)) != cudaSuccess) return e;
+  const size_t part_bytes = (size_t)ctas * 4 * BM * D * sizeof(float);
+  if ((e = scratch_alloc(dev, ml_bytes + part_bytes + (size_t)ctas * 2 * sizeof(int4), a.stream, &block)) != cudaSuccess) return e;
   Params p{a.s, TokenBlocks{2 * tile_tokens, a.causal ? 1 : 0, a.s.heads}, a.group, tile_tokens, static_cast<uint16_t*>(a.o),
            (INT8 ? a.scale : fabsf(a.scale)) * 1.4426950408889634f, !INT8 && a.scale < 0.f ? 1 : 0,
            static_cast<const int8_t*>(a.kc), static_cast<const int8_t*>(a.vc), a.ks, a.vs, a.kcs, a.vcs, a.kss, a.vss,
-           reinterpret_cast<float4*>(static_cast<char*>(block) + ml_bytes), static_cast<float2*>(block)};
+           reinterpret_cast<float4*>(static_cast<char*>(block) + ml_bytes), static_cast<float2*>(block),
+           reinterpret_cast<int4*>(static_cast<char*>(block) + ml_bytes + part_bytes)};
   cudaLaunchConfig_t cfg = {};
   cudaLaunchAttribute pdl[1];
   pdl[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -1007,10 +1031,10 @@ cudaError_t launch(const PagedAttnArgs& a, int dev) {
   e = cudaLaunchKernelEx(&cfg, kern, mq, mk, mv, p);
   if (e == cudaSuccess) {
     note_launch();
-    cfg.gridDim = dim3((unsigned)ctas, 2);
-    cfg.blockDim = dim3(BM * D / kMergeCols);
+    cfg.gridDim = dim3((unsigned)ctas, 2, D / (kMergeCols * kMergeThreads / BM));
+    cfg.blockDim = dim3(kMergeThreads);
     cfg.dynamicSmemBytes = 0;
-    if ((e = cudaLaunchKernelEx(&cfg, merge_chunk<D, BF16>, p, ctas)) == cudaSuccess) note_launch();
+    if ((e = cudaLaunchKernelEx(&cfg, merge_chunk<D, BF16>, p)) == cudaSuccess) note_launch();
   }
   if (e == cudaSuccess) e = cudaGetLastError();
   const cudaError_t ef = cudaFreeAsync(block, a.stream);
