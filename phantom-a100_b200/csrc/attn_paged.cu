@@ -56,7 +56,8 @@ struct Cfg {
   static constexpr int BR = 8 * NT;
   static constexpr int ROW = INT8 ? D : 128;              // bytes of a swizzled row (16-bit: 64 columns)
   static constexpr int BLOCKS = INT8 ? 1 : D / 64;        // such blocks across d
-  static constexpr bool WIDE = !INT8 && D == 128 && NT == 1;
+  static constexpr bool WIDE = !INT8 && D == 128;
+  static_assert(INT8 || NT == 1);
   static constexpr int SLOT = (WIDE ? 32 : 16) * 1024, HALF = SLOT / 2;  // a tile: its keys, its values
   static constexpr int BN = HALF / (D * (INT8 ? 1 : 2));  // keys of a tile: 32, 64 or 128
   static constexpr int MT = BN <= 64 || NT == 1 ? BN / 32 : 2;  // 16 MT keys at a time go through a warp
@@ -87,6 +88,7 @@ template <int NT, int BN>
 struct RowBlocks {
   int group, causal, heads;
   static constexpr int kTile = BN, kUnit = 2, BR = 8 * NT;
+  static constexpr float kPart = NT == 1 ? 0.8f : 2.f;
   __device__ int count(const Seq& x) const { return (x.n * group + BR - 1) / BR; }
   __device__ int key_end(const Seq& x, int rb) const {
     if (!causal) return x.len;
@@ -797,18 +799,19 @@ cudaError_t launch(const PagedAttnArgs& a, int dev) {
   return e != cudaSuccess ? e : ef;
 }
 
-template <int D, int NT>
+template <int D, bool INT8, int NT>
 cudaError_t launch_d(const PagedAttnArgs& a, int dev) {
-  return a.int8 ? (a.bf16 ? launch<D, true, true, NT>(a, dev) : launch<D, false, true, NT>(a, dev))
-                : (a.bf16 ? launch<D, true, false, NT>(a, dev) : launch<D, false, false, NT>(a, dev));
+  return a.bf16 ? launch<D, true, INT8, NT>(a, dev) : launch<D, false, INT8, NT>(a, dev);
 }
 
 }  // namespace rows
 
+// Units of 16 rows for 9 to 16 of them; with a 16-bit cache the chunk kernel has those (capi.cu).
 cudaError_t launch_paged_attn_rows(const PagedAttnArgs& a, int dev, int rows) {
-  using namespace rows;
-  if (rows <= 8) return a.d == 64 ? launch_d<64, 1>(a, dev) : launch_d<128, 1>(a, dev);
-  return a.d == 64 ? launch_d<64, 2>(a, dev) : launch_d<128, 2>(a, dev);
+  using namespace phantom::rows;
+  if (!a.int8) return a.d == 64 ? launch_d<64, false, 1>(a, dev) : launch_d<128, false, 1>(a, dev);
+  if (a.d == 64) return rows <= 8 ? launch_d<64, true, 1>(a, dev) : launch_d<64, true, 2>(a, dev);
+  return rows <= 8 ? launch_d<128, true, 1>(a, dev) : launch_d<128, true, 2>(a, dev);
 }
 
 }  // namespace phantom

@@ -73,6 +73,7 @@ struct Cfg {
 struct TokenBlocks {
   int per, causal, heads;
   static constexpr int kTile = BN, kUnit = 4;
+  static constexpr float kPart = 0.1f;
   __device__ int count(const Seq& x) const { return (x.n + per - 1) / per; }
   __device__ int key_end(const Seq& x, int blk) const {
     return causal ? min(max(x.len - x.n + min(x.n, (blk + 1) * per), 0), x.len) : x.len;

@@ -472,10 +472,12 @@ int phantom_attn_paged(const phantom_paged_cache* cache, const void* q, long lon
   a.causal = causal != 0;
   a.scale = scale != 0.f ? scale : 1.f / sqrtf((float)cache->head_dim);
   a.stream = static_cast<cudaStream_t>(stream);
-  // Query rows of one key head in one sequence, as expected: up to one 16-row block the rows kernel reads the keys once
-  // and is bound by that; above, its blocks would each read them, and the chunk kernel takes up to 256 rows at a time.
+  // Query rows of one key head in one sequence, as expected: few go to the rows kernel, which is bound by the keys it reads,
+  // more to the chunk kernel, which takes up to 256 at a time. Measured (us, rows / chunk; 32 contexts of 200-4096, 8 key
+  // heads): 16-bit, d = 128: 4 rows 56 / 71, 16 rows 86 / 70; d = 64: 16 rows 60 / 58. 8-bit, where the chunk kernel is
+  // slower: 16 rows 76 / 117, 32 rows (8 of 4000) 95 / 58.
   const long long new_tokens = max_new > 0 ? max_new : (total_new + cache->batch - 1) / cache->batch;
-  const bool few = new_tokens * a.group <= 16;
+  const bool few = new_tokens * a.group <= (a.int8 ? 16 : 8);
   const cudaError_t e = few ? launch_paged_attn_rows(a, dev.id, (int)std::min(new_tokens * a.group, 1LL << 30)) : launch_paged_attn_chunk(a, dev.id);
   if (e != cudaSuccess) return cuda_fail(name, e);
   g_last_error.clear();

@@ -50,7 +50,7 @@ __device__ __forceinline__ int seq_index(const PagedSeqs& s, int tok) {
 // `Blocks` says how the rows are cut: kTile keys to a tile; count(x) blocks; the keys key_end(x, blk) that a block sees;
 // head_tiles(x) tiles in all of one head. A unit costs something besides its tiles (its queries, its output, the start of
 // its pipeline), as much as kUnit tiles; these are counted before its first one when the shares are cut, and a share that
-// ends among them has nothing of the unit.
+// ends among them has nothing of the unit. Joining a part of a shared unit takes as long as kPart tiles.
 
 // At least one tile, so that rows without any key are written too (as zeros).
 template <typename Blocks>
@@ -116,7 +116,10 @@ struct Walk {
       units += __shfl_xor_sync(0xffffffffu, units, m);
       most = max(most, __shfl_xor_sync(0xffffffffu, most, m));
     }
-    ctas = (int)min((long long)grid, total);
+    // No smaller shares than pay: with s tiles to a share the longest unit takes as long as s tiles and most / s parts to
+    // join, kPart tiles each, least where s^2 = kPart most.
+    const long long least = max(1LL, (long long)sqrtf(Blocks::kPart * (float)most));
+    ctas = (int)min((long long)grid, quotient(total + least - 1, least));
     share = ctas > 0 ? quotient(total, ctas) : 0;
     more = (int)(total - share * ctas);
     by_unit = units <= grid && most + kUnit <= share + kJoinTiles;
