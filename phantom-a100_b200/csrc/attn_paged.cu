@@ -46,7 +46,8 @@ constexpr int kJoiners = 4;
 constexpr int kUnitRing = 4;
 constexpr int kErrCopyWait = 1, kErrTileWait = 4, kErrJoinWait = 8;
 
-// Warps: eight consumers, in pairs that take the tiles in turn; the joiners; four producers. Registers (setmaxnreg, by
+// Warps: eight consumers, in pairs that take the tiles in turn; the joiners; two producers and two
+// idle warps that complete their warpgroup. Registers (setmaxnreg, by
 // warpgroup): 512 threads launch with 128 each; 2 * 168 + 104 + 72 = 4 * 128.
 constexpr int kConsumers = 8, PRODUCER = kConsumers + kJoiners, kThreads = 32 * (PRODUCER + 4);
 constexpr int kRegsConsumer = 168, kRegsJoiner = 104, kRegsProducer = 72;
@@ -66,15 +67,12 @@ struct Cfg {
   // which so sees every phase of its barriers. (With a slot passed between pairs, a pair could wait for a phase whose
   // predecessor was still open, and parity would let it by.)
   static constexpr int PAIRS = WIDE ? 3 : 4, WARPS = 2 * PAIRS, SLOTS = 2 * PAIRS;
-  // producers of a tile: keys, values, and an 8-bit cache's scales of each
-  static constexpr int PRODUCERS = INT8 ? 4 : 2;
   static constexpr int OFF_MERGE = SLOTS * SLOT;          // [WARPS][BR][D] fp32
   static constexpr int OFF_ML = OFF_MERGE + WARPS * BR * D * 4;
   static constexpr int Q_ROW = 2 * D + 16;                // padded: lanes of 8 rows and 4 words read without conflicts
   static constexpr int OFF_Q = OFF_ML + WARPS * BR * 8;
-  static constexpr int OFF_SCALE = OFF_Q + kUnitRing * BR * Q_ROW;
-  static constexpr int OFF_IDS = OFF_SCALE + (INT8 ? SLOTS * 2 * BN * 4 : 0);  // page ids, 64 to each producer
-  static constexpr int OFF_UNIT = OFF_IDS + PRODUCERS * 64 * 4;
+  static constexpr int OFF_IDS = OFF_Q + kUnitRing * BR * Q_ROW;  // page ids, 64 to each producer
+  static constexpr int OFF_UNIT = OFF_IDS + 2 * 64 * 4;
   static constexpr int OFF_BAR = OFF_UNIT + kUnitRing * 48;
   static constexpr int OFF_FLAG = OFF_BAR + (2 * SLOTS + 2 * kUnitRing + 2) * 8;
   static constexpr int SMEM = OFF_FLAG + 16 + 1024;       // + slack to align the base
@@ -154,7 +152,7 @@ __device__ __forceinline__ uint32_t turn(uint32_t x) {
 struct Unit {
   int cnt, tile0, end, id;    // its tiles here, the first of them; the keys that its rows see; id -1 ends the roles
   int len, n, row0, tok0;     // the sequence: cached and new tokens; the unit's first row; packed place of its first token
-  int h, c0, c1, pad;         // key head; the first and the last CTA that have tiles of it
+  int h, c0, c1, b;           // key head; the first and the last CTA that have tiles of it; the sequence
 };
 
 template <int D, bool BF16, bool INT8, int NT>
@@ -180,7 +178,7 @@ attn_rows(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUten
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < C::SLOTS; ++s) {
-      mbar_init(full(s), C::PRODUCERS);
+      mbar_init(full(s), 2);   // the producers
       mbar_init(empty(s), 2);  // the consuming pair
     }
     for (int u = 0; u < kUnitRing; ++u) {
@@ -208,7 +206,7 @@ attn_rows(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUten
       const int4 a = r[0], b = r[1], c = r[2];
       x.cnt = a.x, x.tile0 = a.y, x.end = a.z, x.id = a.w;
       x.len = b.x, x.n = b.y, x.row0 = b.z, x.tok0 = b.w;
-      x.h = c.x, x.c0 = c.y, x.c1 = c.z;
+      x.h = c.x, x.c0 = c.y, x.c1 = c.z, x.b = c.w;
     }
     return x;
   };
@@ -216,24 +214,21 @@ attn_rows(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUten
   if (warp >= PRODUCER) {
     setmaxnreg_dec<kRegsProducer>();
     const int role = warp - PRODUCER;
-    if (role >= C::PRODUCERS) return;
-    // Producers: of the keys (and of the units' records and queries), of the values, and of an 8-bit cache's scales of
-    // each, a copy to a page. Each walks the CTA's share by itself. One elected lane issues the copies, whose issue is what
-    // limits pages of 16 tokens, hence a warp for each kind. Page ids wait in shared memory, 32 pages and more ahead.
+    if (role >= 2) return;
+    // Producers, of the keys (and of the units' records and queries) and of the values, a copy to a page. Each walks the
+    // CTA's share by itself. One elected lane issues the copies, whose issue is what limits pages of 16 tokens, hence a warp
+    // for each. Page ids wait in shared memory.
     const bool vals = role & 1;
     const CUtensorMap* map = vals ? &tmV : &tmK;
-    if (role < 2 && elect_one()) tma_prefetch_desc(map);
+    if (elect_one()) tma_prefetch_desc(map);
     __syncwarp();
     Walk<Blocks> w;
     w.start(p.s, p.blocks, blockIdx.x, gridDim.x);
     int t = 0, nu = 0;
     bool ok = true;
     const int page_log2 = p.s.page_log2, page = 1 << page_log2, box = min(page, BN);
-    const Strides3 st = vals ? p.vss : p.kss;
-    const float* scale = vals ? p.vs : p.ks;
-    const uint32_t bytes = role < 2 ? box * D * (INT8 ? 1 : 2) : box * 4;  // of a copy
-    const uint32_t dst0 = role < 2 ? sbase + role * C::HALF : sbase + C::OFF_SCALE + vals * BN * 4;
-    const uint32_t slot_bytes = role < 2 ? C::SLOT : 2 * BN * 4;
+    const uint32_t bytes = box * D * (INT8 ? 1 : 2);  // of a copy
+    const uint32_t dst0 = sbase + role * C::HALF;
     int* ids = reinterpret_cast<int*>(smem + C::OFF_IDS) + role * 64;  // page i's id at i % 64
     while (w.cnt > 0) {
       const int end = p.blocks.key_end(w.x, w.blk), cnt = w.cnt;
@@ -254,7 +249,7 @@ attn_rows(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUten
           int4* r = ring + 3 * (nu % kUnitRing);
           r[0] = make_int4(cnt, w.tile, end, nu);
           r[1] = make_int4(w.x.len, w.x.n, row0, w.x.tok0);
-          r[2] = make_int4(w.h, own.x, own.y, 0);
+          r[2] = make_int4(w.h, own.x, own.y, w.b);
           mbar_arrive_expect_tx(q_full(nu), rows * D * 2);
         }
         __syncwarp();
@@ -266,7 +261,6 @@ attn_rows(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUten
         __syncwarp();
         ++nu;
       }
-      const float* head_scale = scale + w.h * st.head;
       for (int i = 0; i < cnt; ++i, ++t) {
         const int s = t % C::SLOTS, round = t / C::SLOTS;
         const int j0 = (w.tile + i) * BN, place = j0 & (page - 1), first = j0 >> page_log2;
@@ -274,14 +268,11 @@ attn_rows(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUten
         if (round > 0 && !(ok = wait(empty(s), (round - 1) & 1, kErrCopyWait))) break;
         if (elect_one()) {
           mbar_arrive_expect_tx(full(s), boxes * bytes);
-          uint32_t dst = dst0 + s * slot_bytes;
+          uint32_t dst = dst0 + s * C::SLOT;
 #pragma unroll 1
           for (int pg = 0; pg < boxes; ++pg, dst += bytes) {
-            const int from = ids[(first + pg) & 63];
-            if (role < 2)  // an id that is out of range reads as zeros (the map's bounds)
-              tma_load_5d(dst, map, full(s), 0, place, 0, w.h, from);
-            else
-              bulk_load(dst, head_scale + max(from, 0) * st.page + place, bytes, full(s));
+            const int from = ids[(first + pg) & 63];  // one that is out of range reads as zeros (the map's bounds)
+            tma_load_5d(dst, map, full(s), 0, place, 0, w.h, from);
           }
         }
         __syncwarp();
@@ -476,6 +467,7 @@ attn_rows(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUten
   const int box_log2 = min(p.s.page_log2, BN == 32 ? 5 : BN == 64 ? 6 : 7), blk_stride = C::ROW << box_log2;
   constexpr int AT = C::BLOCKS == 1 ? 1 : MT;  // one column block: 16 rows further on is a constant away
   static_assert(C::SUB == 1 || C::BLOCKS == 1);
+  static_assert(!INT8 || (BN / 2 == 32 || BN / 2 == 64) && (C::SUB == 1 || (C::SUB == 2 && KEYS == 32)));
   uint32_t at_k[AT], at_v[AT];
 #pragma unroll
   for (int mt = 0; mt < AT; ++mt) {
@@ -531,9 +523,48 @@ attn_rows(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUten
     }
 
     bool ok = true;
+    // 8-bit: the scales of this warp's keys, a lane each (and a lane's second key 32 further on), are read one tile ahead,
+    // their pages' ids while the tile before is waited for and the scales after its first product.
+    constexpr int NQ = INT8 ? BN / 64 : 1;
+    int ids[NQ];
+    float ks[NQ], vs[NQ];
+    auto read_ids = [&](int i) {
+#pragma unroll
+      for (int q = 0; q < NQ; ++q) {
+        const int j = (x.tile0 + i) * BN + kr + 32 * q + lane;
+        ids[q] = j < x.end ? page_of(p.s, x.b, j >> p.s.page_log2) : -1;
+      }
+    };
+    auto read_scales = [&](int i) {
+#pragma unroll
+      for (int q = 0; q < NQ; ++q) {
+        const int place = ((x.tile0 + i) * BN + kr + 32 * q + lane) & ((1 << p.s.page_log2) - 1);
+        ks[q] = vs[q] = 0.f;
+        if (ids[q] >= 0) {
+          ks[q] = p.ks[ids[q] * p.kss.page + x.h * p.kss.head + place];
+          vs[q] = p.vs[ids[q] * p.vss.page + x.h * p.vss.head + place];
+        }
+      }
+    };
+    if (INT8 && first < x.cnt) {
+      read_ids(first);
+      read_scales(first);
+    }
     for (int i = first; i < x.cnt; i += C::PAIRS) {  // tiles of the whole share go to the pairs in turn
       const int s = (t + i) % C::SLOTS;
       if (!(ok = wait(full(s), ((t + i) / C::SLOTS) & 1, kErrTileWait))) break;
+      float ksl[NQ], lvs[NQ], ivs[NQ];  // the key's scale, log2 of the value's, its reciprocal (no effect past the end)
+      if constexpr (INT8) {
+#pragma unroll
+        for (int q = 0; q < NQ; ++q) {
+          const bool in = (x.tile0 + i) * BN + kr + 32 * q + lane < x.end;
+          const float v = least_scale(vs[q]);
+          ksl[q] = ks[q] * p.scale_log2;
+          lvs[q] = in ? __log2f(v) : 0.f;
+          ivs[q] = in ? __fdividef(1.f, v) : 0.f;
+        }
+        if (i + C::PAIRS < x.cnt) read_ids(i + C::PAIRS);
+      }
 #pragma unroll 1
       for (int sub_i = 0; sub_i < C::SUB; ++sub_i) {
         const uint32_t kb = sbase + s * C::SLOT + sub_i * KEYS * C::ROW, vb = kb + C::HALF;
@@ -580,15 +611,17 @@ attn_rows(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUten
         // ---- 8-bit: to the log2 domain, with the values' scales; masks
         float inv_vs[MT][2];
         if constexpr (INT8) {
-          const float* scl = reinterpret_cast<const float*>(smem + C::OFF_SCALE + s * 2 * BN * 4) + kr + sub_i * KEYS + g;
+          if (sub_i == C::SUB - 1 && i + C::PAIRS < x.cnt) read_scales(i + C::PAIRS);
 #pragma unroll
           for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
-              const float a = scl[mt * 16 + e * 8] * p.scale_log2, v = least_scale(scl[BN + mt * 16 + e * 8]),
-                          lv = __log2f(v);
-              // past the end a scale may be anything; p' is 0 there
-              inv_vs[mt][e] = j0 + mt * 16 + e * 8 + g < end ? __fdividef(1.f, v) : 0.f;
+              const int from = ((mt * 16 + e * 8) & 31) + g;
+              auto of_key = [&](const float (&r)[NQ]) {
+                return __shfl_sync(0xffffffffu, C::SUB == 1 ? r[mt >> 1] : r[C::SUB > 1 && sub_i > 0 ? NQ - 1 : 0], from);
+              };
+              const float a = of_key(ksl), lv = of_key(lvs);
+              inv_vs[mt][e] = of_key(ivs);
 #pragma unroll
               for (int nt = 0; nt < NT; ++nt) {
                 sc[mt][nt][2 * e] = fmaf(sc[mt][nt][2 * e], a, lv);
