@@ -251,8 +251,8 @@ int phantom_attn_paged_read(const phantom_paged_cache* cache, void* k, void* v, 
  * PHANTOM_ATTN_I8. Query head h reads key head h / (q_heads / heads). New token i of n sees the first kv_len - n + i + 1
  * tokens of its sequence if causal, all of them otherwise; a token that sees none gets zeros. Scores are multiplied by
  * scale (0: 1 / sqrt(head_dim)). max_new is the largest number of new tokens of a sequence, as the caller expects it: a
- * hint that picks the kernel, not a limit (0: the average). Values cached within the length must be finite even where the
- * causal mask hides them; what lies past the length may be anything. */
+ * hint that picks the kernel, not a limit (0: the average). 16-bit values cached within the length must be finite even
+ * where the causal mask hides them; what lies past the length may be anything. */
 int phantom_attn_paged(const phantom_paged_cache* cache, const void* q, long long q_token, long long q_head, void* o,
                        int total_new, int q_heads, int dtype, int causal, float scale, int max_new, void* stream);
 

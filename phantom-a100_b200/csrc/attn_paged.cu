@@ -10,24 +10,26 @@
 //   * Queries are the narrow operand. The matrix instruction takes 16 keys by 16 of d from shared memory against 8 query
 //     rows (new tokens x query heads of one key head, token-major) held in registers: scores come out as keys x queries,
 //     are turned around by movmatrix, and meet V^T the same way. With queries as the 16-high operand a group of 4 or 8
-//     heads left half of every instruction and of the softmax unused (16 contexts of 4096 tokens, 8 key heads: 812
-//     instructions for each 32 keys and warp, against 310).
-//   * Work is cut evenly: all (sequence, head, row block) units in a row, tiles of 64 keys, and every CTA takes its share
+//     heads left half of every instruction and of the softmax unused (812 instructions for 32 keys of a key head, all roles
+//     counted, against 610).
+//   * Work is cut evenly: all (sequence, head, row block) units in a row, tiles of 64 or 128 keys, and every CTA takes its share
 //     (paged_dev.cuh). Ragged lengths then cost nothing, and one long sequence spreads over the GPU. The parts of a unit
 //     that several CTAs share (fp32 rows, reference maximum, sum) are joined in the order of the CTAs by the one that
 //     finishes last: the result depends on the lengths and the GPU's SM count alone.
 //   * Two producer warps read the page table and keep a ring of tiles in flight by TMA (a box per page, swizzled, so that
 //     pages of 16 tokens land as one conflict-free tile), two tiles to each pair of consumer warps.
-//   * Eight consumer warps work without meeting: two to a tile, 32 keys each, every warp with its own running maximum,
-//     sum and output. At the end of a unit they leave these in shared memory and go on to the next, whose queries a
-//     producer has brought there; four further warps join and write them. (With the consumers doing this themselves a
-//     unit cost them 3.9 us besides its tiles.)
+//   * Six or eight consumer warps work without meeting: two to a tile, half of its keys each, every warp with its own
+//     running maximum, sum and output. At the end of a unit they leave these in shared memory and go on to the next, whose
+//     queries a producer has brought there; four further warps join and write them. (With the consumers doing this
+//     themselves a unit cost them 3.9 us besides its tiles.)
 //
 // Precision: scores and sums are fp32. 16-bit caches: P enters the second product as hi + lo (two 16-bit numbers), so its
 // rounding (which alone would be as large as the output's) is gone; the tensor cores idle here and the second product is
-// free. 8-bit caches: keys and values enter as the whole numbers they are (exact in fp16, and in bf16), the key's scale
-// multiplies the score, and the value's goes into the exponent: p'_j = 2^(s_j + log2 vs_j - m') is p_j vs_j normalised to
-// at most 1, whatever the scales, and is rounded to fp16 once; the sum adds p'_j / vs_j.
+// free. 8-bit caches: keys and values enter as the whole numbers they are, exact in fp16. bf16 queries turn into fp16 with
+// a power of two for each row, exact but for what is below 2^-31 of the row's largest: fp16's 10 bits take a byte as it is,
+// where bf16 needs a subtraction for each (contexts of 2000 to 16383 tokens, pages of 64: 60.6 us, and 62.7 in bf16). The
+// key's scale multiplies the score, and the value's goes into the exponent: p'_j = 2^(s_j + log2 vs_j - m') is p_j vs_j
+// normalised to at most 1, whatever the scales, and is rounded to fp16 once; the sum adds p'_j / vs_j.
 #include <cuda.h>
 #include <math_constants.h>
 
@@ -46,9 +48,8 @@ constexpr int kJoiners = 4;
 constexpr int kUnitRing = 4;
 constexpr int kErrCopyWait = 1, kErrTileWait = 4, kErrJoinWait = 8;
 
-// Warps: eight consumers, in pairs that take the tiles in turn; the joiners; two producers and two
-// idle warps that complete their warpgroup. Registers (setmaxnreg, by
-// warpgroup): 512 threads launch with 128 each; 2 * 168 + 104 + 72 = 4 * 128.
+// Warps: eight consumers, in pairs that take the tiles in turn; the joiners; two producers and two idle warps that complete
+// their warpgroup. Registers (setmaxnreg, by warpgroup): 512 threads launch with 128 each; 2 * 168 + 104 + 72 = 4 * 128.
 constexpr int kConsumers = 8, PRODUCER = kConsumers + kJoiners, kThreads = 32 * (PRODUCER + 4);
 constexpr int kRegsConsumer = 168, kRegsJoiner = 104, kRegsProducer = 72;
 
@@ -60,7 +61,7 @@ struct Cfg {
   static constexpr bool WIDE = !INT8 && D == 128;
   static_assert(INT8 || NT == 1);
   static constexpr int SLOT = (WIDE ? 32 : 16) * 1024, HALF = SLOT / 2;  // a tile: its keys, its values
-  static constexpr int BN = HALF / (D * (INT8 ? 1 : 2));  // keys of a tile: 32, 64 or 128
+  static constexpr int BN = HALF / (D * (INT8 ? 1 : 2));  // keys of a tile: 64 or 128
   static constexpr int MT = BN <= 64 || NT == 1 ? BN / 32 : 2;  // 16 MT keys at a time go through a warp
   static constexpr int SUB = BN / (32 * MT);              // times
   // Two slots to a pair, so that a pair's next tile is on its way while it works on one. A slot's tiles all go to one pair,
@@ -78,7 +79,6 @@ struct Cfg {
   static constexpr int SMEM = OFF_FLAG + 16 + 1024;       // + slack to align the base
   static_assert(SMEM <= 227 * 1024, "shared memory plan exceeds 227 KB");
 };
-
 
 // ------------------------------------------------------------------------------------------------ units and tiles
 // Units of 8 NT rows; tiles of BN keys.
@@ -305,7 +305,7 @@ attn_rows(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUten
   float2* ml = reinterpret_cast<float2*>(smem + C::OFF_ML);
   if (warp >= kConsumers) {
     setmaxnreg_dec<kRegsJoiner>();
-    // Joiners: a unit's rows from the eight warps' sums, to the output or to the parts of a shared unit.
+    // Joiners: a unit's rows from the consumers' sums, to the output or to the parts of a shared unit.
     constexpr int PER = BR * D / 128;  // columns of a thread: 16, 8 or 4
     const int tid = threadIdx.x - 32 * kConsumers;
     const int r = tid / (128 / BR), col = (tid % (128 / BR)) * PER;
@@ -365,7 +365,7 @@ attn_rows(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUten
         joiners_meet();
         done = *joined != 0;
         if (done) {
-          // Warp v takes every fourth part, all rows of it at once (32 lanes to a row), and the four sums meet in shared memory.
+          // Warp v takes every fourth part, four rows of it at once (32 lanes to a row); the four sums meet in shared memory.
           const int parts = x.c1 - x.c0 + 1, rows = min(BR, x.n * group - x.row0);
           const int v = warp - kConsumers;
           constexpr int W = D / 32;  // columns of a lane
@@ -460,11 +460,11 @@ attn_rows(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUten
   const int pair = warp >> 1;
   constexpr int KEYS = 16 * MT;  // that go through this warp at a time
   const int kr = (warp & 1) * (BN / 2);  // its first key of its pair's tiles
-  // Where this lane's rows for ldmatrix lie in a tile: 16 keys from kr + KEYS sub + 16 mt, matrices (keys 0-7, 8-15) x (first, second
-  // 16-byte chunk of a pair); V^T of 16-bit values has the two the other way around. Boxes of min(page, 64) tokens, each
+  // Where this lane's rows for ldmatrix lie in a tile: 16 keys from kr + KEYS sub + 16 mt, matrices (keys 0-7, 8-15) x
+  // (first, second 16-byte chunk of a pair); V^T of 16-bit values has the two the other way around. Boxes of min(page, 64) tokens, each
   // [64-column block][token][ROW bytes]; a chunk lies at its number ^ the row's swizzle, so stepping over pairs of chunks
   // is an XOR with 32 times the pair's number.
-  const int box_log2 = min(p.s.page_log2, BN == 32 ? 5 : BN == 64 ? 6 : 7), blk_stride = C::ROW << box_log2;
+  const int box_log2 = min(p.s.page_log2, BN == 64 ? 6 : 7), blk_stride = C::ROW << box_log2;
   constexpr int AT = C::BLOCKS == 1 ? 1 : MT;  // one column block: 16 rows further on is a constant away
   static_assert(C::SUB == 1 || C::BLOCKS == 1);
   static_assert(!INT8 || (BN / 2 == 32 || BN / 2 == 64) && (C::SUB == 1 || (C::SUB == 2 && KEYS == 32)));
@@ -490,6 +490,7 @@ attn_rows(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUten
     // numbers meet another's.)
     uint32_t qb[NT][D / 16][2];
     int lim[NT][2];
+    float q_back[NT][2];  // 8-bit caches, bf16: of the rows of this lane's scores, what their queries were divided by
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
       const uint8_t* src = smem + C::OFF_Q + ((u % kUnitRing) * BR + nt * 8 + g) * C::Q_ROW;
@@ -503,6 +504,25 @@ attn_rows(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUten
           qb[nt][k][0] = *reinterpret_cast<const uint32_t*>(src + k * 32 + 4 * t4) ^ p.flip;
           qb[nt][k][1] = *reinterpret_cast<const uint32_t*>(src + k * 32 + 16 + 4 * t4) ^ p.flip;
         }
+      }
+      if constexpr (INT8 && BF16) {
+        // to fp16, times the power of two that brings the row's largest to [2^14, 2^15)
+        uint32_t big = 0;
+#pragma unroll
+        for (int k = 0; k < D / 16; ++k) big = __vmaxu2(big, __vmaxu2(qb[nt][k][0] & 0x7FFF7FFFu, qb[nt][k][1] & 0x7FFF7FFFu));
+        big = __vmaxu2(big, __shfl_xor_sync(0xffffffffu, big, 1));
+        big = __vmaxu2(big, __shfl_xor_sync(0xffffffffu, big, 2));
+        const int ex = max((int)(max(big & 0xFFFFu, big >> 16) >> 7) - 127, -111);
+        const float f = __uint_as_float((uint32_t)(141 - ex) << 23), back = __uint_as_float((uint32_t)(113 + ex) << 23);
+#pragma unroll
+        for (int k = 0; k < D / 16; ++k)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const uint32_t y = qb[nt][k][e];
+            qb[nt][k][e] = pack2<false>(__uint_as_float(y << 16) * f, __uint_as_float(y & 0xFFFF0000u) * f);
+          }
+#pragma unroll
+        for (int e = 0; e < 2; ++e) q_back[nt][e] = __shfl_sync(0xffffffffu, back, (2 * t4 + e) * 4);
       }
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
@@ -561,7 +581,7 @@ attn_rows(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUten
           const float v = least_scale(vs[q]);
           ksl[q] = ks[q] * p.scale_log2;
           lvs[q] = in ? __log2f(v) : 0.f;
-          ivs[q] = in ? __fdividef(1.f, v) : 0.f;
+          ivs[q] = in && v == v ? __fdividef(1.f, v) : 0.f;  // (NaN: the logarithm alone passes it on, to rows that see it)
         }
         if (i + C::PAIRS < x.cnt) read_ids(i + C::PAIRS);
       }
@@ -583,19 +603,14 @@ attn_rows(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUten
               ldsm4(kb + mt * 16 * C::ROW + (at_k[0] ^ (k << 5)), r);
 #pragma unroll
               for (int e = 0; e < 4; ++e) {  // r: (keys 0-7, 8-15) of chunk 2 k, then of 2 k + 1
-                if constexpr (BF16) {
-                  a[e >> 1][e & 1] = bytes_bf16<0x4140>(r[e]);
-                  a[e >> 1][2 + (e & 1)] = bytes_bf16<0x4342>(r[e]);
-                } else {
-                  const uint32_t u = r[e] ^ 0x80808080u;
-                  a[e >> 1][e & 1] = bytes_f16<0x4140>(u);
-                  a[e >> 1][2 + (e & 1)] = bytes_f16<0x4342>(u);
-                }
+                const uint32_t u = r[e] ^ 0x80808080u;
+                a[e >> 1][e & 1] = bytes_f16<0x4140>(u);
+                a[e >> 1][2 + (e & 1)] = bytes_f16<0x4342>(u);
               }
 #pragma unroll
               for (int nt = 0; nt < NT; ++nt) {
-                mma16816<BF16>(sc[mt][nt], a[0], qb[nt][2 * k][0], qb[nt][2 * k][1]);
-                mma16816<BF16>(sc[mt][nt], a[1], qb[nt][2 * k + 1][0], qb[nt][2 * k + 1][1]);
+                mma16816<false>(sc[mt][nt], a[0], qb[nt][2 * k][0], qb[nt][2 * k][1]);
+                mma16816<false>(sc[mt][nt], a[1], qb[nt][2 * k + 1][0], qb[nt][2 * k + 1][1]);
               }
             }
           } else {
@@ -624,8 +639,8 @@ attn_rows(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUten
               inv_vs[mt][e] = of_key(ivs);
 #pragma unroll
               for (int nt = 0; nt < NT; ++nt) {
-                sc[mt][nt][2 * e] = fmaf(sc[mt][nt][2 * e], a, lv);
-                sc[mt][nt][2 * e + 1] = fmaf(sc[mt][nt][2 * e + 1], a, lv);
+                sc[mt][nt][2 * e] = fmaf(sc[mt][nt][2 * e], BF16 ? a * q_back[nt][0] : a, lv);
+                sc[mt][nt][2 * e + 1] = fmaf(sc[mt][nt][2 * e + 1], BF16 ? a * q_back[nt][1] : a, lv);
               }
             }
         }

@@ -493,7 +493,7 @@ attn_chunk(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUte
       vs = least_scale(vs);
       scl[(tid & ~1) * 2 + (tid & 1)] = ks * p.scale_log2;  // of a pair of keys: two of these, then two of those
       scl[(tid & ~1) * 2 + (tid & 1) + 2] = past ? 0.f : __log2f(vs);
-      scl[2 * BN + tid] = past ? 0.f : __fdividef(1.f, vs);
+      scl[2 * BN + tid] = past || vs != vs ? 0.f : __fdividef(1.f, vs);  // (NaN: only the logarithm passes it on)
       __syncwarp();
       if (lane == 0) mbar_arrive(sc_full(j));
       // -- keys; the values' bytes take their place

@@ -53,7 +53,8 @@ def paged_attn(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, pa
     their keys and values first). Query head h reads key head h // (query heads / heads); new token i of n sees the first
     kv_lens[b] - n + i + 1 tokens if causal, else all kv_lens[b]; one that sees none gets zeros. `scale` of the scores: 1 /
     sqrt(d) by default. `max_new`: the largest number of new tokens of a sequence, a hint that picks the kernel and changes
-    nothing else (default: the average)."""
+    nothing else (default: the average). 16-bit values within kv_lens[b] must be finite, those that the causal mask hides
+    too; what the pages hold past it may be anything."""
     if scale is not None and not 0.0 < abs(scale) < float("inf"):
         raise RuntimeError(f"paged_attn: scale must be finite and not zero (got {scale})")
     return _ext().paged_attn(q, k_cache, v_cache, page_table, kv_lens, cu_new, k_scale, v_scale, causal, max_new,

@@ -143,6 +143,35 @@ def test_vectors_of_very_different_scales():
         check(c, True, hint)
 
 
+@pytest.mark.parametrize("hint", [1, 4096], ids=["rows", "chunk"])
+def test_zero_scales_and_zero_queries(hint):
+    """8-bit caches of other writers: vectors of zeros with the scale 0 count in the sum of weights; and queries of zeros or
+    of very different sizes."""
+    c = Case([3], [500], 1, 4, 64, 16, BF16, True, seed=4)
+    ids, place = c.places(0, 500)
+    for cache, scale, held in ((c.k_cache, c.k_scale, c.keys), (c.v_cache, c.v_scale, c.values)):
+        cache[ids[::5], :, place[::5]] = 0
+        scale[ids[::5], :, place[::5]] = 0.0
+        held[0][::5] = 0.0
+    c.q[0, 1] = 0
+    c.q[1] *= 2.0 ** -100
+    c.q[2, 2, 7] = 300.0
+    check(c, True, hint)
+
+
+@pytest.mark.parametrize("hint", [1, 4096], ids=["rows", "chunk"])
+def test_only_rows_that_see_a_nan_turn_nan(hint):
+    """8-bit caches: a vector with a NaN was appended as the last but one of the new tokens."""
+    for scales in ("k_scale", "v_scale"):
+        c = Case([5], [300], 2, 2, 128, 16, F16, True)
+        clean = attend(c, True, hint)
+        ids, place = c.places(0, 300)
+        getattr(c, scales)[ids[298], 0, place[298]] = float("nan")
+        out = attend(c, True, hint)
+        assert out[3:, :2].isnan().all()
+        assert torch.equal(out[:3], clean[:3]) and torch.equal(out[:, 2:], clean[:, 2:])
+
+
 def test_results_repeat_bit_for_bit():
     for int8 in (False, True):
         for hint in (1, 4096):
