@@ -16,7 +16,7 @@
 //     (paged_dev.cuh). Ragged lengths then cost nothing, and one long sequence spreads over the GPU. The parts of a unit
 //     that several CTAs share (fp32 rows, reference maximum, sum) are joined in the order of the CTAs by the one that
 //     finishes last: the result depends on the lengths and the GPU's SM count alone.
-//   * Two producer warps read the page table and keep a ring of tiles in flight by TMA (a box per page, swizzled, so that
+//   * Producer warps for keys and for values read the page table and keep a ring of tiles in flight by TMA (a box per page, swizzled, so that
 //     pages of 16 tokens land as one conflict-free tile), two tiles to each pair of consumer warps.
 //   * Six or eight consumer warps work without meeting: two to a tile, half of its keys each, every warp with its own
 //     running maximum, sum and output. At the end of a unit they leave these in shared memory and go on to the next, whose
@@ -48,7 +48,7 @@ constexpr int kJoiners = 4;
 constexpr int kUnitRing = 4;
 constexpr int kErrCopyWait = 1, kErrTileWait = 4, kErrJoinWait = 8;
 
-// Warps: eight consumers, in pairs that take the tiles in turn; the joiners; two producers and two idle warps that complete
+// Warps: eight consumers, in pairs that take the tiles in turn; the joiners; three producers and an idle warp that completes
 // their warpgroup. Registers (setmaxnreg, by warpgroup): 512 threads launch with 128 each; 2 * 168 + 104 + 72 = 4 * 128.
 constexpr int kConsumers = 8, PRODUCER = kConsumers + kJoiners, kThreads = 32 * (PRODUCER + 4);
 constexpr int kRegsConsumer = 168, kRegsJoiner = 104, kRegsProducer = 72;
@@ -109,7 +109,7 @@ struct Params {
   uint32_t flip;     // sign bits to flip in the queries (a negative scale)
   float* part;       // parts of shared units, [place][8 NT] rows of D sums of values
   float2* ml;        // their (reference maximum, sum)
-  unsigned long long* flags;
+  unsigned long long* words;  // of shared units, at the number of their first CTA
   unsigned long long call;
 };
 
@@ -148,7 +148,7 @@ __device__ __forceinline__ uint32_t turn(uint32_t x) {
   return y;
 }
 
-// What the key producer tells the others of a unit (48 bytes).
+// What the records' producer tells the others of a unit (48 bytes).
 struct Unit {
   int cnt, tile0, end, id;    // its tiles here, the first of them; the keys that its rows see; id -1 ends the roles
   int len, n, row0, tok0;     // the sequence: cached and new tokens; the unit's first row; packed place of its first token
@@ -214,18 +214,53 @@ attn_rows(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUten
   if (warp >= PRODUCER) {
     setmaxnreg_dec<kRegsProducer>();
     const int role = warp - PRODUCER;
-    if (role >= 2) return;
-    // Producers, of the keys (and of the units' records and queries) and of the values, a copy to a page. Each walks the
-    // CTA's share by itself. One elected lane issues the copies, whose issue is what limits pages of 16 tokens, hence a warp
-    // for each. Page ids wait in shared memory.
-    const bool vals = role & 1;
-    const CUtensorMap* map = vals ? &tmV : &tmK;
-    if (elect_one()) tma_prefetch_desc(map);
+    if (role > 2) return;
+    // Producers, of the keys, of the values, and of the units' records and queries. Each walks the CTA's share by itself.
+    if (role < 2 && elect_one()) tma_prefetch_desc(role ? &tmV : &tmK);
     __syncwarp();
     Walk<Blocks> w;
     w.start(p.s, p.blocks, blockIdx.x, gridDim.x);
-    int t = 0, nu = 0;
     bool ok = true;
+    if (role == 2) {
+      int nu = 0;
+      for (; w.cnt > 0; w.advance(p.s, p.blocks)) {
+        if (nu >= kUnitRing && !(ok = wait(q_empty(nu), (nu / kUnitRing - 1) & 1, kErrCopyWait))) break;
+        const int row0 = w.blk * BR, rows = min(BR, w.x.n * group - row0);
+        if (elect_one()) mbar_expect_tx(q_full(nu), rows * D * 2);
+        __syncwarp();
+        if (lane < rows) {
+          const int tok = (row0 + lane) / group;
+          bulk_load(sbase + C::OFF_Q + ((nu % kUnitRing) * BR + lane) * C::Q_ROW,
+                    p.q + (w.x.tok0 + tok) * p.q_token + (w.h * group + (row0 + lane - tok * group)) * p.q_head, D * 2, q_full(nu));
+        }
+        const int2 own = w.owners(blockIdx.x);
+        if (elect_one()) {
+          int4* r = ring + 3 * (nu % kUnitRing);
+          r[0] = make_int4(w.cnt, w.tile, p.blocks.key_end(w.x, w.blk), nu);
+          r[1] = make_int4(w.x.len, w.x.n, row0, w.x.tok0);
+          r[2] = make_int4(w.h, own.x, own.y, w.b);
+          mbar_arrive(q_full(nu));
+        }
+        __syncwarp();
+        ++nu;
+      }
+      if (ok && nu >= kUnitRing) ok = wait(q_empty(nu), (nu / kUnitRing - 1) & 1, kErrCopyWait);
+      if (ok) {
+        if (elect_one()) {
+          ring[3 * (nu % kUnitRing)] = make_int4(0, 0, 0, -1);
+          mbar_arrive(q_full(nu));
+        }
+        __syncwarp();
+        ++nu;
+      }
+      if (!ok) *abort_flag = 1;
+      for (int u = max(0, nu - kUnitRing); u < nu; ++u) mbar_wait_drain(q_full(u), (u / kUnitRing) & 1);
+      return;
+    }
+    // Keys and values: a copy to a page. One elected lane issues the copies, whose issue is what limits pages of 16 tokens,
+    // hence a warp for each. Page ids wait in shared memory.
+    const CUtensorMap* map = role ? &tmV : &tmK;
+    int t = 0;
     const int page_log2 = p.s.page_log2, page = 1 << page_log2, box = min(page, BN);
     const uint32_t bytes = box * D * (INT8 ? 1 : 2);  // of a copy
     const uint32_t dst0 = sbase + role * C::HALF;
@@ -239,28 +274,8 @@ attn_rows(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUten
         ahead += 32;
       };
       ids_more();
-      ids_more();
+      if (ahead < pages) ids_more();
       __syncwarp();
-      if (role == 0) {
-        if (nu >= kUnitRing && !(ok = wait(q_empty(nu), (nu / kUnitRing - 1) & 1, kErrCopyWait))) break;
-        const int row0 = w.blk * BR, rows = min(BR, w.x.n * group - row0);
-        const int2 own = w.owners(blockIdx.x);
-        if (elect_one()) {
-          int4* r = ring + 3 * (nu % kUnitRing);
-          r[0] = make_int4(cnt, w.tile, end, nu);
-          r[1] = make_int4(w.x.len, w.x.n, row0, w.x.tok0);
-          r[2] = make_int4(w.h, own.x, own.y, w.b);
-          mbar_arrive_expect_tx(q_full(nu), rows * D * 2);
-        }
-        __syncwarp();
-        if (lane < rows) {
-          const int tok = (row0 + lane) / group;
-          bulk_load(sbase + C::OFF_Q + ((nu % kUnitRing) * BR + lane) * C::Q_ROW,
-                    p.q + (w.x.tok0 + tok) * p.q_token + (w.h * group + (row0 + lane - tok * group)) * p.q_head, D * 2, q_full(nu));
-        }
-        __syncwarp();
-        ++nu;
-      }
       for (int i = 0; i < cnt; ++i, ++t) {
         const int s = t % C::SLOTS, round = t / C::SLOTS;
         const int j0 = (w.tile + i) * BN, place = j0 & (page - 1), first = j0 >> page_log2;
@@ -283,18 +298,6 @@ attn_rows(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUten
       if (!ok) break;
       w.advance(p.s, p.blocks);
     }
-    if (role == 0) {
-      if (ok && nu >= kUnitRing) ok = wait(q_empty(nu), (nu / kUnitRing - 1) & 1, kErrCopyWait);
-      if (ok) {
-        if (elect_one()) {
-          ring[3 * (nu % kUnitRing)] = make_int4(0, 0, 0, -1);
-          mbar_arrive(q_full(nu));
-        }
-        __syncwarp();
-        ++nu;
-      }
-      for (int u = max(0, nu - kUnitRing); u < nu; ++u) mbar_wait_drain(q_full(u), (u / kUnitRing) & 1);
-    }
     if (!ok) *abort_flag = 1;
     // every issued copy lands before this CTA's shared memory is released
     for (int i = max(0, t - C::SLOTS); i < t; ++i) mbar_wait_drain(full(i % C::SLOTS), (i / C::SLOTS) & 1);
@@ -313,10 +316,12 @@ attn_rows(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUten
       const Unit x = next_unit(u);
       __syncwarp();
       if (x.id >= 0 && lane == 0) mbar_arrive(q_empty(u));
+      const int row = x.row0 + r, tok = row / group;
+      const bool there = row < x.n * group;
+      uint2* dst = reinterpret_cast<uint2*>(
+          p.o + ((long long)(x.tok0 + tok) * p.s.heads * group + x.h * group + (row - tok * group)) * D + col);
       // all four warps go on, or none (a wait that gave up ends the roles; no warp may be left at a barrier)
       if (!joiners_all(x.id >= 0 && wait(join_full, u & 1, kErrJoinWait))) break;
-      const int row = x.row0 + r;
-      const bool there = row < x.n * group;
       float M = -CUDART_INF_F, L = 0.f, acc[PER];
 #pragma unroll
       for (int i = 0; i < PER; ++i) acc[i] = 0.f;
@@ -348,59 +353,57 @@ attn_rows(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUten
       } else {
         const long long slot = Walk<Blocks>::place(blockIdx.x, (int)blockIdx.x == x.c0);
         if (there) {
-          float* dst = p.part + (slot * BR + r) * D + col;
+          float* to = p.part + (slot * BR + r) * D + col;
 #pragma unroll
           for (int i = 0; i < PER; i += 4)
-            *reinterpret_cast<float4*>(dst + i) = make_float4(acc[i], acc[i + 1], acc[i + 2], acc[i + 3]);
+            *reinterpret_cast<float4*>(to + i) = make_float4(acc[i], acc[i + 1], acc[i + 2], acc[i + 3]);
           if (col == 0) p.ml[slot * BR + r] = make_float2(M, L);
         }
         joiners_meet();
-        if (warp == kConsumers) {
-          if (lane == 0) flag_set(p.flags + slot, p.call);
-          __syncwarp();
-          const bool all = flags_all(p.flags, 1, x.c0, x.c1, p.call);
-          if (all) flags_clear(p.flags, 1, x.c0, x.c1);
-          if (lane == 0) *joined = all;
-        }
+        const int parts = x.c1 - x.c0 + 1;
+        if (threadIdx.x == 32 * kConsumers) *joined = last_part(p.words + x.c0, p.call, parts);
         joiners_meet();
         done = *joined != 0;
         if (done) {
-          // Warp v takes every fourth part, four rows of it at once (32 lanes to a row); the four sums meet in shared memory.
-          const int parts = x.c1 - x.c0 + 1, rows = min(BR, x.n * group - x.row0);
+          // Warp v takes every fourth part, four rows of it at once (32 lanes to a row), each with a running maximum; the
+          // four warps' sums meet in shared memory as the consumers' did.
+          const int rows = min(BR, x.n * group - x.row0);
           const int v = warp - kConsumers;
           constexpr int W = D / 32;  // columns of a lane
           float* sums = merge;       // [warp][BR][D]
-          auto part_ml = [&](int c, int row) { return __ldcg(p.ml + (2LL * (x.c0 + c) + (c == 0)) * BR + row); };
           for (int r0 = 0; r0 < rows; r0 += 4) {
             float m4[4], l4[4], a4[4][W];
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
               m4[k] = -CUDART_INF_F;
-              for (int c = lane; c < parts; c += 32) m4[k] = fmaxf(m4[k], part_ml(c, min(r0 + k, rows - 1)).x);
               l4[k] = 0.f;
 #pragma unroll
               for (int e = 0; e < W; ++e) a4[k][e] = 0.f;
             }
+#pragma unroll 1
+            for (int c = v; c < parts; c += 2 * kJoiners) {  // two parts' loads at once
+              float2 y[2][4];
+              float f[2][4][W];
 #pragma unroll
-            for (int k = 0; k < 4; ++k) {
+              for (int i = 0; i < 2; ++i)
 #pragma unroll
-              for (int o = 16; o > 0; o >>= 1) m4[k] = fmaxf(m4[k], __shfl_xor_sync(0xffffffffu, m4[k], o));
-              m4[k] = m4[k] == -CUDART_INF_F ? 0.f : m4[k];
-            }
-#pragma unroll 2
-            for (int c = v; c < parts; c += kJoiners) {
-              const float* src = p.part + ((2LL * (x.c0 + c) + (c == 0)) * BR + r0) * D + lane * W;
+                for (int k = 0; k < 4; ++k) {
+                  const int part = c + i * kJoiners;
+                  const bool in = part < parts && r0 + k < rows;
+                  const long long at = Walk<Blocks>::place(x.c0 + part, part == 0) * BR + r0 + k;
+                  y[i][k] = in ? __ldcg(p.ml + at) : make_float2(-CUDART_INF_F, 0.f);
+                  const float* src = p.part + at * D + lane * W;
+                  if constexpr (W == 4) *reinterpret_cast<float4*>(f[i][k]) = in ? __ldcg(reinterpret_cast<const float4*>(src)) : make_float4(0.f, 0.f, 0.f, 0.f);
+                  else *reinterpret_cast<float2*>(f[i][k]) = in ? __ldcg(reinterpret_cast<const float2*>(src)) : make_float2(0.f, 0.f);
+                }
 #pragma unroll
               for (int k = 0; k < 4; ++k) {
-                if (r0 + k >= rows) continue;
-                const float2 y = part_ml(c, r0 + k);
-                const float wt = ex2(y.x - m4[k]);
-                l4[k] = fmaf(wt, y.y, l4[k]);
-                float f[W];
-                if constexpr (W == 4) *reinterpret_cast<float4*>(f) = __ldcg(reinterpret_cast<const float4*>(src + k * D));
-                else *reinterpret_cast<float2*>(f) = __ldcg(reinterpret_cast<const float2*>(src + k * D));
+                const float y0 = y[0][k].x, y1 = y[1][k].x, top = fmaxf(m4[k], fmaxf(y0, y1)), ref = top == -CUDART_INF_F ? 0.f : top;
+                const float wt = ex2(m4[k] - ref), w0 = ex2(y0 - ref), w1 = ex2(y1 - ref);
+                m4[k] = top;
+                l4[k] = fmaf(l4[k], wt, fmaf(w0, y[0][k].y, w1 * y[1][k].y));
 #pragma unroll
-                for (int e = 0; e < W; ++e) a4[k][e] = fmaf(wt, f[e], a4[k][e]);
+                for (int e = 0; e < W; ++e) a4[k][e] = fmaf(a4[k][e], wt, fmaf(w0, f[0][k][e], w1 * f[1][k][e]));
               }
             }
 #pragma unroll
@@ -412,24 +415,28 @@ attn_rows(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUten
             }
           }
           joiners_meet();
-          M = 0.f;  // (of a row without keys all sums are 0)
+          M = -CUDART_INF_F;
           L = 0.f;
 #pragma unroll
           for (int i = 0; i < PER; ++i) acc[i] = 0.f;
           if (there) {
+#pragma unroll
+            for (int u4 = 0; u4 < kJoiners; ++u4) M = fmaxf(M, ml[u4 * BR + r].x);
+            const float ref = M == -CUDART_INF_F ? 0.f : M;
 #pragma unroll 1
             for (int u4 = 0; u4 < kJoiners; ++u4) {
-              L += ml[u4 * BR + r].y;
+              const float2 y = ml[u4 * BR + r];
+              const float wt = ex2(y.x - ref);
+              L = fmaf(wt, y.y, L);
 #pragma unroll
               for (int i = 0; i < PER; i += 4) {
                 const float4 f = *reinterpret_cast<const float4*>(sums + (u4 * BR + r) * D + col + i);
-                acc[i] += f.x;
-                acc[i + 1] += f.y;
-                acc[i + 2] += f.z;
-                acc[i + 3] += f.w;
+                acc[i] = fmaf(wt, f.x, acc[i]);
+                acc[i + 1] = fmaf(wt, f.y, acc[i + 1]);
+                acc[i + 2] = fmaf(wt, f.z, acc[i + 2]);
+                acc[i + 3] = fmaf(wt, f.w, acc[i + 3]);
               }
             }
-            if (L == 0.f) M = -CUDART_INF_F;
           }
           joiners_meet();
         }
@@ -438,8 +445,6 @@ attn_rows(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUten
       }
       if (done && there) {
         const float inv = M == -CUDART_INF_F ? 0.f : 1.f / L;
-        uint2* dst = reinterpret_cast<uint2*>(
-            p.o + ((long long)(x.tok0 + row / group) * p.s.heads * group + x.h * group + row % group) * D + col);
 #pragma unroll
         for (int i = 0; i < PER / 4; ++i)
           dst[i] = make_uint2(pack2<BF16>(acc[4 * i] * inv, acc[4 * i + 1] * inv), pack2<BF16>(acc[4 * i + 2] * inv, acc[4 * i + 3] * inv));
@@ -821,7 +826,7 @@ cudaError_t launch(const PagedAttnArgs& a, int dev) {
     return cudaErrorInvalidValue;
   const size_t places = (size_t)ctas * 2, part_bytes = places * C::BR * D * sizeof(float), ml_bytes = places * C::BR * sizeof(float2);
   void* block = nullptr;
-  if ((e = scratch_alloc(dev, part_bytes + ml_bytes + places * 8, a.stream, &block)) != cudaSuccess) return e;
+  if ((e = scratch_alloc(dev, part_bytes + ml_bytes + (size_t)ctas * 8, a.stream, &block)) != cudaSuccess) return e;
   char* base = static_cast<char*>(block);
   constexpr int BN = C::BN;
   Params<NT, BN> p{a.s, static_cast<const uint16_t*>(a.q), a.q_token, a.q_head, static_cast<uint16_t*>(a.o), a.ks, a.vs, a.kss, a.vss,

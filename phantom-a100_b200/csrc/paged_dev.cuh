@@ -204,30 +204,39 @@ struct Walk {
   }
 };
 
-// The parts of a shared unit are joined by the CTA that finds all of them written. Each part has a 64-bit flag that holds
-// the call's number (unique in the process) once the part is in memory. A CTA writes its part, then its flag (release), then,
-// past a fence.sc, reads all the unit's flags: in the order that the fences have, the CTA of the last one finds them all. (Two
-// may; they write the same result.) It then clears them, so that a call replayed from a graph, whose number is the same
-// each time, finds none set. Flags need no initialisation: what a pool's memory held before does not equal the number.
-__device__ __forceinline__ void flag_set(unsigned long long* flag, unsigned long long call) {
-  asm volatile("st.release.gpu.global.u64 [%0], %1;" ::"l"(flag), "l"(call) : "memory");
-  asm volatile("fence.sc.gpu;" ::: "memory");
+// The parts of a shared unit are joined by the CTA that arrives last. Each unit has a 64-bit word: the call's number (unique
+// in the process; its last kCountBits dropped) and how many parts are in memory. It needs no initialisation: what a pool's
+// memory held before does not equal the number, and the first to arrive puts the number there. An arrival on the old value
+// counts for nothing, so whoever made one starts over once the number is there; each CTA changes the word at most twice
+// before that, which bounds the loop. The last one leaves 0, for a call replayed from a graph has the same number each time.
+// (A flag for each part, set and then all of them read past a fence.sc, took 3200 cycles.)
+constexpr int kCountBits = 12;
+__device__ __forceinline__ unsigned long long atom_add64(unsigned long long* word, unsigned long long y) {
+  unsigned long long old;
+  asm volatile("atom.add.acq_rel.gpu.global.u64 %0, [%1], %2;" : "=l"(old) : "l"(word), "l"(y) : "memory");
+  return old;
 }
-__device__ __forceinline__ unsigned long long flag_get(const unsigned long long* flag) {
-  unsigned long long y;
-  asm volatile("ld.relaxed.gpu.global.u64 %0, [%1];" : "=l"(y) : "l"(flag) : "memory");
-  return y;
+__device__ __forceinline__ unsigned long long atom_cas64(unsigned long long* word, unsigned long long from, unsigned long long to) {
+  unsigned long long old;
+  asm volatile("atom.cas.acq_rel.gpu.global.b64 %0, [%1], %2, %3;" : "=l"(old) : "l"(word), "l"(from), "l"(to) : "memory");
+  return old;
 }
-// Whole warp: are the flags of the unit whose parts the CTAs c0 ... c1 have all set? `per` flags to a place.
-__device__ __forceinline__ bool flags_all(const unsigned long long* flags, int per, int c0, int c1, unsigned long long call) {
-  bool all = true;
-  for (int c = c0 + (int)(threadIdx.x & 31); c <= c1; c += 32) all &= flag_get(flags + (2LL * c + (c == c0)) * per) == call;
-  all = __all_sync(0xffffffffu, all);
-  asm volatile("fence.acq_rel.gpu;" ::: "memory");
-  return all;
-}
-__device__ __forceinline__ void flags_clear(unsigned long long* flags, int per, int c0, int c1) {
-  for (int c = c0 + (int)(threadIdx.x & 31); c <= c1; c += 32) flags[(2LL * c + (c == c0)) * per] = 0;
+// One thread, whose CTA's part is written (and seen by this thread): is it the last of `parts` > 1?
+__device__ __forceinline__ bool last_part(unsigned long long* word, unsigned long long call, int parts) {
+  const unsigned long long tag = call >> kCountBits;
+  unsigned long long old = atom_add64(word, 1);
+  if (old >> kCountBits != tag) {
+    for (unsigned long long seen = old + 1;;) {
+      const unsigned long long y = atom_cas64(word, seen, tag << kCountBits | 1);
+      if (y == seen) return false;  // the first
+      if (y >> kCountBits == tag) break;
+      seen = y;
+    }
+    old = atom_add64(word, 1);
+  }
+  const bool last = (int)(old & ((1 << kCountBits) - 1)) + 1 == parts;
+  if (last) *word = 0;
+  return last;
 }
 
 // ------------------------------------------------------------------------------------------------ copies, 8-bit values
