@@ -16,8 +16,9 @@
 //     (paged_dev.cuh). Ragged lengths then cost nothing, and one long sequence spreads over the GPU. The parts of a unit
 //     that several CTAs share (fp32 rows, reference maximum, sum) are joined in the order of the CTAs by the one that
 //     finishes last: the result depends on the lengths and the GPU's SM count alone.
-//   * Producer warps for keys and for values read the page table and keep a ring of tiles in flight by TMA (a box per page, swizzled, so that
-//     pages of 16 tokens land as one conflict-free tile), two tiles to each pair of consumer warps.
+//   * Producer warps for keys and for values read the page table and keep a ring of tiles in flight by TMA (a box per page,
+//     swizzled, so that pages of 16 tokens land as one conflict-free tile), two tiles to each pair of consumer warps. A
+//     third brings the queries.
 //   * Six or eight consumer warps work without meeting: two to a tile, half of its keys each, every warp with its own
 //     running maximum, sum and output. At the end of a unit they leave these in shared memory and go on to the next, whose
 //     queries a producer has brought there; four further warps join and write them. (With the consumers doing this
@@ -85,8 +86,10 @@ struct Cfg {
 template <int NT, int BN>
 struct RowBlocks {
   int group, causal, heads;
-  static constexpr int kTile = BN, kUnit = 2, BR = 8 * NT;
-  static constexpr float kPart = NT == 1 ? 0.8f : 2.f;
+  // Measured (us): kJoin 8 | 5: 4 sequences of 500 tokens 10.7 | 12.0, 8 of 700 12.6 | 15.0, 32 of 200 to 4095 the same.
+  // kPart 0.4 | 0.8: one of 4096 14.3 | 15.6, of 1024 11.9 | 12.1; 16 rows, 0.5 | 2: one of 1000 17.3 | 23.3.
+  static constexpr int kTile = BN, kUnit = 2, kJoin = 8, BR = 8 * NT;
+  static constexpr float kPart = NT == 1 ? 0.4f : 0.5f;
   __device__ int count(const Seq& x) const { return (x.n * group + BR - 1) / BR; }
   __device__ int key_end(const Seq& x, int rb) const {
     if (!causal) return x.len;
@@ -176,18 +179,13 @@ attn_rows(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUten
   const int group = p.blocks.group, causal = p.blocks.causal;
   int* status = p.s.status;
 
-  if (threadIdx.x == 0) {
-    for (int s = 0; s < C::SLOTS; ++s) {
-      mbar_init(full(s), 2);   // the producers
-      mbar_init(empty(s), 2);  // the consuming pair
-    }
-    for (int u = 0; u < kUnitRing; ++u) {
-      mbar_init(q_full(u), 1);
-      mbar_init(q_empty(u), C::WARPS + kJoiners);
-    }
-    mbar_init(join_full, C::WARPS);
-    mbar_init(join_empty, kJoiners);
-    *abort_flag = 0;
+  if (warp == 0) {
+    constexpr int N = 2 * C::SLOTS;  // of full (the two producers arrive) and empty (the consuming pair does)
+    static_assert(N + 2 * kUnitRing + 2 <= 32);
+    if (lane < N + 2 * kUnitRing + 2)
+      mbar_init(bars + 8u * lane, lane < N ? 2 : lane < N + kUnitRing ? 1 : lane < N + 2 * kUnitRing ? C::WARPS + kJoiners :
+                                  lane == N + 2 * kUnitRing ? C::WARPS : kJoiners);
+    if (lane == 0) *abort_flag = 0;
     fence_mbar_init();
   }
   __syncthreads();

@@ -72,7 +72,7 @@ struct Cfg {
 // Units of `per` new tokens; tiles of 128 keys.
 struct TokenBlocks {
   int per, causal, heads;
-  static constexpr int kTile = BN, kUnit = 4;
+  static constexpr int kTile = BN, kUnit = 4, kJoin = 5;
   static constexpr float kPart = 0.1f;
   __device__ int count(const Seq& x) const { return (x.n + per - 1) / per; }
   __device__ int key_end(const Seq& x, int blk) const {

@@ -50,7 +50,7 @@ __device__ __forceinline__ int seq_index(const PagedSeqs& s, int tok) {
 // `Blocks` says how the rows are cut: kTile keys to a tile; count(x) blocks; the keys key_end(x, blk) that a block sees;
 // head_tiles(x) tiles in all of one head. A unit costs something besides its tiles (its queries, its output, the start of
 // its pipeline), as much as kUnit tiles; these are counted before its first one when the shares are cut, and a share that
-// ends among them has nothing of the unit. Joining a part of a shared unit takes as long as kPart tiles.
+// ends among them has nothing of the unit. Joining a shared unit costs as much as kJoin tiles, and kPart tiles for each part.
 
 // At least one tile, so that rows without any key are written too (as zeros).
 template <typename Blocks>
@@ -68,8 +68,6 @@ __device__ __forceinline__ long long sum_tiles(const Blocks& k, const Seq& x) {
   for (int i = k.count(x) - 1; i >= 0; --i) w += tiles_of(k, x, i);
   return w;
 }
-
-constexpr int kJoinTiles = 5;
 
 // A whole warp walks one CTA's share; every value is uniform over the warp. Positions count tiles and units' own costs.
 template <typename Blocks>
@@ -94,46 +92,48 @@ struct Walk {
   }
   __device__ void start(const PagedSeqs& s, const Blocks& k, int cta, int grid) {
     const int lane = threadIdx.x & 31;
-    auto seq_work = [&](int i) { return i < s.batch ? head_work(k, seq_of(s, i)) * s.heads : 0LL; };
-    // Whole units, one to a CTA, where that takes no more than kJoinTiles tiles longer than even shares: joining a shared
-    // unit costs about as much (measured: 4 us, a tile of 32 KB 0.75 us). A head's last block sees the most keys.
-    long long units = 0, w = 0, total = 0;
+    // Whole units, one to a CTA, where that takes no more than kJoin tiles longer than even shares. A head's last block sees
+    // the most keys.
+    long long w = 0, total = 0;
+    unsigned units = 0, units0 = 0;  // (of a lane's sequence among the first 32; kept within 32 bits, the grid is smaller)
     int most = 0;
     for (int i0 = 0; i0 < s.batch; i0 += 32) {
       long long y = 0;
+      unsigned u = 0;
       if (i0 + lane < s.batch) {
         const Seq q = seq_of(s, i0 + lane);
-        y = head_work(k, q) * s.heads;
         const int c = k.count(q);
-        units += (long long)c * s.heads;
+        y = (k.head_tiles(q) + (long long)c * kUnit) * s.heads;
+        u = (unsigned)min((long long)c * s.heads, 1LL << 20);
         if (c > 0) most = max(most, tiles_of(k, q, c - 1));
       }
       const long long z = scan(y, lane);
-      if (i0 == 0) w = z;  // (up to 32 sequences: one scan gives the total and the place)
+      if (i0 == 0) w = z, units0 = u;  // (up to 32 sequences: one scan gives the total and the place)
       total += __shfl_sync(0xffffffffu, z, 31);
+      units = min(units + __reduce_add_sync(0xffffffffu, u), 1u << 30);
     }
-    for (int m = 16; m > 0; m >>= 1) {
-      units += __shfl_xor_sync(0xffffffffu, units, m);
-      most = max(most, __shfl_xor_sync(0xffffffffu, most, m));
-    }
+    most = __reduce_max_sync(0xffffffffu, most);
     // No smaller shares than pay: with s tiles to a share the longest unit takes as long as s tiles and most / s parts to
     // join, kPart tiles each, least where s^2 = kPart most.
     const long long least = max(1LL, (long long)sqrtf(Blocks::kPart * (float)most));
     ctas = (int)min((long long)grid, quotient(total + least - 1, least));
     share = ctas > 0 ? quotient(total, ctas) : 0;
     more = (int)(total - share * ctas);
-    by_unit = units <= grid && most + kUnit <= share + kJoinTiles;
+    by_unit = units <= (unsigned)grid && most + kUnit <= share + Blocks::kJoin;
     if (by_unit) ctas = (int)units;
     cnt = 0;
     if (cta >= ctas) return;
     // the place of the share's beginning, or of the CTA's unit, among all
     const long long pos = by_unit ? cta : first(cta);
     auto seq_part = [&](int i) {
-      return by_unit ? (i < s.batch ? (long long)k.count(seq_of(s, i)) * s.heads : 0LL) : seq_work(i);
+      if (i >= s.batch) return 0LL;
+      const Seq q = seq_of(s, i);
+      return by_unit ? (long long)k.count(q) * s.heads : head_work(k, q) * s.heads;
     };
+    if (by_unit) w = scan(units0, lane);
     long long before = 0;
     for (int i0 = 0;; i0 += 32) {
-      if (i0 > 0 || by_unit) w = scan(seq_part(i0 + lane), lane);
+      if (i0 > 0) w = scan(seq_part(i0 + lane), lane);
       const unsigned past = __ballot_sync(0xffffffffu, before + w > pos);
       if (past) {
         const int l = __ffs(past) - 1;
