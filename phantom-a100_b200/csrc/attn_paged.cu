@@ -857,12 +857,12 @@ cudaError_t launch_d(const PagedAttnArgs& a, int dev) {
 
 }  // namespace rows
 
-// Units of 16 rows for 9 to 16 of them; with a 16-bit cache the chunk kernel has those (capi.cu).
-cudaError_t launch_paged_attn_rows(const PagedAttnArgs& a, int dev, int rows) {
+// Units of 8 rows, or (8-bit caches alone, whose conversion then serves twice the rows) of 16.
+cudaError_t launch_paged_attn_rows(const PagedAttnArgs& a, int dev, bool wide) {
   using namespace phantom::rows;
   if (!a.int8) return a.d == 64 ? launch_d<64, false, 1>(a, dev) : launch_d<128, false, 1>(a, dev);
-  if (a.d == 64) return rows <= 8 ? launch_d<64, true, 1>(a, dev) : launch_d<64, true, 2>(a, dev);
-  return rows <= 8 ? launch_d<128, true, 1>(a, dev) : launch_d<128, true, 2>(a, dev);
+  if (a.d == 64) return wide ? launch_d<64, true, 2>(a, dev) : launch_d<64, true, 1>(a, dev);
+  return wide ? launch_d<128, true, 2>(a, dev) : launch_d<128, true, 1>(a, dev);
 }
 
 }  // namespace phantom

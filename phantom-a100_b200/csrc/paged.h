@@ -55,8 +55,8 @@ struct PagedAttnArgs {
 };
 
 // Few query rows for each key head (decoding): attn_paged.cu. Right for any number of them.
-// `rows`: how many to expect.
-cudaError_t launch_paged_attn_rows(const PagedAttnArgs& a, int dev, int rows);
+// `wide` (8-bit caches): units of 16 rows instead of 8.
+cudaError_t launch_paged_attn_rows(const PagedAttnArgs& a, int dev, bool wide);
 // Many query rows (chunks of prompts): attn_paged_tc_sm100.cu.
 cudaError_t launch_paged_attn_chunk(const PagedAttnArgs& a, int dev);
 

@@ -159,6 +159,21 @@ def test_zero_scales_and_zero_queries(hint):
     check(c, True, hint)
 
 
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("new,group,hint", [([1, 1, 1], 16, 1), ([2, 0, 2], 12, 2), ([5, 1, 3], 9, 1), ([1, 2, 1], 16, 2)])
+@pytest.mark.parametrize("dtype,d", [(BF16, 128), (F16, 128), (BF16, 64), (F16, 64)])
+def test_long_8_bit_contexts_of_9_to_32_rows(dtype, d, new, group, hint, causal):
+    """Units of 16 rows: taken where the keys of 4 heads and 3 sequences with room for 10240 tokens are read more than once."""
+    check(Case(new, [8000, 500, 3333], 4, group, d, 1024, dtype, True), causal, hint)
+
+
+@pytest.mark.parametrize("dtype,int8", [(BF16, False), (BF16, True), (F16, False)])
+@pytest.mark.parametrize("new", [[3] * 4, [8, 1, 0, 5]])
+def test_a_few_new_tokens(new, dtype, int8):
+    """Several blocks of rows to a sequence, as many as max_new says."""
+    check(Case(new, [700, 33, 64, 300], 2, 4, 128, 16, dtype, int8), True, max(new))
+
+
 @pytest.mark.parametrize("hint", [1, 4096], ids=["rows", "chunk"])
 def test_only_rows_that_see_a_nan_turn_nan(hint):
     """8-bit caches: a vector with a NaN was appended as the last but one of the new tokens."""
