@@ -434,7 +434,8 @@ attn_chunk(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUte
     // 8-bit pages to 16-bit tiles: keys of tile j, its values, keys of tile j + 1, ... A thread has one 16-byte chunk of a
     // row in every pass over 16 (d = 64: 32) rows; the next item's bytes are on their way into the place that the
     // current one's leave. Eight lanes that store together have four chunks of a column block in two rows: swizzled, these
-    // meet no bank twice. Rows past the unit's end turn into whatever the page holds, numbers all (their weights are 0).
+    // meet no bank twice. Rows past the unit's end turn into whatever the page holds, numbers all (their weights are 0);
+    // rows without a page into zeros, of weight like any key's where they are within the length.
     constexpr int STEP = D == 128 ? 16 : 32, N = BN / STEP;  // rows at a time; times
     const int tid = threadIdx.x - 32 * CONV_WARP;
     const int chunk = D == 128 ? (lane & 3) + 4 * ((lane >> 3) & 1) : lane & 3;
@@ -446,7 +447,8 @@ attn_chunk(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUte
     int nu = 0, i = 0, j0 = 0;
     bool ok = true;
     Unit x = take_unit(0, ok);
-    // Byte offsets of the tile's 16-row pieces (a page has whole ones), a lane each; -1: no keys there that the unit sees.
+    // Byte offsets of the tile's 16-row pieces (a page has whole ones), a lane each; -1: no page there, or no keys that the
+    // unit sees.
     long long k_off = -1, v_off = -1;
     int id = -1;
     const int8_t *k_base = nullptr, *v_base = nullptr;
@@ -460,12 +462,13 @@ attn_chunk(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUte
       v_base = p.vc + x.h * p.vcs.head + (row_in & 15) * p.vcs.token + chunk * 16;
     };
     // Pass n's 16 bytes of this thread lie in its own place of shared memory, filled one item ahead by its own asynchronous
-    // copies (a copy group to a pass, empty where there is nothing to copy), so the roles meet nowhere but at the ring.
+    // copies (a copy group to a pass; of no bytes, which fills zeros in, where there is no page), so the roles meet nowhere
+    // but at the ring.
     const uint32_t raw = sbase + C::OFF_RAW + tid * 16;
     auto load = [&](int n, const int8_t* base, long long off) {
       const long long o = __shfl_sync(0xffffffffu, off, (n * STEP + row_in) >> 4);
-      if (o >= 0)
-        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(raw + n * 2048), "l"(base + o) : "memory");
+      asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(raw + n * 2048), "l"(base + max(o, 0LL)),
+                   "r"(o < 0 ? 0 : 16) : "memory");
       asm volatile("cp.async.commit_group;" ::: "memory");
     };
     auto take = [&](int n, uint32_t (&in)[4]) {  // the oldest of the N groups in flight
@@ -477,9 +480,10 @@ attn_chunk(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUte
     auto load_scales = [&]() {
       const int from = __shfl_sync(0xffffffffu, id, (tid >> 4) & 7);
       const int place = (j0 + tid) & page_mask;
-      past = from < 0 || j0 + tid >= x.end;
-      ks = past ? 0.f : p.ks[from * p.kss.page + x.h * p.kss.head + place];
-      vs = past ? 1.f : p.vs[from * p.vss.page + x.h * p.vss.head + place];
+      past = j0 + tid >= x.end;
+      const bool none = past || from < 0;
+      ks = none ? 0.f : p.ks[from * p.kss.page + x.h * p.kss.head + place];
+      vs = none ? 0.f : p.vs[from * p.vss.page + x.h * p.vss.head + place];
     };
     if (x.id >= 0) {
       begin_tile();

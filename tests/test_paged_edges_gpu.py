@@ -1,0 +1,83 @@
+"""GPU: the paged entry points where their inputs are out of range, not finite or extreme, and what a failed call leaves."""
+import pytest
+import torch
+
+from paged_case import U, Case, assert_attention, quantise64
+
+pytestmark = pytest.mark.gpu
+
+import cuda_attn  # noqa: E402
+
+F16, BF16 = torch.float16, torch.bfloat16
+STATUS_PAGE = 512
+both_kernels = pytest.mark.parametrize("hint", [1, 4096], ids=["rows", "chunk"])
+
+
+@pytest.fixture(autouse=True)
+def _gpu(cuda_ok):
+    cuda_attn.device_status()
+    yield
+    assert cuda_attn.device_status() == 0
+
+
+def attend(c, causal=True, max_new=0, scale=None):
+    return cuda_attn.paged_attn(c.q, *c.where(), **c.scales(), causal=causal, max_new=max_new, scale=scale)
+
+
+def pools(c):
+    return [x for x in (c.k_cache, c.v_cache, c.k_scale, c.v_scale) if x is not None]
+
+
+def same(x, y):
+    """Equal, NaNs in the same places among them."""
+    return torch.equal(torch.nan_to_num(x.float(), nan=7.0), torch.nan_to_num(y.float(), nan=7.0))
+
+
+def soil(shape, dtype):
+    """Leaves NaNs in the memory that the next tensor of this size is given."""
+    torch.full(shape, float("nan"), device="cuda", dtype=dtype)
+
+
+# ------------------------------------------------------------------------------------------------ pages out of range
+
+
+@both_kernels
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("dtype,int8", [(F16, False), (BF16, False), (F16, True), (BF16, True)])
+def test_tokens_without_a_page_are_zeros(dtype, int8, d, causal, hint):
+    """Within the length, under a page id that is out of range: keys and values of zeros, to the attention (they count in the
+    sum of weights) as to paged_read. Single pages, a run of them that covers whole tiles, and all of a sequence's."""
+    new, kv = [3, 140, 2, 1], [700, 900, 40, 333]
+    c = Case(new, kv, 2, 4, d, 16, dtype, int8)
+    bad = [[0, 5, 43], list(range(8, 41)) + [56], [0, 1, 2], [20]]
+    for b, pages in enumerate(bad):
+        for i, page in enumerate(pages):
+            c.table[b, page] = (-1, c.k_cache.shape[0], 1 << 30, -(1 << 31))[i % 4]
+            for held in (c.keys, c.values):
+                held[b][16 * page:16 * page + 16] = 0
+    out = attend(c, causal, hint)
+    assert cuda_attn.device_status() == STATUS_PAGE
+    assert_attention(out, *c.attention64(causal), dtype, int8)
+    assert not out[143:145].any()  # the third sequence has no page at all
+
+    soil((146, 2, d), dtype), soil((146, 2, d), dtype)
+    read = cuda_attn.paged_read(*c.where(), 146, dtype=dtype, **c.scales())
+    assert cuda_attn.device_status() == STATUS_PAGE
+    for got, held in zip(read, (c.keys, c.values)):
+        want = torch.cat([x[t - n:] for x, n, t in zip(held, new, kv)])
+        assert torch.equal(got, want.to(dtype))
+
+    before = [x.clone() for x in pools(c)]
+    x = torch.ones(146, 2, d, device="cuda", dtype=dtype)
+    cuda_attn.paged_append(x, x, *c.where(), **c.scales())
+    assert cuda_attn.device_status() == STATUS_PAGE
+    good = torch.zeros(c.k_cache.shape[0], 16, dtype=torch.bool, device="cuda")
+    for b, (n, t) in enumerate(zip(new, kv)):
+        for j in range(t - n, t):
+            if j // 16 not in bad[b]:
+                good[c.table[b, j // 16], j % 16] = True
+    q, s = quantise64(x[0, 0])
+    for was, now, put in zip(before, pools(c), (q if int8 else x[0, 0], q if int8 else x[0, 0], s, s)):
+        was.transpose(1, 2)[good] = put
+        assert same(was, now)
