@@ -49,8 +49,8 @@ constexpr int kJoiners = 4;
 constexpr int kUnitRing = 4;
 constexpr int kErrCopyWait = 1, kErrTileWait = 4, kErrJoinWait = 8;
 
-// Warps: eight consumers, in pairs that take the tiles in turn; the joiners; three producers and an idle warp that completes
-// their warpgroup. Registers (setmaxnreg, by warpgroup): 512 threads launch with 128 each; 2 * 168 + 104 + 72 = 4 * 128.
+// Warps: eight consumers, in pairs that take the tiles in turn; the joiners; three producers and, completing their warpgroup,
+// one that zeroes the rows of no sequence. Registers (setmaxnreg, by warpgroup): 512 threads launch with 128 each; 2 * 168 + 104 + 72 = 4 * 128.
 constexpr int kConsumers = 8, PRODUCER = kConsumers + kJoiners, kThreads = 32 * (PRODUCER + 4);
 constexpr int kRegsConsumer = 168, kRegsJoiner = 104, kRegsProducer = 72;
 
@@ -212,7 +212,10 @@ attn_rows(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUten
   if (warp >= PRODUCER) {
     setmaxnreg_dec<kRegsProducer>();
     const int role = warp - PRODUCER;
-    if (role > 2) return;
+    if (role > 2) {
+      zero_unowned(p.s, p.o, p.s.heads * group * (D / 8), blockIdx.x * 32 + lane, gridDim.x * 32);
+      return;
+    }
     // Producers, of the keys, of the values, and of the units' records and queries. Each walks the CTA's share by itself.
     if (role < 2 && elect_one()) tma_prefetch_desc(role ? &tmV : &tmK);
     __syncwarp();
@@ -447,12 +450,6 @@ attn_rows(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUten
         for (int i = 0; i < PER / 4; ++i)
           dst[i] = make_uint2(pack2<BF16>(acc[4 * i] * inv, acc[4 * i + 1] * inv), pack2<BF16>(acc[4 * i + 2] * inv, acc[4 * i + 3] * inv));
       }
-    }
-    if (blockIdx.x == 0) {
-      // zeroes the rows of packed tokens that belong to no sequence
-      const int first = min(max(p.s.cu_new[p.s.batch], 0), p.s.total);
-      const long long row = (long long)p.s.heads * group * D;
-      for (long long i = first * row + tid; i < p.s.total * row; i += 128) p.o[i] = 0;
     }
     return;
   }

@@ -924,7 +924,8 @@ attn_chunk(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUte
 
 // Joins the parts of the units that several CTAs of attn_chunk shared. Block (c, query tile, 32 columns): the unit that CTA c
 // is the first to continue; thread = query row and 8 columns; the parts in the order of the CTAs, four on their way at
-// once, in one pass with a running maximum. Block (0, 0, 0) also zeroes the rows of packed tokens that belong to no sequence.
+// once, in one pass with a running maximum. Blocks (0, ...), for which there is no such unit, zero the rows of packed tokens
+// that belong to no sequence.
 constexpr int kMergeCols = 8, kMergeThreads = 512;
 template <int D, bool BF16>
 __global__ void __launch_bounds__(kMergeThreads) merge_chunk(const Params p) {
@@ -932,11 +933,8 @@ __global__ void __launch_bounds__(kMergeThreads) merge_chunk(const Params p) {
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const int g = blockIdx.y, c0 = blockIdx.x - 1;
   if (c0 < 0) {
-    if (g == 0 && blockIdx.z == 0) {
-      const int first = min(max(p.s.cu_new[p.s.batch], 0), p.s.total);
-      const long long row = (long long)p.s.heads * p.group * D;
-      for (long long i = first * row + threadIdx.x; i < p.s.total * row; i += blockDim.x) p.o[i] = 0;
-    }
+    const int block = g * gridDim.z + blockIdx.z;
+    zero_unowned(p.s, p.o, p.s.heads * p.group * (D / 8), block * kMergeThreads + threadIdx.x, 2 * gridDim.z * kMergeThreads);
     return;
   }
   const int4 a = p.starts[2 * blockIdx.x], b = p.starts[2 * blockIdx.x + 1];

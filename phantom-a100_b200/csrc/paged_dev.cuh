@@ -44,6 +44,15 @@ __device__ __forceinline__ int seq_index(const PagedSeqs& s, int tok) {
   return b;
 }
 
+// Zeroes the rows of packed tokens that belong to no sequence: those from cu_new[batch] on (a captured call's unused ones,
+// nothing wrong) and those before cu_new[0], which has to be 0. `row`: 16-byte pieces of a token. Worker `me` of `n`.
+__device__ __forceinline__ void zero_unowned(const PagedSeqs& s, void* o, int row, long long me, long long n) {
+  const int first = min(max(s.cu_new[0], 0), s.total), last = max(min(max(s.cu_new[s.batch], 0), s.total), first);
+  if (me == 0 && s.cu_new[0] != 0) atomicOr(s.status, PHANTOM_ATTN_STATUS_PAGE);
+  const long long lead = (long long)first * row, count = lead + (long long)(s.total - last) * row, skip = (long long)last * row - lead;
+  for (long long i = me; i < count; i += n) static_cast<uint4*>(o)[i < lead ? i : i + skip] = make_uint4(0, 0, 0, 0);
+}
+
 // ------------------------------------------------------------------------------------------------ even shares of work
 // An attention call's work: units (sequence, key head, block of query rows) in a row, each of as many tiles of keys as its
 // rows see. CTA c of G takes the tiles [c W / G, (c + 1) W / G) of all W, so a unit may be shared by several CTAs.

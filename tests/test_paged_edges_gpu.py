@@ -81,3 +81,38 @@ def test_tokens_without_a_page_are_zeros(dtype, int8, d, causal, hint):
     for was, now, put in zip(before, pools(c), (q if int8 else x[0, 0], q if int8 else x[0, 0], s, s)):
         was.transpose(1, 2)[good] = put
         assert same(was, now)
+
+
+# ------------------------------------------------------------------------------------------------ packed rows of no sequence
+
+
+@both_kernels
+@pytest.mark.parametrize("lead,trail", [(1, 0), (3, 4), (700, 5), (0, 900)])
+@pytest.mark.parametrize("d,int8", [(64, False), (128, True)])
+def test_packed_tokens_before_and_after_the_sequences(d, int8, lead, trail, hint):
+    """cu_new of a slice: tokens before its first are of no sequence, which is out of range; those after its last may be."""
+    c = Case([2, 40, 3], [50, 60, 500], 3, 4, d, 16, F16, int8)
+    want = attend(c, True, hint)
+    n = c.total
+    c.cu += lead
+    q = torch.ones(lead + n + trail, 12, d, device="cuda", dtype=F16)
+    q[lead:lead + n] = c.q
+    for _ in range(2):
+        soil(q.shape, F16)
+        out = cuda_attn.paged_attn(q, *c.where(), **c.scales(), max_new=hint)
+        assert cuda_attn.device_status() == (STATUS_PAGE if lead else 0)
+        assert torch.equal(out[lead:lead + n], want)
+        assert not out[:lead].any() and not out[lead + n:].any()
+    soil((lead + n + trail, 3, d), F16), soil((lead + n + trail, 3, d), F16)
+    k, v = cuda_attn.paged_read(*c.where(), lead + n + trail, dtype=F16, **c.scales())
+    assert cuda_attn.device_status() == (STATUS_PAGE if lead else 0)
+    for x in (k, v):
+        assert not x[:lead].any() and not x[lead + n:].any()
+    before = [x.clone() for x in pools(c)]
+    x = torch.zeros(lead + n + trail, 3, d, device="cuda", dtype=F16)
+    x[:lead] = x[lead + n:] = 1.0
+    x[lead:lead + n] = k[lead:lead + n]
+    cuda_attn.paged_append(x, x, *c.where(), **c.scales())
+    assert cuda_attn.device_status() == (STATUS_PAGE if lead else 0)
+    if not int8:
+        assert same(before[0], c.k_cache)  # the new tokens' own keys were written, and nothing else
