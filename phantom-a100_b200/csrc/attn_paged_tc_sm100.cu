@@ -124,16 +124,17 @@ struct Unit {
   int h, slot, id, b;          // key head; place of the partial result (-1: the unit is whole); id -1 ends the roles
 };
 
+// NaN if a score is: the polynomial of softmax64 loses NaNs, so the row's maximum carries them.
 template <int N>
 __device__ __forceinline__ float row_max(const float (&s)[N]) {
   float a[8];
 #pragma unroll
-  for (int k = 0; k < 8; ++k) a[k] = fmaxf(s[k], s[k + 8]);
+  for (int k = 0; k < 8; ++k) a[k] = max_nan(s[k], s[k + 8]);
 #pragma unroll
   for (int i = 16; i < N; i += 16)
 #pragma unroll
-    for (int k = 0; k < 8; ++k) a[k] = max3(a[k], s[i + k], s[i + 8 + k]);
-  return fmaxf(max3(a[0], a[1], a[2]), max3(a[3], a[4], max3(a[5], a[6], a[7])));
+    for (int k = 0; k < 8; ++k) a[k] = max3_nan(a[k], s[i + k], s[i + 8 + k]);
+  return max_nan(max3_nan(a[0], a[1], a[2]), max3_nan(a[3], a[4], max3_nan(a[5], a[6], a[7])));
 }
 
 // p = exp2(s * scale - sub) of 64 scores as packed 16-bit pairs; returns the sum of the unrounded values. Every fourth pair
@@ -675,6 +676,7 @@ attn_chunk(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUte
     const uint32_t t_o = tmem + lane_off + (g ? C::T_O1 : C::T_O0);
     uint8_t* stage = smem + C::OFF_OST + warp * C::OST_WARP;
     const int row_tok = r_local / p.group;  // this row's token within the query tile
+    const bool in_use = row_tok < p.tile_tokens;
     // multiplies this lane's row of O
     auto rescale_o = [&](float alpha) {
       const float2 a2 = make_float2(alpha, alpha);
@@ -816,7 +818,7 @@ attn_chunk(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUte
         if (j == 0) {
           m_used = m_new;
         } else {
-          need = m_new > m_used + kRescaleThreshold;
+          need = in_use && !(m_new <= m_used + kRescaleThreshold);  // (a NaN goes on to l and O)
           if (need) {
             alpha = ex2(m_used - m_new);
             m_used = m_new;
@@ -826,7 +828,8 @@ attn_chunk(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUte
           tc_fence_after();
           if (__any_sync(0xffffffffu, need)) rescale_o(alpha);
         }
-        const float sub = m_used == -CUDART_INF_F ? 0.f : m_used;
+        // (infinity less infinity is no weight: all of the row turns NaN, which the sum keeps)
+        const float sub = m_used == -CUDART_INF_F ? 0.f : m_used == CUDART_INF_F ? CUDART_NAN_F : m_used;
         uint32_t pk[32];
         float psum = softmax64<BF16, 0>(s, p.scale_log2, sub, pk);
         tmem_st32(t_p, pk);

@@ -116,3 +116,42 @@ def test_packed_tokens_before_and_after_the_sequences(d, int8, lead, trail, hint
     assert cuda_attn.device_status() == (STATUS_PAGE if lead else 0)
     if not int8:
         assert same(before[0], c.k_cache)  # the new tokens' own keys were written, and nothing else
+
+
+# ------------------------------------------------------------------------------------------------ values that are not finite
+
+
+@both_kernels
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("dtype", [F16, BF16])
+def test_a_nan_of_a_16_bit_key_reaches_the_rows_that_see_it(dtype, d, hint):
+    """At every place of a stretch of keys, the causal edge among them; no other row changes."""
+    c = Case([5], [300], 2, 2, d, 16, dtype, False)
+    clean = attend(c, True, hint)
+    ids, place = c.places(0, 300)
+    for j in list(range(0, 300, 37)) + list(range(262, 300)):
+        at = (ids[j], 0, place[j], j % d)
+        was = c.k_cache[at].clone()
+        c.k_cache[at] = float("nan")
+        out = attend(c, True, hint)
+        sees = max(0, j - 295)  # the first row that does
+        assert out[sees:, :2].isnan().all(), j
+        assert torch.equal(out[:sees], clean[:sees]) and torch.equal(out[:, 2:], clean[:, 2:]), j
+        c.k_cache[at] = was
+
+
+@both_kernels
+@pytest.mark.parametrize("dtype", [F16, BF16])
+def test_infinite_keys(dtype, hint):
+    """An infinite key gives an infinite score: NaN where it is positive, no weight where it is negative. In the first tile
+    of a row and in a later one."""
+    for j in list(range(3, 19)) + list(range(250, 266)):
+        c = Case([4], [300], 1, 8, 128, 16, dtype, False)
+        ids, place = c.places(0, 300)
+        c.k_cache[ids[j], 0, place[j], 5] = c.keys[0][j, 0, 5] = float("inf")
+        c.q[..., 5] = torch.where(c.q[..., 5].abs() < 0.25, 0.25, c.q[..., 5])
+        out = attend(c, True, hint)
+        ref, size = c.attention64(True)
+        up = c.q[..., 5] > 0
+        assert out[up].isnan().all(), j
+        assert_attention(out[~up], ref[~up], size[~up], dtype)
