@@ -138,8 +138,8 @@ __device__ __forceinline__ float row_max(const float (&s)[N]) {
 }
 
 // p = exp2(s * scale - sub) of 64 scores as packed 16-bit pairs; returns the sum of the unrounded values. Every fourth pair
-// by the FMA pipe's polynomial, as in attn_tc_sm100.cu; its least value is 2^-125, which is nothing beside a row's largest
-// p (at least 2^-8) unless it meets a value of 1e30.
+// by the FMA pipe's polynomial, as in attn_tc_sm100.cu. That one's least value is 2^-125, in fp16 a zero; bf16 would keep it,
+// and a key that the row does not see may have a value of 1e38, so bf16 takes the polynomial that ends in an exact zero.
 template <bool BF16, int OFF>
 __device__ __forceinline__ float softmax64(const float (&s)[BN], float scale_log2, float sub, uint32_t (&p)[32]) {
   const float2 sc = make_float2(scale_log2, scale_log2), nm = make_float2(-sub, -sub);
@@ -148,7 +148,7 @@ __device__ __forceinline__ float softmax64(const float (&s)[BN], float scale_log
   for (int c = 0; c < 32; ++c) {
     float2 x = fma2(make_float2(s[OFF + 2 * c], s[OFF + 2 * c + 1]), sc, nm);
     if ((0x09 >> (c & 7)) & 1) {
-      x = exp2_fma2(x);
+      x = BF16 ? exp2_fma2_zero(x) : exp2_fma2(x);
     } else {
       x.x = ex2(x.x);
       x.y = ex2(x.y);

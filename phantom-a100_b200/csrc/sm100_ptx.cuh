@@ -378,6 +378,21 @@ __device__ __forceinline__ float2 exp2_fma2(float2 x) {
                      __uint_as_float(__float_as_uint(p.y) + (__float_as_uint(t.y) << 23)));
 }
 
+// The same with an exact 0 for x <= -127: the cubic is 1 at f = 0 (fitted so: 1.0e-4), whose bits less 127 << 23 are none.
+__device__ __forceinline__ float2 exp2_fma2_zero(float2 x) {
+  constexpr float kMagic = 12582912.0f;
+  x.x = fmaxf(x.x, -127.f);
+  x.y = fmaxf(x.y, -127.f);
+  const float2 t = add2(x, make_float2(kMagic, kMagic));
+  const float2 r = add2(t, make_float2(-kMagic, -kMagic));
+  const float2 f = fma2(r, make_float2(-1.f, -1.f), x);
+  float2 p = fma2(make_float2(0.0550089329f, 0.0550089329f), f, make_float2(0.2422109693f, 0.2422109693f));
+  p = fma2(p, f, make_float2(0.6932829022f, 0.6932829022f));
+  p = fma2(p, f, make_float2(1.f, 1.f));
+  return make_float2(__uint_as_float(__float_as_uint(p.x) + (__float_as_uint(t.x) << 23)),
+                     __uint_as_float(__float_as_uint(p.y) + (__float_as_uint(t.y) << 23)));
+}
+
 // Pack two fp32 values into one 32-bit word of two 16-bit values (lo in bits 0-15), round to nearest.
 template <bool BF16>
 __device__ __forceinline__ uint32_t pack2(float lo, float hi) {

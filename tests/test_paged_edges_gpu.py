@@ -155,3 +155,21 @@ def test_infinite_keys(dtype, hint):
         up = c.q[..., 5] > 0
         assert out[up].isnan().all(), j
         assert_attention(out[~up], ref[~up], size[~up], dtype)
+
+
+@both_kernels
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("dtype,int8,huge", [(F16, False, 6e4), (BF16, False, 3e38), (BF16, True, 3e38)])
+def test_hidden_values_of_any_size_have_no_weight(dtype, int8, huge, d, hint):
+    """The last 60 new tokens' values are the largest finite numbers; the rows before do not see them."""
+    c = Case([200, 130], [200, 700], 2, 2, d, 16, dtype, int8)
+    clean = attend(c, True, hint)
+    for b, t in enumerate(c.kv):
+        ids, place = (x[t - 60:] for x in c.places(b, t))
+        if int8:
+            c.v_scale[ids, :, place] = huge / 127
+        else:
+            c.v_cache[ids, :, place] = huge
+    out = attend(c, True, hint)
+    for rows in (slice(0, 140), slice(200, 270)):
+        assert torch.equal(out[rows], clean[rows])
