@@ -94,7 +94,7 @@ struct RowBlocks {
   __device__ int key_end(const Seq& x, int rb) const {
     if (!causal) return x.len;
     const int last = min(x.n * group - 1, rb * BR + BR - 1) / group;
-    return min(max(x.len - x.n + last + 1, 0), x.len);
+    return min(max(x.off + last + 1, 0), x.len);
   }
   __device__ long long head_tiles(const Seq& x) const { return sum_tiles(*this, x); }
 };
@@ -154,7 +154,7 @@ __device__ __forceinline__ uint32_t turn(uint32_t x) {
 // What the records' producer tells the others of a unit (48 bytes).
 struct Unit {
   int cnt, tile0, end, id;    // its tiles here, the first of them; the keys that its rows see; id -1 ends the roles
-  int len, n, row0, tok0;     // the sequence: cached and new tokens; the unit's first row; packed place of its first token
+  int off, n, row0, tok0;     // the sequence: where its new tokens begin, how many; the unit's first row; its packed place
   int h, c0, c1, b;           // key head; the first and the last CTA that have tiles of it; the sequence
 };
 
@@ -203,7 +203,7 @@ attn_rows(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUten
       const int4* r = ring + 3 * (u % kUnitRing);
       const int4 a = r[0], b = r[1], c = r[2];
       x.cnt = a.x, x.tile0 = a.y, x.end = a.z, x.id = a.w;
-      x.len = b.x, x.n = b.y, x.row0 = b.z, x.tok0 = b.w;
+      x.off = b.x, x.n = b.y, x.row0 = b.z, x.tok0 = b.w;
       x.h = c.x, x.c0 = c.y, x.c1 = c.z, x.b = c.w;
     }
     return x;
@@ -238,7 +238,7 @@ attn_rows(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUten
         if (elect_one()) {
           int4* r = ring + 3 * (nu % kUnitRing);
           r[0] = make_int4(w.cnt, w.tile, p.blocks.key_end(w.x, w.blk), nu);
-          r[1] = make_int4(w.x.len, w.x.n, row0, w.x.tok0);
+          r[1] = make_int4(w.x.off, w.x.n, row0, w.x.tok0);
           r[2] = make_int4(w.h, own.x, own.y, w.b);
           mbar_arrive(q_full(nu));
         }
@@ -484,7 +484,7 @@ attn_rows(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUten
   for (int u = 0;; ++u) {
     const Unit x = next_unit(u);
     if (x.id < 0) break;
-    const int R = x.n * group, row0 = x.row0, off = x.len - x.n, end = x.end;
+    const int R = x.n * group, row0 = x.row0, off = x.off, end = x.end;
     // the queries as B operands: of row 8 nt + g; 8-bit caches: columns in the order that their bytes come in (4 t4 ... + 3
     // of 16). Keys that the rows 8 nt + 2 t4 + e of this lane's scores see. (Rows past the last hold anything; no row's
     // numbers meet another's.)
@@ -527,12 +527,12 @@ attn_rows(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUten
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
         const int row = row0 + nt * 8 + 2 * t4 + e;
-        lim[nt][e] = row >= R ? 0 : causal ? min(x.len, off + row / group + 1) : x.len;
+        lim[nt][e] = row >= R ? 0 : causal ? min(end, off + row / group + 1) : end;
       }
     }
     __syncwarp();
     if (lane == 0) mbar_arrive(q_empty(u));
-    const int lim_least = causal ? max(0, min(x.len, off + row0 / group + 1)) : x.len;  // of the block's rows
+    const int lim_least = causal ? max(0, min(end, off + row0 / group + 1)) : end;  // of the block's rows
     float m[NT][2], l[NT][2], o[D / 16][NT][4];
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {

@@ -76,13 +76,13 @@ struct TokenBlocks {
   static constexpr float kPart = 0.1f;
   __device__ int count(const Seq& x) const { return (x.n + per - 1) / per; }
   __device__ int key_end(const Seq& x, int blk) const {
-    return causal ? min(max(x.len - x.n + min(x.n, (blk + 1) * per), 0), x.len) : x.len;
+    return causal ? min(max(x.off + min(x.n, (blk + 1) * per), 0), x.len) : x.len;
   }
   __device__ long long head_tiles(const Seq& x) const {
-    const int c = count(x), off = x.len - x.n;
+    const int c = count(x), off = x.off;
     if (c < 3) return sum_tiles(*this, x);
     if (!causal) return (long long)c * tiles_of(*this, x, 0);
-    if (off < 0) return sum_tiles(*this, x);
+    if (off < 0 || off + x.n > x.len) return sum_tiles(*this, x);
     // sum over the c - 1 whole blocks of ceil((off + i per) / 128), i = 1 ... c - 1, and the last: a sum of
     // floor((a i + r) / m), taken by the Euclidean descent on (a, m)
     long long w = tiles_of(*this, x, c - 1), n = c - 1, a = per, r = off + per + kTile - 1, m = kTile;
@@ -120,8 +120,8 @@ struct Params {
 // What the producer tells the other roles of a unit (48 bytes).
 struct Unit {
   int cnt, tile0, end, has_b;  // its tiles here, the first of them; the keys it sees; whether it has a second query tile
-  int len, n, tok, tok0;       // the sequence: cached and new tokens; its new token that the unit begins with; packed place
-  int h, slot, id, b;          // key head; place of the partial result (-1: the unit is whole); id -1 ends the roles
+  int len, back, tok, tok0;    // the sequence: cached tokens, its new ones begin `back` before; the unit's first; packed place
+  int h, slot, n, b;           // key head; place of the partial result (-1: the unit is whole); new tokens, -1 ends the roles
 };
 
 // NaN if a score is: the polynomial of softmax64 loses NaNs, so the row's maximum carries them.
@@ -256,25 +256,25 @@ attn_chunk(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUte
   auto publish = [&](int u, const Unit& x) {
     int4* r = ring + 3 * (u % kUnitRing);
     r[0] = make_int4(x.cnt, x.tile0, x.end, x.has_b);
-    r[1] = make_int4(x.len, x.n, x.tok, x.tok0);
-    r[2] = make_int4(x.h, x.slot, x.id, x.b);
+    r[1] = make_int4(x.len, x.back, x.tok, x.tok0);
+    r[2] = make_int4(x.h, x.slot, x.n, x.b);
   };
   auto record = [&](int u) {
     const int4* r = ring + 3 * (u % kUnitRing);
     const int4 a = r[0], b = r[1], c = r[2];
     Unit x;
     x.cnt = a.x, x.tile0 = a.y, x.end = a.z, x.has_b = a.w;
-    x.len = b.x, x.n = b.y, x.tok = b.z, x.tok0 = b.w;
-    x.h = c.x, x.slot = c.y, x.id = c.z, x.b = c.w;
+    x.len = b.x, x.back = b.y, x.tok = b.z, x.tok0 = b.w;
+    x.h = c.x, x.slot = c.y, x.n = c.z, x.b = c.w;
     return x;
   };
   auto wait = [&](uint32_t bar, int parity, int code) {
     return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag, status, code)) != 0;
   };
-  // Next unit of a consuming role (its id is -1 at the end, or when a wait gave up).
+  // Next unit of a consuming role (its n is -1 at the end, or when a wait gave up).
   auto next_unit = [&](int u, bool& ok) -> Unit {
     Unit x;
-    x.id = -1;
+    x.n = -1;
     if ((ok = wait(q_full(u), (u >> 1) & 1, kErrMmaWait))) {
       x = record(u);
       __syncwarp();
@@ -283,14 +283,14 @@ attn_chunk(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUte
     return x;
   };
 
-  // A role that works ahead: the record of unit u as soon as it is published (id -1 at the end).
+  // A role that works ahead: the record of unit u as soon as it is published (n -1 at the end).
   auto take_unit = [&](int u, bool& ok) -> Unit {
     Unit x;
-    x.id = -1;
+    x.n = -1;
     if ((ok = wait(rec_full(u), (u / kUnitRing) & 1, kErrTmaWait))) {
       x = record(u);
       __syncwarp();
-      if (x.id >= 0 && lane == 0) mbar_arrive(unit_read(u));
+      if (x.n >= 0 && lane == 0) mbar_arrive(unit_read(u));
     }
     return x;
   };
@@ -356,7 +356,7 @@ attn_chunk(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUte
         __syncwarp();
         for (int nu = 0;; ++nu) {
           const Unit x = take_unit(nu, ok);
-          if (x.id < 0) break;
+          if (x.n < 0) break;
           begin_unit(x.b, x.h, x.tile0, x.end);
           for (int i = 0; ok && i < x.cnt; ++i) copy_tile((x.tile0 + i) * BN, x.end);
           if (!ok) break;
@@ -383,25 +383,25 @@ attn_chunk(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUte
       for (;; ++nu) {
         if (nu > 1 && !(ok = wait(unit_read(nu), ((nu >> 1) - 1) & 1, kErrTmaWait))) break;
         Unit x = {};
-        x.id = w.cnt > 0 ? nu : -1;
-        if (x.id >= 0) {
+        x.n = w.cnt > 0 ? w.x.n : -1;
+        if (x.n >= 0) {
           x.b = w.b;
           x.h = w.h;
           x.cnt = w.cnt;
           x.tile0 = w.tile;
           x.end = p.blocks.key_end(w.x, w.blk);
           x.tok = w.blk * p.blocks.per;
-          x.len = w.x.len, x.n = w.x.n, x.tok0 = w.x.tok0;
+          x.len = w.x.len, x.back = (int)min((long long)w.x.len - w.x.off, 0x7fffffffLL), x.tok0 = w.x.tok0;
           x.has_b = x.tok + p.tile_tokens < x.n;
           x.slot = x.cnt == w.nt ? -1 : w.place(blockIdx.x, w.tile == 0);
         }
         if (elect_one()) {
           publish(nu, x);
           mbar_arrive(rec_full(nu));
-          if (x.id < 0) mbar_arrive(q_full(nu));
+          if (x.n < 0) mbar_arrive(q_full(nu));
         }
         __syncwarp();
-        if (x.id < 0) {
+        if (x.n < 0) {
           ++nq;
           break;
         }
@@ -486,12 +486,12 @@ attn_chunk(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUte
       ks = none ? 0.f : p.ks[from * p.kss.page + x.h * p.kss.head + place];
       vs = none ? 0.f : p.vs[from * p.vss.page + x.h * p.vss.head + place];
     };
-    if (x.id >= 0) {
+    if (x.n >= 0) {
       begin_tile();
       for (int n = 0; n < N; ++n) load(n, k_base, k_off);
       load_scales();
     }
-    for (int t = 0, j = 0; ok && x.id >= 0; ++j) {
+    for (int t = 0, j = 0; ok && x.n >= 0; ++j) {
       // -- the tile's scales
       if (j >= 4 && !(ok = wait(sc_empty(j), (j / 4 - 1) & 1, kErrTmaWait))) break;
       float* scl = reinterpret_cast<float*>(smem + C::OFF_SCALE) + (j & 3) * 3 * BN;
@@ -534,7 +534,7 @@ attn_chunk(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUte
         x = take_unit(++nu, ok);
       }
       k_off = -1;
-      if (x.id >= 0) begin_tile();
+      if (x.n >= 0) begin_tile();
       s = t % C::STAGES;
       if (!ok || (t >= C::STAGES && !(ok = wait(kv_empty(s), (t / C::STAGES - 1) & 1, kErrTmaWait)))) break;
       dst = sbase + C::OFF_KV + s * C::TILE;
@@ -552,7 +552,7 @@ attn_chunk(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUte
         st_shared_v4(dst + at_lo + n * STEP * 128, w[0], w[1], w[2], w[3]);
         st_shared_v4(dst + at_hi + n * STEP * 128, w[4], w[5], w[6], w[7]);
       }
-      if (x.id >= 0) load_scales();
+      if (x.n >= 0) load_scales();
       fence_proxy_async_smem();
       __syncwarp();
       if (lane == 0) mbar_arrive(kv_full(s));
@@ -581,7 +581,7 @@ attn_chunk(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUte
       bool ok = true;
       for (;;) {
         const Unit x = next_unit(nu, ok);
-        if (x.id < 0) break;
+        if (x.n < 0) break;
         for (int q = 0; ok && q < x.cnt; ++q) {
           const int tk = tb + 2 * q, sk = tk % C::STAGES;
           if (!(ok = kv_wait(tk))) break;
@@ -633,7 +633,7 @@ attn_chunk(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUte
       bool ok = true;
       for (;; ++nu) {
         const Unit x = next_unit(nu, ok);
-        if (x.id < 0) break;
+        if (x.n < 0) break;
         for (int q = 0; ok && q < x.cnt; ++q) {
           const int tv = tb + 2 * q + 1, sv = tv % C::STAGES;
           if (!(ok = kv_wait(tv))) break;
@@ -697,12 +697,12 @@ attn_chunk(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUte
     bool ok = true;
     for (int nu = 0;; ++nu) {
       Unit x = next_unit(nu, ok);
-      if (x.id < 0) break;
+      if (x.n < 0) break;
       const int tb = tiles;  // the share's tiles before this unit
       tiles += x.cnt;
       if (g == 1 && !x.has_b) continue;
       const int tile_tok = x.tok + g * p.tile_tokens;
-      const int see = x.len - x.n + tile_tok + 1;  // causal: keys that the tile's first row sees
+      const int see = x.len - x.back + tile_tok + 1;  // causal: keys that the tile's first row sees
       const bool causal = p.blocks.causal;
       const int lim = causal ? min(x.len, see + row_tok) : x.len;
       const int lim_least = causal ? min(x.len, see) : x.len;

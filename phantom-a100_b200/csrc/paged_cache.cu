@@ -114,9 +114,9 @@ __device__ __forceinline__ int find_page(const PagedSeqs& s, int tok, int* place
   *place = 0;
   if (b >= s.batch) return -1;  // of no sequence: nothing wrong
   const Seq x = seq_of(s, b);
-  const int pos = x.len - (x.tok0 + x.n - tok);
+  const int pos = x.off + (tok - x.tok0);
   *place = pos & ((1 << s.page_log2) - 1);
-  if (pos >= 0 && tok >= x.tok0) return page_of(s, b, pos >> s.page_log2);
+  if (pos >= 0 && pos < x.len && tok >= x.tok0) return page_of(s, b, pos >> s.page_log2);
   if ((threadIdx.x & 31) == 0) atomicOr(s.status, PHANTOM_ATTN_STATUS_PAGE);
   return -1;
 }

@@ -7,9 +7,10 @@
 
 namespace phantom {
 
-// One sequence: its first packed token, new tokens, cached tokens.
+// One sequence: its first packed token, new tokens, cached tokens within its row of the page table, and the position of
+// its first new token. Token i of the new ones is at off + i, whatever had to be bounded; there may be no place for it.
 struct Seq {
-  int tok0, n, len;
+  int tok0, n, len, off;
 };
 
 __device__ __forceinline__ Seq seq_of(const PagedSeqs& s, int b) {
@@ -19,6 +20,7 @@ __device__ __forceinline__ Seq seq_of(const PagedSeqs& s, int b) {
   x.tok0 = min(max(c0, 0), s.total);
   x.n = min(max(c1, x.tok0), s.total) - x.tok0;
   x.len = (int)min((long long)max(len, 0), min(room, 0x7ffff000LL));
+  x.off = (int)max((long long)min(len, 0x7fff0000) - ((long long)c1 - x.tok0), -0x7fffffffLL);
   if (x.tok0 != c0 || x.tok0 + x.n != c1 || x.len != len) atomicOr(s.status, PHANTOM_ATTN_STATUS_PAGE);
   return x;
 }

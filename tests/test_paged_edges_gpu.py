@@ -83,6 +83,60 @@ def test_tokens_without_a_page_are_zeros(dtype, int8, d, causal, hint):
         assert same(was, now)
 
 
+@pytest.mark.parametrize("over", [1, 2, 5, 50])
+@pytest.mark.parametrize("dtype,int8", [(F16, False), (BF16, True)])
+def test_new_tokens_past_the_page_table(dtype, int8, over):
+    """kv_lens counts more tokens than the table's row has room for: the new tokens that have a place keep it, those past it
+    are not written and read as zeros; a token sees the cached ones before it, as many as there are."""
+    new, kv = [5, 140, 1], [160, 320, 320]  # whole pages: 10 and 20 of the table's 20, a length out of range in two rows
+    c = Case(new, kv, 2, 4, 128, 16, dtype, int8)
+    c.table = c.table[:, :20].contiguous()
+    c.lens[1:] += over
+    before, x = [p.clone() for p in pools(c)], torch.randn(146, 2, 128, device="cuda", dtype=dtype)
+    cuda_attn.paged_append(x, x, *c.where(), **c.scales())
+    assert cuda_attn.device_status() == STATUS_PAGE
+    packed, at = [], 0
+    for b, (n, t) in enumerate(zip(new, c.lens.tolist())):
+        for i in range(n):
+            j = t - n + i
+            if j < (160 if b == 0 else 320):
+                packed.append((at + i, int(c.table[b, j // 16]), j % 16))
+        at += n
+    rows, ids, place = (torch.tensor(y, device="cuda") for y in zip(*packed))
+    q, s = quantise64(x[rows])
+    for was, put in zip(before, (q, q, s, s) if int8 else (x[rows], x[rows])):
+        was[ids, :, place] = put
+    assert all(same(was, now) for was, now in zip(before, pools(c)))
+
+    soil((146, 2, 128), dtype), soil((146, 2, 128), dtype)
+    k, v = cuda_attn.paged_read(*c.where(), 146, dtype=dtype, **c.scales())
+    assert cuda_attn.device_status() == STATUS_PAGE
+    want = torch.zeros_like(k)
+    want[rows] = (q.float() * s[..., None]).to(dtype) if int8 else x[rows]
+    assert torch.equal(k, want) and torch.equal(v, want)
+
+    # the rows of tokens within the room: as with lengths that end there
+    for hint in (1, 4096):
+        out = attend(c, True, hint)
+        assert cuda_attn.device_status() == STATUS_PAGE
+        for b, (n, t) in enumerate(zip(new, c.lens.tolist())):
+            start = sum(new[:b])
+            room = 160 if b == 0 else 320
+            inside = max(0, n - max(0, t - room))
+            alone = [torch.tensor(y, dtype=torch.int32, device="cuda") for y in ([min(t, room)], [0, n])]
+            ask = c.q[start:start + n]
+            every = cuda_attn.paged_attn(ask, c.k_cache, c.v_cache, c.table[b:b + 1], *alone, **c.scales(), causal=False, max_new=hint)
+            past = torch.arange(n, device="cuda") >= inside
+            tol = 2.0 ** -7 if dtype == BF16 else 2.0 ** -10  # two sums of the same terms, rounded to 16 bits each
+            assert ((out[start:start + n] - every).abs()[past] <= tol * (1 + every.abs()[past])).all()
+            if inside:
+                alone[0][0], alone[1][1] = min(t, room), inside
+                some = cuda_attn.paged_attn(ask[:inside], c.k_cache, c.v_cache, c.table[b:b + 1], *alone, **c.scales(), max_new=hint)
+                diff = (out[start:start + inside] - some).abs()
+                assert (diff <= tol * (1 + some.abs())).all()
+    cuda_attn.device_status()
+
+
 # ------------------------------------------------------------------------------------------------ packed rows of no sequence
 
 
