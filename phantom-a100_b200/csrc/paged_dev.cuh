@@ -81,6 +81,8 @@ __device__ __forceinline__ long long sum_tiles(const Blocks& k, const Seq& x) {
 }
 
 // A whole warp walks one CTA's share; every value is uniform over the warp. Positions count tiles and units' own costs.
+// Lengths and offsets are read more than once, and a caller may (by mistake) have them change meanwhile: whatever the reads
+// give, the walk ends, and its units, blocks and owners are ones that exist.
 template <typename Blocks>
 struct Walk {
   static constexpr int kUnit = Blocks::kUnit;
@@ -144,6 +146,7 @@ struct Walk {
     if (by_unit) w = scan(units0, lane);
     long long before = 0;
     for (int i0 = 0;; i0 += 32) {
+      if (i0 >= s.batch) return;
       if (i0 > 0) w = scan(seq_part(i0 + lane), lane);
       const unsigned past = __ballot_sync(0xffffffffu, before + w > pos);
       if (past) {
@@ -157,8 +160,10 @@ struct Walk {
     }
     x = seq_of(s, b);
     const int count = k.count(x);
+    if (count == 0) return;
     const long long head = by_unit ? count : head_work(k, x);
     long long r = pos - before;
+    if (r >= head * s.heads) return;
     h = (int)quotient(r, head);
     r -= h * head;
     blk = 0;
@@ -167,6 +172,7 @@ struct Walk {
       r = 0;
     }
     for (int i0 = 0; !by_unit && count > 1; i0 += 32) {
+      if (i0 >= count) return;
       const int y = i0 + lane < count ? tiles_of(k, x, i0 + lane) + kUnit : 0;
       w = scan(y, lane);
       const unsigned past = __ballot_sync(0xffffffffu, w > r);
@@ -193,7 +199,7 @@ struct Walk {
   }
   __device__ int owner(long long pos) const {
     const long long big = more * (share + 1);
-    return (int)(pos < big ? quotient(pos, share + 1) : more + quotient(pos - big, share));
+    return (int)min(pos < big ? quotient(pos, share + 1) : more + quotient(pos - big, share), ctas - 1LL);
   }
   // A unit that several CTAs share: CTA c's part of it lies in the place 2 c + 1 if its first tile is c's, else 2 c.
   __device__ static int place(int cta, bool begins) { return 2 * cta + (begins ? 1 : 0); }
@@ -205,8 +211,10 @@ struct Walk {
       blk = 0;
       if (++h == s.heads) {
         h = 0;
-        do x = seq_of(s, ++b);
-        while (x.n == 0);
+        do {
+          if (++b >= s.batch) return;
+          x = seq_of(s, b);
+        } while (x.n == 0);
       }
     }
     nt = tiles_of(k, x, blk);
