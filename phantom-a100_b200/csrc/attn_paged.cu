@@ -313,7 +313,8 @@ attn_rows(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUten
     constexpr int PER = BR * D / 128;  // columns of a thread: 16, 8 or 4
     const int tid = threadIdx.x - 32 * kConsumers;
     const int r = tid / (128 / BR), col = (tid % (128 / BR)) * PER;
-    for (int u = 0;; ++u) {
+    int u = 0;
+    for (;; ++u) {
       const Unit x = next_unit(u);
       __syncwarp();
       if (x.id >= 0 && lane == 0) mbar_arrive(q_empty(u));
@@ -449,6 +450,17 @@ attn_rows(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUten
 #pragma unroll
         for (int i = 0; i < PER / 4; ++i)
           dst[i] = make_uint2(pack2<BF16>(acc[4 * i] * inv, acc[4 * i + 1] * inv), pack2<BF16>(acc[4 * i + 2] * inv, acc[4 * i + 3] * inv));
+      }
+    }
+    if (*abort_flag && warp == kConsumers) {
+      // A wait gave up: this CTA's parts from unit u on will not come, but they are counted, so that the last to be counted
+      // leaves 0 in each word. A replay of a graph has the same call's number: it would take a count that was left for its own.
+      Walk<Blocks> w;
+      w.start(p.s, p.blocks, blockIdx.x, gridDim.x);
+      for (int v = 0; w.cnt > 0; w.advance(p.s, p.blocks), ++v) {
+        const int2 own = w.owners(blockIdx.x);
+        if (v >= u && own.x != own.y && lane == 0) last_part(p.words + own.x, p.call, own.y - own.x + 1);
+        __syncwarp();
       }
     }
     return;

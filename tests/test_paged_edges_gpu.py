@@ -227,3 +227,48 @@ def test_hidden_values_of_any_size_have_no_weight(dtype, int8, huge, d, hint):
     out = attend(c, True, hint)
     for rows in (slice(0, 140), slice(200, 270)):
         assert torch.equal(out[rows], clean[rows])
+
+
+# ------------------------------------------------------------------------------------------------ after a wait that gave up
+
+
+def test_a_replay_after_one_that_gave_up():
+    """A captured call whose length grows to 6e8 tokens (all in one page) keeps a CTA at its part for longer than a wait's
+    limit of a second: the call ends soon after and says so. The counts of the parts that were done must not stay for the
+    next replays, which would join parts that are not there yet."""
+    heads, page, small, huge = 60, 1024, 1 << 16, 617 << 20
+    kc, vc = (torch.randn(1, heads, page, 128, device="cuda").to(BF16) for _ in "kv")
+    table = torch.zeros(1, 617 << 10, dtype=torch.int32, device="cuda")
+    lens = torch.tensor([small], dtype=torch.int32, device="cuda")
+    cu = torch.tensor([0, 1], dtype=torch.int32, device="cuda")
+    q = torch.randn(1, heads, 128, device="cuda").to(BF16)
+
+    def step():
+        return cuda_attn.paged_attn(q, kc, vc, table, lens, cu, max_new=1)
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        o = step()
+
+    def replays(n):
+        wrong = 0
+        for _ in range(n):
+            q.copy_(torch.randn(1, heads, 128, device="cuda"))
+            graph.replay()
+            got = o.clone()
+            wrong += not torch.equal(got, step())
+        return wrong
+
+    assert replays(20) == 0
+    lens.fill_(huge)
+    graph.replay()
+    status = cuda_attn.device_status()
+    assert status & 15 and not status & STATUS_PAGE
+    lens.fill_(small)
+    assert replays(40) == 0
+    del graph
