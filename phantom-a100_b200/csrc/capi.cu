@@ -443,6 +443,9 @@ int phantom_attn_paged_read(const phantom_paged_cache* cache, void* k, void* v, 
 int phantom_attn_paged(const phantom_paged_cache* cache, const void* q, long long q_token, long long q_head, void* o,
                        int total_new, int q_heads, int dtype, int causal, float scale, int max_new, void* stream) {
   const char* name = "paged_attn";
+  const float scale_log2 = scale * 1.4426950408889634f;  // as the kernels use it
+  if (max_new < 0 || !(scale_log2 - scale_log2 == 0.f))
+    return fail(PHANTOM_ATTN_ERR_INVALID, "%s: max_new must not be negative and scale must be finite", name);
   Device dev;
   PagedAttnArgs a{};
   int rc = check_paged(name, cache, total_new, dtype, &dev, &a.s);
@@ -452,8 +455,6 @@ int phantom_attn_paged(const phantom_paged_cache* cache, const void* q, long lon
                 cache->heads);
   if ((long long)total_new * (q_heads / cache->heads) > 0x7fffffffLL - 1024)
     return fail(PHANTOM_ATTN_ERR_UNSUPPORTED, "%s: query rows of a key head exceed 2^31 (total_new = %d)", name, total_new);
-  if (max_new < 0 || !(scale - scale == 0.f))
-    return fail(PHANTOM_ATTN_ERR_INVALID, "%s: max_new must not be negative and scale must be finite", name);
   if (!stride_ok(q_token, 2) || !stride_ok(q_head, 2))
     return fail(PHANTOM_ATTN_ERR_INVALID, "%s: strides of q must be multiples of 16 bytes", name);
   if ((rc = check_paged_ptr(name, "q", q, dev.id, 16)) != PHANTOM_ATTN_OK ||

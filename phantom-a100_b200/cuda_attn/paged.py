@@ -20,6 +20,8 @@ device_status() says so (bit 512).
 """
 from __future__ import annotations
 
+import ctypes
+
 import torch
 
 from . import _ext  # defined above this module's import in the package
@@ -55,7 +57,7 @@ def paged_attn(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, pa
     sqrt(d) by default. `max_new`: the largest number of new tokens of a sequence, a hint that picks the kernel and changes
     nothing else (default: the average). 16-bit values within kv_lens[b] must be finite, those that the causal mask hides
     too; what the pages hold past it may be anything."""
-    if scale is not None and not 0.0 < abs(scale) < float("inf"):
-        raise RuntimeError(f"paged_attn: scale must be finite and not zero (got {scale})")
+    if scale is not None and not 0.0 < abs(ctypes.c_float(scale).value) < float("inf"):
+        raise RuntimeError(f"paged_attn: scale must be finite and not zero in float32 (got {scale})")
     return _ext().paged_attn(q, k_cache, v_cache, page_table, kv_lens, cu_new, k_scale, v_scale, causal, max_new,
                              0.0 if scale is None else scale)

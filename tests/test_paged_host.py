@@ -91,3 +91,20 @@ def test_page_pool():
     assert pool.reserve(3, 80) and not pool.free
     pool.release(2), pool.release(3)
     assert sorted(pool.free) == list(range(6))
+
+
+@pytest.mark.parametrize("scale", [1e-50, -1e-46, 0.0, 1e39, -1e300, float("nan"), float("-inf")])
+def test_scales_that_float32_does_not_hold(scale):
+    """The library takes a float, and 0 for the default."""
+    kc = torch.zeros(4, 2, 16, 64, dtype=torch.float16)
+    i = torch.zeros(1, 2, dtype=torch.int32)
+    with pytest.raises(RuntimeError, match="scale must be finite and not zero"):
+        cuda_attn.paged_attn(torch.zeros(1, 4, 64, dtype=torch.float16), kc, kc, i, i[0, :1], i[0], scale=scale)
+
+
+def test_scales_that_the_kernels_cannot_use(lib):
+    """They multiply it with log2(e) first. (Before anything else is looked at; scales in range pass, to the next refusal.)"""
+    for scale, text in ((3e38, "scale must be finite"), (-3e38, "scale must be finite"), (float("inf"), "scale must be finite"),
+                        (float("nan"), "scale must be finite"), (2e38, "null cache"), (1e-40, "null cache")):
+        rc = lib.lib.phantom_attn_paged(None, 4096, 512, 64, 4096, 3, 8, F16, 1, scale, 0, None)
+        assert rc == ERR_INVALID and text in lib.last_error(), (scale, lib.last_error())
