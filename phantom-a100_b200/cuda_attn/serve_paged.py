@@ -21,9 +21,13 @@ class PagePool:
     """Free pages of a pool, and which of them each sequence has."""
 
     def __init__(self, pages: int, page: int):
-        self.page = page
+        self.page, self.pages = page, pages
         self.free = list(range(pages - 1, -1, -1))
         self.of: dict[int, list[int]] = {}
+
+    def holds(self, tokens: int) -> bool:
+        """Whether `tokens` tokens of a sequence fit when nothing else is there."""
+        return -(-tokens // self.page) <= self.pages
 
     def reserve(self, seq: int, tokens: int) -> bool:
         """Give a sequence the pages that `tokens` tokens need; False, and nothing changed, if there are not enough."""
@@ -50,6 +54,8 @@ class Request:
 class Server:
     def __init__(self, heads: int = 8, group: int = 4, d: int = 128, page: int = 16, pages: int = 512, vocab: int = 1000,
                  dtype: torch.dtype = torch.bfloat16, int8: bool = False, chunk: int = 256, seed: int = 0, device: str = "cuda"):
+        if chunk < 1:
+            raise ValueError(f"a chunk has at least one token (got {chunk})")
         g = torch.Generator(device=device).manual_seed(seed)
         self.heads, self.group, self.d, self.chunk, self.dtype, self.device = heads, group, d, chunk, dtype, device
 
@@ -69,6 +75,14 @@ class Server:
         self.requests: dict[int, Request] = {}
 
     def submit(self, prompt: list[int], want: int) -> int:
+        """Queue a request for `want` tokens after a prompt; one that could never run is refused."""
+        vocab = self.wq.shape[0]
+        if not prompt or want < 1:
+            raise ValueError(f"a request needs a prompt and at least one token to decode (got {len(prompt)} and {want})")
+        if not all(0 <= t < vocab for t in prompt):
+            raise ValueError(f"a prompt's tokens must be from 0 to {vocab - 1}")
+        if not self.pool.holds(len(prompt) + want):
+            raise ValueError(f"{len(prompt)} + {want} tokens exceed the pool of {self.pool.pages} pages of {self.pool.page} tokens")
         seq = len(self.requests)
         self.requests[seq] = Request(prompt, want, list(prompt))
         self.waiting.append(seq)
@@ -85,13 +99,15 @@ class Server:
         return [torch.tensor(x, dtype=torch.int32, device=self.device) for x in (rows, lens, cu)]
 
     def step(self) -> list[int]:
-        """One step of all sequences that have room; the finished ones, still in the cache."""
+        """One step of all sequences that have room; the finished ones, still in the cache until their pages are released."""
         from . import paged_append, paged_attn
         while self.waiting:
             r = self.requests[self.waiting[0]]
             if not self.pool.reserve(self.waiting[0], len(r.prompt) + r.want):
                 break
             self.running.append(self.waiting.pop(0))
+        if not self.running and self.waiting:
+            raise RuntimeError("no room for the next request: finished sequences keep their pages until they are released")
         if not self.running:
             return []
         seqs, reqs = list(self.running), [self.requests[s] for s in self.running]
@@ -161,8 +177,11 @@ def main(argv=None) -> int:
     ap.add_argument("--dtype", choices=["fp16", "bf16"], default="bf16")
     a = ap.parse_args(argv)
     from . import device_status
-    server, worst, steps = run(a.requests, pages=a.pages, page=a.page, chunk=a.chunk, int8=a.int8,
-                               dtype={"fp16": torch.float16, "bf16": torch.bfloat16}[a.dtype])
+    try:
+        server, worst, steps = run(a.requests, pages=a.pages, page=a.page, chunk=a.chunk, int8=a.int8,
+                                   dtype={"fp16": torch.float16, "bf16": torch.bfloat16}[a.dtype])
+    except ValueError as e:
+        ap.error(str(e))
     tokens = sum(len(r.tokens) for r in server.requests.values())
     print(f"served {a.requests} requests, {tokens} tokens in {steps} steps; largest distance from the dense kernel {worst:.2e}, "
           f"{len(server.pool.free)} of {a.pages} pages free, device status {device_status()}")

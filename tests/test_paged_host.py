@@ -108,3 +108,31 @@ def test_scales_that_the_kernels_cannot_use(lib):
                         (float("nan"), "scale must be finite"), (2e38, "null cache"), (1e-40, "null cache")):
         rc = lib.lib.phantom_attn_paged(None, 4096, 512, 64, 4096, 3, 8, F16, 1, scale, 0, None)
         assert rc == ERR_INVALID and text in lib.last_error(), (scale, lib.last_error())
+
+
+def test_requests_that_could_never_run_are_refused():
+    """They would wait at the head of the queue for good, and all behind them."""
+    from cuda_attn.serve_paged import Server
+    with pytest.raises(ValueError, match="at least one token"):
+        Server(heads=1, group=1, d=64, chunk=0, device="cpu")
+    s = Server(heads=1, group=1, d=64, page=16, pages=5, vocab=50, device="cpu")
+    for prompt, want, text in (([1] * 70, 11, "exceed the pool"), ([1] * 81, 1, "exceed the pool"), ([], 3, "needs a prompt"),
+                               ([1, 2], 0, "at least one token"), ([1, 50], 2, "from 0 to 49"), ([-1], 2, "from 0 to 49")):
+        with pytest.raises(ValueError, match=text):
+            s.submit(prompt, want)
+    assert not s.waiting and not s.requests and s.step() == []
+    s.submit([1] * 70, 10)
+    assert s.pool.reserve(99, 16)  # a finished sequence that nobody released
+    with pytest.raises(RuntimeError, match="released"):
+        s.step()
+
+
+def test_serving_command_refuses_a_pool_that_is_too_small(monkeypatch, capsys):
+    from cuda_attn import serve_paged
+
+    def small(requests, **kw):
+        serve_paged.Server(heads=1, group=1, d=64, device="cpu", page=kw["page"], pages=kw["pages"]).submit([1] * 900, 39)
+    monkeypatch.setattr(serve_paged, "run", small)
+    with pytest.raises(SystemExit) as e:
+        serve_paged.main(["--pages", "50"])
+    assert e.value.code == 2 and "exceed the pool of 50 pages" in capsys.readouterr().err
