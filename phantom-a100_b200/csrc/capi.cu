@@ -519,9 +519,10 @@ int phantom_attn_device_status(int* status) {
   const int v = v_main | (v_noalloc != 0 ? v_noalloc | PHANTOM_ATTN_STATUS_NOALLOC : 0);
   *status = v;
   g_last_error.clear();
-  return v == 0 ? PHANTOM_ATTN_OK : fail(PHANTOM_ATTN_ERR_DEVICE, "device status 0x%x: %s", v,
-                                           v == PHANTOM_ATTN_STATUS_PAGE ? "a paged call's length, offset or page id was out of range"
-                                                                         : "a bounded wait expired");
+  if (v == 0) return PHANTOM_ATTN_OK;
+  const bool page = (v & PHANTOM_ATTN_STATUS_PAGE) != 0, wait = (v & ~PHANTOM_ATTN_STATUS_PAGE) != 0;
+  return fail(PHANTOM_ATTN_ERR_DEVICE, "device status 0x%x: %s%s%s", v, wait ? "a bounded wait expired" : "",
+              wait && page ? "; " : "", page ? "a paged call's length, offset or page id was out of range" : "");
 }
 
 int phantom_attn_wait_expiry_probe(void* stream) {

@@ -1,4 +1,6 @@
 """GPU: the paged entry points where their inputs are out of range, not finite or extreme, and what a failed call leaves."""
+import ctypes
+
 import pytest
 import torch
 
@@ -230,6 +232,21 @@ def test_hidden_values_of_any_size_have_no_weight(dtype, int8, huge, d, hint):
 
 
 # ------------------------------------------------------------------------------------------------ after a wait that gave up
+
+
+def test_the_status_names_all_that_happened(capi):
+    """A wait that gave up does not hide that a page was out of range too, nor the reverse."""
+    status = ctypes.c_int()
+    c = Case([1], [40], 1, 1, 64, 16, F16, False)
+    c.table.fill_(-1)
+    for probe, page in ((False, True), (True, True)):
+        if page:
+            attend(c)
+        if probe:
+            capi.wait_expiry_probe()
+        assert capi.lib.phantom_attn_device_status(ctypes.byref(status)) != 0
+        said = capi.last_error()
+        assert ("wait expired" in said) == probe and ("out of range" in said) == page, said
 
 
 def test_a_replay_after_one_that_gave_up():
