@@ -231,6 +231,32 @@ def test_hidden_values_of_any_size_have_no_weight(dtype, int8, huge, d, hint):
         assert torch.equal(out[rows], clean[rows])
 
 
+@both_kernels
+@pytest.mark.parametrize("int8", [False, True])
+def test_large_scores_stay_between_the_values(int8, hint):
+    """Scores in the hundreds: a softmax of one or two keys, which none of an output's columns leaves: beyond the least and the
+    largest value that its row sees lies only what rounding the probabilities and the output moves it by (paged_case)."""
+    c = Case([3, 200], [700, 300], 2, 2, 128, 16, BF16, int8, scale=8.0)
+    c.q.mul_(8.0)
+    out = attend(c, True, hint).double()
+    at = 0
+    for b, (n, t) in enumerate(zip(c.new, c.kv)):
+        v = c.values[b]
+        lo, hi, size = (f(0)[0][t - n:].repeat_interleave(2, 1) for f in (v.cummin, v.cummax, v.abs().cummax))
+        tol = (U[BF16] + 2 * (2.0 ** -11 if int8 else U[BF16]) + 2.0 ** -12) * size
+        o = out[at:at + n]
+        assert ((o >= lo - tol) & (o <= hi + tol)).all()
+        at += n
+
+
+@both_kernels
+@pytest.mark.parametrize("dtype,int8", [(F16, False), (BF16, False), (BF16, True)])
+def test_a_scale_of_next_to_nothing(dtype, int8, hint):
+    """The least scales that float32 holds: every key that a row sees has the same weight."""
+    c = Case([2, 130], [300, 200], 1, 4, 64, 16, dtype, int8)
+    assert_attention(attend(c, True, hint, 1e-40), *c.attention64(True, 0.0), dtype, int8)
+
+
 # ------------------------------------------------------------------------------------------------ after a wait that gave up
 
 
