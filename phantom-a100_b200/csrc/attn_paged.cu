@@ -12,10 +12,11 @@
 //     are turned around by movmatrix, and meet V^T the same way. With queries as the 16-high operand a group of 4 or 8
 //     heads left half of every instruction and of the softmax unused (812 instructions for 32 keys of a key head, all roles
 //     counted, against 610).
-//   * Work is cut evenly: all (sequence, head, row block) units in a row, tiles of 64 or 128 keys, and every CTA takes its share
-//     (paged_dev.cuh). Ragged lengths then cost nothing, and one long sequence spreads over the GPU. The parts of a unit
-//     that several CTAs share (fp32 rows, reference maximum, sum) are joined in the order of the CTAs by the one that
-//     finishes last: the result depends on the lengths and the GPU's SM count alone.
+//   * Work is cut evenly: all (sequence, head, row block) units in a row, tiles of 64 or 128 keys, and every CTA takes its
+//     share (paged_dev.cuh). Ragged lengths then cost nothing, and one long sequence spreads over the GPU. The parts of a
+//     unit that several CTAs share (fp32 rows, reference maximum, sum) are joined in the order of the CTAs by the one that
+//     finishes last: a call's result does not depend on which does. (It depends on the lengths of the whole batch, on the
+//     GPU's SM count and on the choice of kernel and unit in capi.cu.)
 //   * Producer warps for keys and for values read the page table and keep a ring of tiles in flight by TMA (a box per page,
 //     swizzled, so that pages of 16 tokens land as one conflict-free tile), two tiles to each pair of consumer warps. A
 //     third brings the queries.
@@ -30,7 +31,9 @@
 // a power of two for each row, exact but for what is below 2^-31 of the row's largest: fp16's 10 bits take a byte as it is,
 // where bf16 needs a subtraction for each (contexts of 2000 to 16383 tokens, pages of 64: 60.6 us, and 62.7 in bf16). The
 // key's scale multiplies the score, and the value's goes into the exponent: p'_j = 2^(s_j + log2 vs_j - m') is p_j vs_j
-// normalised to at most 1, whatever the scales, and is rounded to fp16 once; the sum adds p'_j / vs_j.
+// normalised to at most 1, whatever the scales, and is rounded to fp16 once; the sum adds p'_j / vs_j. (fp32 spans the scales
+// that meet in a row: one 2^126 below what has the largest p'_j loses its weight. A vector of zeros counts as 2^-100, so
+// values of 1e10 beside vectors of zeros are the limit.)
 #include <cuda.h>
 #include <math_constants.h>
 
@@ -50,7 +53,8 @@ constexpr int kUnitRing = 4;
 constexpr int kErrCopyWait = 1, kErrTileWait = 4, kErrJoinWait = 8;
 
 // Warps: eight consumers, in pairs that take the tiles in turn; the joiners; three producers and, completing their warpgroup,
-// one that zeroes the rows of no sequence. Registers (setmaxnreg, by warpgroup): 512 threads launch with 128 each; 2 * 168 + 104 + 72 = 4 * 128.
+// one that zeroes the rows of no sequence. Registers (setmaxnreg, by warpgroup): 512 threads launch with 128 each;
+// 2 * 168 + 104 + 72 = 4 * 128.
 constexpr int kConsumers = 8, PRODUCER = kConsumers + kJoiners, kThreads = 32 * (PRODUCER + 4);
 constexpr int kRegsConsumer = 168, kRegsJoiner = 104, kRegsProducer = 72;
 
@@ -85,7 +89,7 @@ struct Cfg {
 // Units of 8 NT rows; tiles of BN keys.
 template <int NT, int BN>
 struct RowBlocks {
-  int group, causal, heads;
+  int group, causal;
   // Measured (us): kJoin 8 | 5: 4 sequences of 500 tokens 10.7 | 12.0, 8 of 700 12.6 | 15.0, 32 of 200 to 4095 the same.
   // kPart 0.4 | 0.8: one of 4096 14.3 | 15.6, of 1024 11.9 | 12.1; 16 rows, 0.5 | 2: one of 1000 17.3 | 23.3.
   static constexpr int kTile = BN, kUnit = 2, kJoin = 8, BR = 8 * NT;
@@ -473,9 +477,9 @@ attn_rows(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUten
   constexpr int KEYS = 16 * MT;  // that go through this warp at a time
   const int kr = (warp & 1) * (BN / 2);  // its first key of its pair's tiles
   // Where this lane's rows for ldmatrix lie in a tile: 16 keys from kr + KEYS sub + 16 mt, matrices (keys 0-7, 8-15) x
-  // (first, second 16-byte chunk of a pair); V^T of 16-bit values has the two the other way around. Boxes of min(page, 64) tokens, each
-  // [64-column block][token][ROW bytes]; a chunk lies at its number ^ the row's swizzle, so stepping over pairs of chunks
-  // is an XOR with 32 times the pair's number.
+  // (first, second 16-byte chunk of a pair); V^T of 16-bit values has the two the other way around. Boxes of
+  // min(page, BN) tokens, each [64-column block][token][ROW bytes]; a chunk lies at its number ^ the row's swizzle, so
+  // stepping over pairs of chunks is an XOR with 32 times the pair's number.
   const int box_log2 = min(p.s.page_log2, BN == 64 ? 6 : 7), blk_stride = C::ROW << box_log2;
   constexpr int AT = C::BLOCKS == 1 ? 1 : MT;  // one column block: 16 rows further on is a constant away
   static_assert(C::SUB == 1 || C::BLOCKS == 1);
@@ -837,7 +841,7 @@ cudaError_t launch(const PagedAttnArgs& a, int dev) {
   char* base = static_cast<char*>(block);
   constexpr int BN = C::BN;
   Params<NT, BN> p{a.s, static_cast<const uint16_t*>(a.q), a.q_token, a.q_head, static_cast<uint16_t*>(a.o), a.ks, a.vs, a.kss, a.vss,
-               RowBlocks<NT, BN>{a.group, a.causal ? 1 : 0, a.s.heads},
+               RowBlocks<NT, BN>{a.group, a.causal ? 1 : 0},
                (INT8 ? a.scale : fabsf(a.scale)) * 1.4426950408889634f, !INT8 && a.scale < 0.f ? 0x80008000u : 0u,
                reinterpret_cast<float*>(base), reinterpret_cast<float2*>(base + part_bytes),
                reinterpret_cast<unsigned long long*>(base + part_bytes + ml_bytes), next_call()};

@@ -15,8 +15,10 @@
 //     scales take no part in the products: the softmax multiplies a key's scale into the score and puts the value's into
 //     the exponent, as in attn_paged.cu.
 //
-// The probabilities are rounded to the 16-bit type of V (fp16 for an 8-bit cache), as tcgen05.mma wants P and V of one type: half an ulp of each,
-// which adds to the output an error of the size of its own rounding (sqrt(2) times in all).
+// The probabilities are rounded to the 16-bit type of V (fp16 for an 8-bit cache), as tcgen05.mma wants P and V of one type:
+// half an ulp of each, which adds to the output an error of the size of its own rounding (sqrt(2) times in all); their sum
+// is of the unrounded ones, in fp32. For bf16 that is coarser than fused_tc, which stages V as fp16: here that would be a
+// pass over the cache, or P as hi + lo half as many matrix instructions again.
 #include <cuda.h>
 #include <math_constants.h>
 
@@ -71,7 +73,7 @@ struct Cfg {
 
 // Units of `per` new tokens; tiles of 128 keys.
 struct TokenBlocks {
-  int per, causal, heads;
+  int per, causal;
   static constexpr int kTile = BN, kUnit = 4, kJoin = 5;
   static constexpr float kPart = 0.1f;
   __device__ int count(const Seq& x) const { return (x.n + per - 1) / per; }
@@ -1019,7 +1021,7 @@ cudaError_t launch(const PagedAttnArgs& a, int dev) {
   void* block = nullptr;
   const size_t part_bytes = (size_t)ctas * 4 * BM * D * sizeof(float);
   if ((e = scratch_alloc(dev, ml_bytes + part_bytes + (size_t)ctas * 2 * sizeof(int4), a.stream, &block)) != cudaSuccess) return e;
-  Params p{a.s, TokenBlocks{2 * tile_tokens, a.causal ? 1 : 0, a.s.heads}, a.group, tile_tokens, static_cast<uint16_t*>(a.o),
+  Params p{a.s, TokenBlocks{2 * tile_tokens, a.causal ? 1 : 0}, a.group, tile_tokens, static_cast<uint16_t*>(a.o),
            (INT8 ? a.scale : fabsf(a.scale)) * 1.4426950408889634f, !INT8 && a.scale < 0.f ? 1 : 0,
            static_cast<const int8_t*>(a.kc), static_cast<const int8_t*>(a.vc), a.ks, a.vs, a.kcs, a.vcs, a.kss, a.vss,
            reinterpret_cast<float4*>(static_cast<char*>(block) + ml_bytes), static_cast<float2*>(block),

@@ -473,11 +473,13 @@ int phantom_attn_paged(const phantom_paged_cache* cache, const void* q, long lon
   a.causal = causal != 0;
   a.scale = scale != 0.f ? scale : 1.f / sqrtf((float)cache->head_dim);
   a.stream = static_cast<cudaStream_t>(stream);
-  // Query rows of one key head in one sequence, as expected. Few go to the rows kernel, which reads the keys for every 8 (8-bit
-  // caches: or 16) of them, more to the chunk kernel, which takes up to 256 at a time but starts and ends slower. Measured (us, rows / chunk; 8 key heads, d = 128). 16-bit, 32 contexts of 2000: 8 rows 50 / 69, 16 rows 89 / 70;
-  // 8-bit: 16 rows, in units of 8, 82 / 110, 32 rows 153 / 112. While the rows kernel's reads are short (64 MB) the difference
-  // in start and end decides: 24 rows of 4 contexts of 1000: 15 / 20, 8-bit 16 / 24; of 4 of 300: 9 / 18; past the bound, of 4
-  // of 4000: 35 / 28. The host knows no lengths, so what the page table has room for is taken.
+  // Query rows of one key head in one sequence, as expected. Few go to the rows kernel, which reads the keys for every 8
+  // (8-bit caches: or 16) of them, more to the chunk kernel, which takes up to 256 at a time but starts and ends slower.
+  // Measured (us, rows / chunk; 8 key heads, d = 128). 16-bit, 32 contexts of 2000: 8 rows 50 / 69, 16 rows 89 / 70; 8-bit:
+  // 16 rows, in units of 8, 82 / 110, 32 rows 153 / 112. While the rows kernel's reads are short (64 MB) the difference in
+  // start and end decides: 24 rows of 4 contexts of 1000: 15 / 20, 8-bit 16 / 24; of 4 of 300: 9 / 18; past the bound, of 4
+  // of 4000: 35 / 28. The host knows no lengths, so what the page table has room for is taken. The kernels round
+  // differently, so the choice is seen in the last bits of the outputs.
   const long long new_tokens = max_new > 0 ? max_new : (total_new + cache->batch - 1) / cache->batch;
   const long long rows = std::min(new_tokens * a.group, 1LL << 30);
   auto keys = [&](int per) {  // that units of `per` rows may read, all heads
@@ -486,7 +488,8 @@ int phantom_attn_paged(const phantom_paged_cache* cache, const void* q, long lon
   // Units of 16 rows read half as often but take longer for each tile: 16 rows of 8 contexts of 1000 20 us, in units of 8 rows
   // 16 (d = 64: 13.7, 12.8); 24 rows of the same 18 and 24 (14 and 19).
   const bool wide = a.int8 && rows > 8 && keys(8) > 160e3;
-  const bool few = rows <= (a.int8 ? 16 : 8) || (rows <= 32 && keys(wide ? 16 : 8) * 2 * a.d * (a.int8 ? 1 : 2) <= (double)(64 << 20));
+  const double reads = keys(wide ? 16 : 8) * 2 * a.d * (a.int8 ? 1 : 2);
+  const bool few = rows <= (a.int8 ? 16 : 8) || (rows <= 32 && reads <= (double)(64 << 20));
   const cudaError_t e = few ? launch_paged_attn_rows(a, dev.id, wide) : launch_paged_attn_chunk(a, dev.id);
   if (e != cudaSuccess) return cuda_fail(name, e);
   g_last_error.clear();

@@ -51,7 +51,7 @@ __device__ __forceinline__ int seq_index(const PagedSeqs& s, int tok) {
 __device__ __forceinline__ void zero_unowned(const PagedSeqs& s, void* o, int row, long long me, long long n) {
   const int first = min(max(s.cu_new[0], 0), s.total), last = max(min(max(s.cu_new[s.batch], 0), s.total), first);
   if (me == 0 && s.cu_new[0] != 0) atomicOr(s.status, PHANTOM_ATTN_STATUS_PAGE);
-  const long long lead = (long long)first * row, count = lead + (long long)(s.total - last) * row, skip = (long long)last * row - lead;
+  const long long lead = (long long)first * row, skip = (long long)last * row - lead, count = (long long)s.total * row - skip;
   for (long long i = me; i < count; i += n) static_cast<uint4*>(o)[i < lead ? i : i + skip] = make_uint4(0, 0, 0, 0);
 }
 
