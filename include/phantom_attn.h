@@ -205,7 +205,11 @@ int phantom_attn_get_kv_parts(void);
  * (total_new, heads, head_dim) arrays of a call hold one sequence after another (cu_new[0] = 0, cu_new[batch] = total_new).
  * Lengths, offsets and page ids are device data (32-bit): calls do not synchronise, and can be captured in a graph.
  * Sequences may share pages that are only read. What the table or the lengths give out of range is never followed: such
- * tokens are not written and read as zeros, and PHANTOM_ATTN_STATUS_PAGE is set in the device status word.
+ * tokens are not written and read as zeros, and PHANTOM_ATTN_STATUS_PAGE is set in the device status word. To the attention
+ * a token under a page id out of range is a key and a value of zeros, which counts; tokens past the room of a sequence's
+ * row of the table are not there, and the new tokens keep the positions that kv_lens gives them. Packed tokens from
+ * cu_new[batch] on are of no sequence (nothing wrong: a captured call may leave some unused), and so are those before a
+ * cu_new[0] above 0 (out of range): they are not written, read as zeros, and have zeros for output.
  *
  * Two kinds of cache: 16-bit (dtype PHANTOM_ATTN_F16 / BF16, values as they are), and 8-bit (PHANTOM_ATTN_I8) with fp32
  * scales: a vector x (one token, one head) is held as q = round(127 x / top), ties to even, and scale = top / 127 with
@@ -251,8 +255,12 @@ int phantom_attn_paged_read(const phantom_paged_cache* cache, void* k, void* v, 
  * PHANTOM_ATTN_I8. Query head h reads key head h / (q_heads / heads). New token i of n sees the first kv_len - n + i + 1
  * tokens of its sequence if causal, all of them otherwise; a token that sees none gets zeros. Scores are multiplied by
  * scale (0: 1 / sqrt(head_dim)). max_new is the largest number of new tokens of a sequence, as the caller expects it: a
- * hint that picks the kernel, not a limit (0: the average). 16-bit values cached within the length must be finite even
- * where the causal mask hides them; what lies past the length may be anything. */
+ * hint that picks the kernel, not a limit (0: the average). The kernels differ in speed and in how they round: a call with
+ * the same arguments repeats bit for bit, but the last bits of an output depend on max_new, on the other sequences of the
+ * batch, on table_width (the room, which the choice goes by) and on the GPU's number of SMs. 16-bit values cached within the
+ * length must be finite even where the causal mask hides them; a NaN or an infinite score among the keys reaches the rows
+ * that see it alone, and what lies past the length may be anything. 8-bit caches: a NaN reaches the rows that see it alone;
+ * a value vector whose scale is below 2^-126 of another's (2^-100 for one of zeros) may lose its weight. */
 int phantom_attn_paged(const phantom_paged_cache* cache, const void* q, long long q_token, long long q_head, void* o,
                        int total_new, int q_heads, int dtype, int causal, float scale, int max_new, void* stream);
 

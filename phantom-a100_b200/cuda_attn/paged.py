@@ -15,8 +15,10 @@ page size): a vector x of one token and head is held as round(127 x / top) and t
 are taken as they are (a slice of a fused projection, a pool that holds keys and values interleaved) where their strides
 are multiples of 16 bytes and d is contiguous.
 
-A page id, length or offset that is out of range is not followed: the token is not written, reads as zeros, and
-device_status() says so (bit 512).
+A page id, length or offset that is out of range is not followed: the token is not written, reads as zeros (to the
+attention, under a page id out of range, as a key and a value of zeros; past its row's room as no key at all), and
+device_status() says so (bit 512). Packed tokens after cu_new[-1] are of no sequence and get zeros, and so do those before
+cu_new[0], which should be 0.
 """
 from __future__ import annotations
 
@@ -54,9 +56,11 @@ def paged_attn(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, pa
     """Attention of the new tokens' queries (tokens, query heads, d) over all cached tokens of their sequences (append
     their keys and values first). Query head h reads key head h // (query heads / heads); new token i of n sees the first
     kv_lens[b] - n + i + 1 tokens if causal, else all kv_lens[b]; one that sees none gets zeros. `scale` of the scores: 1 /
-    sqrt(d) by default. `max_new`: the largest number of new tokens of a sequence, a hint that picks the kernel and changes
-    nothing else (default: the average). 16-bit values within kv_lens[b] must be finite, those that the causal mask hides
-    too; what the pages hold past it may be anything."""
+    sqrt(d) by default. `max_new`: the largest number of new tokens of a sequence, a hint that picks the kernel, and with it
+    the speed and the rounding (default: the average). The same call repeats bit for bit; the last bits also depend on the
+    other sequences of the batch and on page_table's width. 16-bit values within kv_lens[b] must be finite, those that the
+    causal mask hides too; a NaN among the keys, or in an int8 cache, reaches the rows that see it alone. What the pages
+    hold past kv_lens[b] may be anything."""
     if scale is not None and not 0.0 < abs(ctypes.c_float(scale).value) < float("inf"):
         raise RuntimeError(f"paged_attn: scale must be finite and not zero in float32 (got {scale})")
     return _ext().paged_attn(q, k_cache, v_cache, page_table, kv_lens, cu_new, k_scale, v_scale, causal, max_new,

@@ -29,7 +29,7 @@ def cut(tmp_path_factory):
     (top / "include").mkdir()
     (top / "include" / "phantom_attn.h").write_text(text(CSRC, "..", "..", "include", "phantom_attn.h"))
     rows = re.search(r"template <int NT, int BN>\nstruct RowBlocks \{.*?\n\};\n", text(CSRC, "attn_paged.cu"), re.S).group()
-    tokens = re.search(r"struct TokenBlocks \{.*?\n\};\n", text(CSRC, "attn_paged_tc_sm100.cu"), re.S).group()
+    tokens = re.search(r"struct (?:alignas\(16\) )?TokenBlocks \{.*?\n\};\n", text(CSRC, "attn_paged_tc_sm100.cu"), re.S).group()
     (src / "blocks.h").write_text("constexpr int BN = 128;\n" + rows.replace("BN", "B_N") + tokens)
     (src / "paged_cut.cpp").write_text(text(HERE, "harness", "paged_cut.cpp"))
     exe = str(top / "cut")
